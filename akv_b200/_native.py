@@ -21,6 +21,8 @@ GATHER_OUT64, GATHER_LITERAL, GATHER_SEG64 = 1, 2, 4
 DROP_RING_UNDERFLOW, DROP_RING_OVERFLOW, DROP_BAD_RANGE, DROP_NO_ACTIVE = 1, 2, 4, 8
 DROP_BAD_PAGE = 16
 REPOSITION_BULK_V = 1
+SLOTS_RING_UNDERFLOW, SLOTS_CAPACITY, SLOTS_BAD_REQUEST = 1, 2, 4
+SLOTS_BAD_PAGE, SLOTS_BAD_PARENT = 8, 16
 
 DTYPE_CODE = {torch.float16: AKV_F16, torch.bfloat16: AKV_BF16, torch.float32: AKV_F32}
 
@@ -104,6 +106,15 @@ SIGNATURES = {
         _I32, _I32, _I32, _P, _I32, _P, _I32, _P, _P, _P, _P, _I64, _I64, _P, _P, _P,
     ],
     "akv_decode_attention_ctas_per_sm": [_I32, _I32],
+    "akv_map_slots": [
+        _P, _I64, _I64, _I64, _P, _I32, _P, _I32, _P, _I32, _I32, _I32, _P, _P, _I64, _P, _I32,
+        _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _I32, _P,
+    ],
+    "akv_qk_norm_rope": [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I32, _I32, _I32, _I32, _I32,
+        _P, _P, _I32, ctypes.c_float, _P, _I32, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64,
+        _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I32, _P, _P,
+    ],
     "akv_context_attention_query_block": [],
     "akv_context_attention": [
         _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P,
@@ -161,6 +172,17 @@ def stream_of(device) -> ctypes.c_void_p:
             index = d.index if d.index is not None else torch.cuda.current_device()
             return ctypes.c_void_p(_raw_stream(index))
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def launch(index: int, fn, *args) -> int:
+    """``fn(*args, stream)`` on the current torch stream of CUDA device
+    ``index``, which is made the current device for the call if it is not
+    (a kernel must be launched from its stream's device)."""
+    if torch.cuda.current_device() == index:
+        return fn(*args, _raw_stream(index) if _raw_stream is not None
+                  else torch.cuda.current_stream(index).cuda_stream)
+    with torch.cuda.device(index):
+        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
 
 
 def check(status: int, what: str) -> None:

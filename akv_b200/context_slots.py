@@ -1,0 +1,149 @@
+"""Slot maps of a batch's new tokens, built on the device from its lengths (C
+ABI ``akv_map_slots``).
+
+The reference's scheduler allocates the slots of a forward's new tokens and
+writes them into ``req_to_token`` from Python
+(akv/system/sglang.patch:3133-3180).  ``SlotMapper.run`` does it in one launch
+for device-resident lengths and a device free list (``FreeSlotRing``, the one
+the Drop pushes its freed slots on): the slot and the position of every new
+token, the row entries, and, where asked, block tables for a paged reader and
+the ancestor masks of drafted token trees for ``context_tree.TreeAttention``.
+
+A verification step lends its pages (``commit=False``): the ring keeps them,
+and the next call gives the same ones out again, so rejected tokens cost
+nothing.  A prompt chunk or a plain decode step takes them (``commit=True``).
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _native
+
+TREE_NODES = 64  # new tokens per request with a tree: one 64-bit mask word each
+
+
+@dataclass
+class SlotMap:
+    """Device views of one call (the mapper's buffers: the next call
+    overwrites them).  New tokens lie in request order, request b's in
+    [new_offsets[b], new_offsets[b + 1])."""
+
+    new_offsets: torch.Tensor   # int32 [batch + 1]
+    slots: torch.Tensor         # int32 [max_new_tokens]; -1: none given out
+    positions: torch.Tensor     # int32 [max_new_tokens]
+    tree_mask: torch.Tensor | None  # int64 [max_new_tokens], with parents
+    block_table: torch.Tensor | None
+    totals: torch.Tensor        # int32 [2]: new tokens, pages taken or lent
+    status: torch.Tensor        # int32 [1]: AKV_SLOTS_* bits
+
+    ERRORS = {
+        _native.SLOTS_RING_UNDERFLOW: "not enough free pages in the ring",
+        _native.SLOTS_CAPACITY: "more new tokens than max_new_tokens",
+        _native.SLOTS_BAD_REQUEST: "a request's row or lengths are out of range",
+        _native.SLOTS_BAD_PAGE: "a row's last slot is not at its offset of a page",
+        _native.SLOTS_BAD_PARENT: "a draft token's parent is not an earlier token",
+    }
+
+    def check(self):
+        """Raise RuntimeError if the call set a status bit (synchronises)."""
+        bits = int(self.status.item())
+        if bits:
+            why = "; ".join(msg for bit, msg in self.ERRORS.items() if bits & bit)
+            raise RuntimeError(f"slot map: {why}")
+
+
+class SlotMapper:
+    """Outputs are allocated once, for up to ``max_batch`` requests with
+    ``max_new_tokens`` new tokens in all; a call allocates nothing, so it can
+    be captured in a CUDA graph.  Calls of one mapper, replays of its graphs
+    among them, share its buffers and must not overlap on the device."""
+
+    def __init__(self, max_batch, max_new_tokens, device, *, page_size=1):
+        if page_size != 1 and (page_size < 4 or page_size > 128 or page_size & (page_size - 1)):
+            raise ValueError("page_size must be 1 or a power of two from 4 to 128")
+        if not 0 < max_batch <= 65535 or not 0 <= max_new_tokens < 2**31:
+            raise ValueError("slot maps hold 1 to 65535 requests and fewer than 2^31 new tokens")
+        device = torch.device(device)
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.device, self._index = device, device.index
+        self.max_batch, self.max_new_tokens = int(max_batch), int(max_new_tokens)
+        self.page_size = int(page_size)
+
+        def vector(n, dtype=torch.int32):
+            return torch.zeros(n, dtype=dtype, device=device)
+
+        self._offsets = vector(self.max_batch + 1)
+        self._slots, self._positions = vector(self.max_new_tokens), vector(self.max_new_tokens)
+        self._mask = vector(self.max_new_tokens, torch.int64)
+        self._totals, self._status, self._work = vector(2), vector(1), vector(2)
+
+    def run(self, req_to_token, row_ids, raw_lens, new_lens, ring, *, next_positions=None,
+            parents=None, block_table=None, commit=True) -> SlotMap:
+        """``req_to_token`` int32 [rows, columns]; ``row_ids``, ``raw_lens`` (columns
+        in use) and ``new_lens`` int32 or int64 [batch]; ``ring`` a
+        ``FreeSlotRing`` of page ids (slots at page_size 1).
+        ``next_positions``: the position of each request's first new token,
+        the Drop's ``next_position`` (default ``raw_lens``).  ``parents``:
+        int32, one per new token, the parent's number in the request or -1
+        (at most 64 new tokens per request); positions then follow the
+        depth.  ``block_table``: int32 [>= batch, columns], filled with the
+        page ids of whole rows.  Two requests of one call must not share a
+        row, unless at most one of them has new tokens.  Failures that only
+        the device sees are bits of ``status`` (``SlotMap.check``)."""
+        batch, index = len(row_ids), self._index
+        if batch > self.max_batch:
+            raise ValueError("batch exceeds max_batch")
+        if req_to_token.dtype != torch.int32 or req_to_token.ndim != 2 or \
+                req_to_token.stride(1) != 1:
+            raise ValueError("req_to_token must be int32 [rows, columns] with unit last stride")
+        for name, t in (("row_ids", row_ids), ("raw_lens", raw_lens), ("new_lens", new_lens),
+                        ("next_positions", next_positions)):
+            if t is not None and (t.shape != (batch,) or not t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous vector of one entry per request")
+        tensors = [req_to_token, row_ids, raw_lens, new_lens, ring.ring, ring.state]
+        if next_positions is not None:
+            tensors.append(next_positions)
+        if parents is not None:
+            if parents.dtype != torch.int32 or parents.ndim != 1 or not parents.is_contiguous():
+                raise ValueError("parents must be a contiguous int32 vector")
+            if parents.numel() < self.max_new_tokens:
+                raise ValueError("parents must hold max_new_tokens entries")
+            tensors.append(parents)
+        table_stride = table_columns = 0
+        if block_table is not None:
+            if block_table.dtype != torch.int32 or block_table.ndim != 2 or \
+                    block_table.stride(1) != 1 or block_table.shape[0] < batch:
+                raise ValueError("block_table must be int32 [>= batch, columns] with unit last stride")
+            table_stride, table_columns = block_table.stride(0), block_table.shape[1]
+            tensors.append(block_table)
+        for t in tensors:
+            if t.get_device() != index:
+                raise ValueError("slot map tensors must be on the mapper's CUDA device")
+        is64 = _native.is64
+        flags = (is64(row_ids), is64(raw_lens), is64(new_lens),
+                 is64(next_positions) if next_positions is not None else 0)
+        result = SlotMap(self._offsets[: batch + 1], self._slots, self._positions,
+                         self._mask if parents is not None else None, block_table, self._totals,
+                         self._status)
+        if batch == 0:
+            for t in (result.new_offsets, result.totals, result.status):
+                t.zero_()
+            return result
+        status = _native.launch(
+            index, _native.lib.akv_map_slots,
+            req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[0],
+            req_to_token.shape[1], row_ids.data_ptr(), flags[0], raw_lens.data_ptr(), flags[1],
+            new_lens.data_ptr(), flags[2], batch, self.page_size, ring.ring.data_ptr(),
+            ring.state.data_ptr(), ring.capacity,
+            None if next_positions is None else next_positions.data_ptr(), flags[3],
+            None if parents is None else parents.data_ptr(), self.max_new_tokens,
+            self._offsets.data_ptr(), self._slots.data_ptr(), self._positions.data_ptr(),
+            self._mask.data_ptr(), None if block_table is None else block_table.data_ptr(),
+            table_stride, table_columns, self._totals.data_ptr(), self._status.data_ptr(),
+            self._work.data_ptr(), int(bool(commit)))
+        _native.check(status, "map_slots")
+        return result

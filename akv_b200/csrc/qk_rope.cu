@@ -1,0 +1,321 @@
+// Per-head RMS norms of Q and K, the position rotation and the store of K and
+// V into the paged cache, in one pass over a layer's projections.
+//
+// For every token and head row x of D elements (fp32 arithmetic, one rounding
+// to the tensors' type at the end):
+//   y = x * rsqrt(mean(x^2) + eps) * w              (skipped without weights)
+//   rotation of y's first R elements by the token's table row (cos | sin):
+//     halves (NEOX):      (y_i, y_{i+R/2}) -> (y_i c - y_{i+R/2} s, y_{i+R/2} c + y_i s)
+//     adjacent pairs:     the same with (y_{2i}, y_{2i+1})
+//   Q rows go to q_out, K rows to k_out and / or k_pool[slot], V rows are
+//   copied to v_pool[slot].  The reference runs its model's q_norm / k_norm,
+//   rotary module and set_kv_buffer one after the other (native SGLang
+//   modules around akv/system/sglang.patch:2437-2445).
+//
+// Bound: HBM.  Each element is read and written once.  A row is shared by
+// D / 16 lanes, each with two 16-byte pieces that rotate into one another
+// (elements [8j, 8j + 8) and [R/2 + 8j, ..) with halves, [16j, 16j + 16) with
+// pairs), so the rotation needs no exchange and the norm's sum is log2(D/16)
+// shuffles.  A lane keeps its 8 cos, 8 sin and 16 weights in registers over
+// kRows rows of its token, all of which it requests before it uses the first.
+
+#include "common.cuh"
+
+namespace akv {
+namespace {
+
+constexpr int kRopeThreads = 256;
+
+struct RopeArgs {
+  const void* q;
+  long long q_st, q_sh;
+  const void* k;
+  long long k_st, k_sh;
+  const void* v;
+  long long v_st, v_sh;
+  void* q_out;
+  long long qo_st, qo_sh;
+  void* k_out;
+  long long ko_st, ko_sh;
+  void* k_pool;
+  long long kp_ss, kp_sh;
+  void* v_pool;
+  long long vp_ss, vp_sh;
+  const void* q_weight;
+  const void* k_weight;
+  int weight_f32;
+  float eps;
+  const void* positions;
+  int positions_is64;
+  const void* slots;
+  int slots_is64;
+  const void* table;
+  int table_dtype;
+  long long table_stride, max_position, num_slots;
+  long long tokens;
+  int hq, hkv, dim, rotary;
+  int q_units, k_units, units;  // units of kRows rows: Q's, K's (and V's), all
+  int* error_flag;
+};
+
+// Eight consecutive elements, as fp32.
+template <typename T>
+struct Eight {
+  Vec16<T> v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = ld16(p + i * Vec16<T>::N);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) st16(p + i * Vec16<T>::N, v[i]);
+  }
+  __device__ __forceinline__ float get(int i) const {
+    return Elem<T>::to_f32(v[i / Vec16<T>::N].e[i % Vec16<T>::N]);
+  }
+  __device__ __forceinline__ void set(int i, float x) {
+    v[i / Vec16<T>::N].e[i % Vec16<T>::N] = Elem<T>::from_f32(x);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const void* base, long long at, float (&out)[8]) {
+  Eight<T> e;
+  e.load(static_cast<const T*>(base) + at);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) out[i] = e.get(i);
+}
+
+// T: element type; LANES: lanes per row (D / 16 rounded up to a power of
+// two); NEOX: halves or adjacent pairs; ROWS: rows per lane group.
+template <typename T, int LANES, bool NEOX, int ROWS>
+__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeArgs a) {
+  const long long group =
+      ((long long)blockIdx.x * kRopeThreads + threadIdx.x) / LANES;
+  const int j = threadIdx.x % LANES;
+  const long long token = group / a.units;
+  const int unit = (int)(group - token * a.units);
+  if (token >= a.tokens) return;  // whole lane groups leave together
+  // Shuffles stay inside the lane group, whose lanes all take the same path.
+  const unsigned lanes =
+      LANES == 32 ? 0xffffffffu
+                  : ((1u << (LANES & 31)) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
+  const int kind = unit < a.q_units ? 0 : unit < a.q_units + a.k_units ? 1 : 2;
+  const int first =
+      (kind == 0 ? unit : kind == 1 ? unit - a.q_units : unit - a.q_units - a.k_units) * ROWS;
+  const int heads = kind == 0 ? a.hq : a.hkv;
+  const bool live = 16 * j < a.dim;  // D / 16 need not be a power of two
+  const bool turned = 16 * j < a.rotary;
+  // This lane's two runs of eight elements.
+  const int e0 = NEOX && turned ? 8 * j : 16 * j;
+  const int e1 = NEOX && turned ? a.rotary / 2 + 8 * j : 16 * j + 8;
+
+  const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v);
+  const long long st = kind == 0 ? a.q_st : kind == 1 ? a.k_st : a.v_st;
+  const long long sh = kind == 0 ? a.q_sh : kind == 1 ? a.k_sh : a.v_sh;
+  src += token * st + first * sh;
+  Eight<T> x0[ROWS], x1[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+    if (live && first + r < heads) {
+      x0[r].load(src + r * sh + e0);
+      x1[r].load(src + r * sh + e1);
+    }
+
+  long long slot = -1;
+  if (kind != 0 && a.slots != nullptr) {
+    slot = ld_index(a.slots, token, a.slots_is64);
+    if (slot >= a.num_slots) {  // never touch memory outside the pools
+      if (a.error_flag) *a.error_flag = 1;
+      slot = -1;
+    }
+  }
+  long long pos = ld_index(a.positions, token, a.positions_is64);
+  if (pos < 0 || pos >= a.max_position) {
+    if (a.error_flag) *a.error_flag = 1;
+    pos = 0;
+    slot = -1;
+  }
+  if (kind == 2) {
+    if (slot < 0 || !live) return;
+    T* dst = static_cast<T*>(a.v_pool) + slot * a.vp_ss + first * a.vp_sh;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (first + r < heads) {
+        x0[r].store(dst + r * a.vp_sh + e0);
+        x1[r].store(dst + r * a.vp_sh + e1);
+      }
+    return;
+  }
+
+  float c[8], s[8];
+  if (turned) {
+    const long long at = pos * a.table_stride + 8 * j;
+    if (a.table_dtype == AKV_F32) {
+      load8<float>(a.table, at, c);
+      load8<float>(a.table, at + a.rotary / 2, s);
+    } else if (a.table_dtype == AKV_BF16) {
+      load8<__nv_bfloat16>(a.table, at, c);
+      load8<__nv_bfloat16>(a.table, at + a.rotary / 2, s);
+    } else {
+      load8<__half>(a.table, at, c);
+      load8<__half>(a.table, at + a.rotary / 2, s);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      c[i] = 1.f;
+      s[i] = 0.f;
+    }
+  }
+  const void* weight = kind == 0 ? a.q_weight : a.k_weight;
+  float w0[8], w1[8];
+  if (weight != nullptr && live) {
+    if (a.weight_f32) {
+      load8<float>(weight, e0, w0);
+      load8<float>(weight, e1, w1);
+    } else {
+      load8<T>(weight, e0, w0);
+      load8<T>(weight, e1, w1);
+    }
+  }
+
+  T* out = static_cast<T*>(kind == 0 ? a.q_out : a.k_out);
+  if (out != nullptr)
+    out += kind == 0 ? token * a.qo_st + first * a.qo_sh : token * a.ko_st + first * a.ko_sh;
+  const long long oh = kind == 0 ? a.qo_sh : a.ko_sh;
+  T* pool = kind == 1 && slot >= 0 && a.k_pool != nullptr
+                ? static_cast<T*>(a.k_pool) + slot * a.kp_ss + first * a.kp_sh
+                : nullptr;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if (first + r >= heads) break;
+    float y0[8], y1[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y0[i] = live ? x0[r].get(i) : 0.f;
+      y1[i] = live ? x1[r].get(i) : 0.f;
+    }
+    if (weight != nullptr) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += y0[i] * y0[i] + y1[i] * y1[i];
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(lanes, ss, d);
+      const float inv = rsqrtf(ss / (float)a.dim + a.eps);
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y0[i] *= inv * w0[i];
+          y1[i] *= inv * w1[i];
+        }
+      }
+    }
+    if (!live) continue;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (NEOX) {
+        x0[r].set(i, y0[i] * c[i] - y1[i] * s[i]);
+        x1[r].set(i, y1[i] * c[i] + y0[i] * s[i]);
+      } else if (i < 4) {  // pairs 0-3 of the lane's run in y0, 4-7 in y1
+        x0[r].set(2 * i, y0[2 * i] * c[i] - y0[2 * i + 1] * s[i]);
+        x0[r].set(2 * i + 1, y0[2 * i + 1] * c[i] + y0[2 * i] * s[i]);
+        x1[r].set(2 * i, y1[2 * i] * c[4 + i] - y1[2 * i + 1] * s[4 + i]);
+        x1[r].set(2 * i + 1, y1[2 * i + 1] * c[4 + i] + y1[2 * i] * s[4 + i]);
+      }
+    }
+    if (out != nullptr) {
+      x0[r].store(out + r * oh + e0);
+      x1[r].store(out + r * oh + e1);
+    }
+    if (pool != nullptr) {
+      x0[r].store(pool + r * a.kp_sh + e0);
+      x1[r].store(pool + r * a.kp_sh + e1);
+    }
+  }
+}
+
+template <typename T, int LANES, bool NEOX>
+int launch_rope(RopeArgs& a, cudaStream_t stream) {
+  constexpr int ROWS = sizeof(T) == 4 ? 2 : 4;
+  a.q_units = (a.hq + ROWS - 1) / ROWS;
+  a.k_units = (a.hkv + ROWS - 1) / ROWS;
+  a.units = a.q_units + a.k_units * (a.v != nullptr ? 2 : 1);
+  const long long threads = a.tokens * a.units * LANES;
+  const long long blocks = (threads + kRopeThreads - 1) / kRopeThreads;
+  if (blocks > INT32_MAX) return AKV_ERR_INVALID;
+  qk_norm_rope_kernel<T, LANES, NEOX, ROWS><<<(unsigned)blocks, kRopeThreads, 0, stream>>>(a);
+  return launch_status();
+}
+
+template <typename T, int LANES>
+int launch_rope_style(RopeArgs& a, int neox, cudaStream_t stream) {
+  return neox ? launch_rope<T, LANES, true>(a, stream) : launch_rope<T, LANES, false>(a, stream);
+}
+
+template <typename T>
+int launch_rope_lanes(RopeArgs& a, int neox, cudaStream_t stream) {
+  if (a.dim <= 32) return launch_rope_style<T, 2>(a, neox, stream);
+  if (a.dim <= 64) return launch_rope_style<T, 4>(a, neox, stream);
+  if (a.dim <= 128) return launch_rope_style<T, 8>(a, neox, stream);
+  if (a.dim <= 256) return launch_rope_style<T, 16>(a, neox, stream);
+  return launch_rope_style<T, 32>(a, neox, stream);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace akv
+
+extern "C" int akv_qk_norm_rope(
+    const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k,
+    int64_t k_stride_token, int64_t k_stride_head, const void* v, int64_t v_stride_token,
+    int64_t v_stride_head, int32_t dtype, int64_t tokens, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim, int32_t is_neox_style,
+    const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+    const void* positions, int32_t positions_is64, const void* cos_sin_cache, int32_t cache_dtype,
+    int64_t cache_stride, int64_t max_position, void* q_out, int64_t q_out_stride_token,
+    int64_t q_out_stride_head, void* k_out, int64_t k_out_stride_token, int64_t k_out_stride_head,
+    void* k_pool, int64_t k_pool_stride_slot, int64_t k_pool_stride_head, void* v_pool,
+    int64_t v_pool_stride_slot, int64_t v_pool_stride_head, int64_t num_slots, const void* slots,
+    int32_t slots_is64, int32_t* error_flag, void* stream) {
+  AKV_NVTX_RANGE("akv_qk_norm_rope");
+  using namespace akv;
+  if (tokens < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      head_dim < 16 || head_dim > 512 || head_dim % 16 || rotary_dim <= 0 ||
+      rotary_dim > head_dim || rotary_dim % 16 || dtype < AKV_F16 || dtype > AKV_F32 ||
+      cache_dtype < AKV_F16 || cache_dtype > AKV_F32 ||
+      ((q_weight || k_weight) && weight_dtype != dtype && weight_dtype != AKV_F32))
+    return AKV_ERR_INVALID;
+  if (tokens == 0) return AKV_OK;
+  if (!q || !k || !q_out || !positions || !cos_sin_cache || max_position <= 0 || (!k_out && !k_pool) ||
+      (k_pool && (!v || !v_pool || !slots || num_slots <= 0)) || (v && !k_pool))
+    return AKV_ERR_INVALID;
+  const int64_t vec = dtype == AKV_F32 ? 4 : 8;  // elements of a 16-byte access
+  const int64_t cache_vec = cache_dtype == AKV_F32 ? 4 : 8;
+  const int64_t strides[] = {q_stride_token,     q_stride_head,      k_stride_token,
+                             k_stride_head,      v_stride_token,     v_stride_head,
+                             q_out_stride_token, q_out_stride_head,  k_out_stride_token,
+                             k_out_stride_head,  k_pool_stride_slot, k_pool_stride_head,
+                             v_pool_stride_slot, v_pool_stride_head};
+  for (int64_t s : strides)
+    if (s % vec) return AKV_ERR_INVALID;
+  const void* bases[] = {q,      k,        v,        q_out,        k_out,
+                         k_pool, v_pool,   q_weight, k_weight,     cos_sin_cache};
+  for (const void* p : bases)
+    if (!aligned16(p)) return AKV_ERR_INVALID;
+  if (cache_stride % cache_vec) return AKV_ERR_INVALID;
+  RopeArgs a{q, q_stride_token, q_stride_head, k, k_stride_token, k_stride_head, v,
+             v_stride_token, v_stride_head, q_out, q_out_stride_token, q_out_stride_head, k_out,
+             k_out_stride_token, k_out_stride_head, k_pool, k_pool_stride_slot,
+             k_pool_stride_head, v_pool, v_pool_stride_slot, v_pool_stride_head, q_weight,
+             k_weight, weight_dtype == AKV_F32, eps, positions, positions_is64, slots, slots_is64,
+             cos_sin_cache, cache_dtype, cache_stride, max_position, num_slots, tokens,
+             num_q_heads, num_kv_heads, head_dim, rotary_dim, 0, 0, 0, error_flag};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case AKV_F16: return launch_rope_lanes<__half>(a, is_neox_style, s);
+    case AKV_BF16: return launch_rope_lanes<__nv_bfloat16>(a, is_neox_style, s);
+    default: return launch_rope_lanes<float>(a, is_neox_style, s);
+  }
+}

@@ -1,0 +1,309 @@
+// Slot maps, positions, draft-tree masks and block tables of a batch's new
+// tokens, built on the device from the requests' lengths.
+//
+// Request b has L = raw_lens[b] tokens in columns [0, L) of its row of
+// req_to_token and receives n = new_lens[b] more.  With pages of p = 2^k
+// token slots (token t of a request at offset t % p of its page),
+//
+//   need_b = ceil((L + n) / p) - ceil(L / p)       pages the new tokens open
+//   base_b = sum of need over the requests before b
+//   new token t in [L, L + n):
+//     page = row[L - 1] / p                        if t / p < ceil(L / p)
+//            ring[(head + base_b + t / p - ceil(L / p)) % capacity]  otherwise
+//     slot = page * p + t % p,  row[t] = slot
+//   position = next_position[b] + depth of the node (with a draft tree)
+//                               + t - L              (without)
+//   mask     = own bit | mask of the parent (64 nodes at most per request)
+//
+// The reference builds these on the host (the scheduler allocates slots and
+// writes req_to_token from Python, akv/system/sglang.patch:3133-3180); the
+// reading side's metadata is page_table.cu.
+//
+// Bound: latency.  The kernel moves about 12-24 bytes per token and 8 per
+// table entry, so one launch with two dependent load rounds is the floor.
+// Every block therefore sums the whole batch's lengths itself (a batch is a
+// few hundred loads from L2) instead of waiting for a scan kernel.
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace akv {
+namespace {
+
+constexpr int kSlotThreads = 256;
+constexpr int kTreeNodes = 64;
+
+struct SlotArgs {
+  int32_t* req_to_token;
+  int64_t row_stride, rows, columns;
+  const void* row_ids;
+  int row_ids_is64;
+  const void* raw_lens;
+  int raw_lens_is64;
+  const void* new_lens;
+  int new_lens_is64;
+  int batch;
+  int shift;  // log2(page size)
+  const int32_t* ring;
+  long long* ring_state;
+  int64_t ring_capacity;
+  const void* next_positions;  // null: the row length
+  int next_is64;
+  const int32_t* parents;      // null: no tree
+  int64_t capacity;            // new tokens the outputs hold
+  int32_t* new_offsets;
+  int32_t* slots;
+  int32_t* positions;
+  int64_t* tree_mask;
+  int32_t* block_table;
+  int64_t table_stride, table_columns;
+  int32_t* totals;             // {new tokens, pages}
+  int32_t* status;
+  unsigned* arrivals;
+  int commit;
+};
+
+struct Request {
+  long long len, fresh, row, need;
+  bool bad;
+};
+
+__device__ __forceinline__ Request load_request(const SlotArgs& a, int b) {
+  Request r;
+  r.row = ld_index(a.row_ids, b, a.row_ids_is64);
+  r.len = ld_index(a.raw_lens, b, a.raw_lens_is64);
+  r.fresh = ld_index(a.new_lens, b, a.new_lens_is64);
+  const long long end = r.len + r.fresh;
+  // A bad request takes part as one without new tokens.
+  r.bad = r.row < 0 || r.row >= a.rows || r.len < 0 || r.fresh < 0 || r.len > a.columns ||
+          r.fresh > a.columns || end > a.columns ||
+          (a.parents != nullptr && r.fresh > kTreeNodes) ||
+          (a.block_table != nullptr && ((end - 1) >> a.shift) >= a.table_columns);
+  if (r.bad) r.fresh = 0;
+  const long long up = (1ll << a.shift) - 1;
+  r.need = r.bad ? 0 : ((end + up) >> a.shift) - ((r.len + up) >> a.shift);
+  return r;
+}
+
+// Sums of one block over the batch, valid in every thread afterwards.
+struct Sums {
+  unsigned long long need, fresh, all_need, all_fresh;
+};
+
+__global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs a) {
+  __shared__ unsigned long long s_sum[4][kSlotThreads / 32];
+  __shared__ int s_bad;
+  __shared__ long long s_ring[2];
+  const int b = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Request me = load_request(a, b);
+  int32_t* row = a.req_to_token + (me.bad ? 0 : me.row) * a.row_stride;
+  const int p_mask = (1 << a.shift) - 1;
+  const long long old_pages = (me.len + p_mask) >> a.shift;
+  // The page the row ends in, if it ends inside one.
+  const bool partial = !me.bad && (me.len & p_mask) != 0;
+  const int last = partial ? row[me.len - 1] : 0;
+  if (tid == 0) {
+    s_bad = 0;
+    s_ring[0] = a.ring_state[0];
+    s_ring[1] = a.ring_state[1];
+  }
+  __syncthreads();
+  Sums s = {0, 0, 0, 0};
+  bool bad = false;
+  for (int i = tid; i < a.batch; i += kSlotThreads) {
+    const Request r = load_request(a, i);
+    s.all_need += r.need;
+    s.all_fresh += r.fresh;
+    if (i < b) {
+      s.need += r.need;
+      s.fresh += r.fresh;
+    }
+    bad |= r.bad;
+  }
+  if (bad) s_bad = 1;
+  s.need = warp_sum(s.need);
+  s.fresh = warp_sum(s.fresh);
+  s.all_need = warp_sum(s.all_need);
+  s.all_fresh = warp_sum(s.all_fresh);
+  if (lane == 0) {
+    s_sum[0][warp] = s.need;
+    s_sum[1][warp] = s.fresh;
+    s_sum[2][warp] = s.all_need;
+    s_sum[3][warp] = s.all_fresh;
+  }
+  __syncthreads();
+  s = Sums{0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < kSlotThreads / 32; ++w) {
+    s.need += s_sum[0][w];
+    s.fresh += s_sum[1][w];
+    s.all_need += s_sum[2][w];
+    s.all_fresh += s_sum[3][w];
+  }
+  const long long head = s_ring[0];
+  const bool short_ring = (long long)s.all_need > s_ring[1] - head;
+  const bool over = (long long)s.all_fresh > a.capacity;
+  const bool refused = short_ring || over;  // of the whole call: no slot is given out
+  // A row whose last slot does not sit at its offset of a page cannot go on.
+  const bool bad_page = partial && (last < 0 || (last & p_mask) != ((me.len - 1) & p_mask));
+  const bool give = !refused && !bad_page;
+  int st = 0;
+  if (me.bad) st |= AKV_SLOTS_BAD_REQUEST;
+  if (bad_page) st |= AKV_SLOTS_BAD_PAGE;
+
+  auto fresh_page = [&](long long k) {
+    return a.ring[(head + (long long)s.need + k) % a.ring_capacity];
+  };
+  const int start = blockIdx.x * kSlotThreads + tid, step = gridDim.x * kSlotThreads;
+  const long long next = a.next_positions ? ld_index(a.next_positions, b, a.next_is64) : me.len;
+  const long long out0 = (long long)s.fresh;
+
+  // New tokens.  With a tree they are one warp's work (64 nodes at most, two
+  // per lane): ancestors by pointer doubling, six rounds of mask |=
+  // mask[up], up = up[up] over shuffles, which is as quick for a chain of 64
+  // nodes as for a flat tree.
+  if (a.parents != nullptr) {
+    if (blockIdx.x == 0 && warp == 0 && me.fresh > 0) {
+      int up[2];
+      unsigned long long mask[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = lane + 32 * h;
+        up[h] = -1;
+        mask[h] = 1ull << i;
+        if (i < me.fresh && out0 + i < a.capacity) {
+          up[h] = a.parents[out0 + i];
+          if (up[h] < -1 || up[h] >= i) {  // not above the node: a root
+            st |= AKV_SLOTS_BAD_PARENT;
+            up[h] = -1;
+          }
+        }
+      }
+#pragma unroll
+      for (int round = 0; round < 6; ++round) {
+        int nu[2];
+        unsigned long long nm[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int src = up[h] & 31;
+          const unsigned long long m0 = __shfl_sync(0xffffffffu, mask[0], src);
+          const unsigned long long m1 = __shfl_sync(0xffffffffu, mask[1], src);
+          const int u0 = __shfl_sync(0xffffffffu, up[0], src);
+          const int u1 = __shfl_sync(0xffffffffu, up[1], src);
+          const bool hi = up[h] >= 32, root = up[h] < 0;
+          nm[h] = root ? mask[h] : mask[h] | (hi ? m1 : m0);
+          nu[h] = root ? -1 : (hi ? u1 : u0);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mask[h] = nm[h];
+          up[h] = nu[h];
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = lane + 32 * h;
+        if (i >= me.fresh || out0 + i >= a.capacity) continue;
+        const long long t = me.len + i, g = t >> a.shift;
+        int slot = -1;
+        if (give) {
+          const int page = g < old_pages ? last >> a.shift : fresh_page(g - old_pages);
+          slot = (page << a.shift) | (int)(t & p_mask);
+          row[t] = slot;
+        }
+        a.slots[out0 + i] = slot;
+        a.positions[out0 + i] = (int32_t)(next + __popcll(mask[h]) - 1);
+        a.tree_mask[out0 + i] = (int64_t)mask[h];
+      }
+    }
+  } else {
+    for (long long i = start; i < me.fresh && out0 + i < a.capacity; i += step) {
+      const long long t = me.len + i, g = t >> a.shift;
+      int slot = -1;
+      if (give) {
+        const int page = g < old_pages ? last >> a.shift : fresh_page(g - old_pages);
+        slot = (page << a.shift) | (int)(t & p_mask);
+        row[t] = slot;
+      }
+      a.slots[out0 + i] = slot;
+      a.positions[out0 + i] = (int32_t)(next + i);
+    }
+  }
+
+  // Block table: the pages of [0, L) from the row, the fresh ones from the
+  // ring (the row's new columns are being written by this launch).
+  if (a.block_table != nullptr && give && !me.bad) {
+    int32_t* out = a.block_table + (long long)b * a.table_stride;
+    const long long pages = old_pages + me.need;
+    for (long long g = start; g < pages; g += step)
+      out[g] = g < old_pages ? row[g << a.shift] >> a.shift : fresh_page(g - old_pages);
+  }
+
+  if (blockIdx.x == 0 && tid == 0) {
+    a.new_offsets[b] = (int32_t)(over ? 0 : s.fresh);
+    if (b == a.batch - 1) {
+      a.new_offsets[a.batch] = (int32_t)(over ? 0 : s.all_fresh);
+      a.totals[0] = (int32_t)(over ? 0 : s.all_fresh);
+      a.totals[1] = (int32_t)(refused ? 0 : s.all_need);
+      if (short_ring) st |= AKV_SLOTS_RING_UNDERFLOW;
+      if (over) st |= AKV_SLOTS_CAPACITY;
+    }
+  }
+  // Status bits gather in arrivals[1] and the last block publishes them (so
+  // a call leaves its own status, not a sum over calls) and, with commit,
+  // takes the pages: every block has read the ring's head by then.
+  if (st) atomicOr(a.arrivals + 1, (unsigned)st);
+  __syncthreads();
+  if (tid == 0) {
+    __threadfence();
+    const unsigned blocks = gridDim.x * gridDim.y;
+    if (atomicInc(a.arrivals, blocks - 1) == blocks - 1) {
+      *a.status = (int32_t)atomicExch(a.arrivals + 1, 0u);
+      if (a.commit && !refused) a.ring_state[0] = head + (long long)s.all_need;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace akv
+
+extern "C" int akv_map_slots(
+    int32_t* req_to_token, int64_t row_stride, int64_t rows, int64_t columns, const void* row_ids,
+    int32_t row_ids_is64, const void* raw_lens, int32_t raw_lens_is64, const void* new_lens,
+    int32_t new_lens_is64, int32_t batch, int32_t page_size, const int32_t* ring,
+    int64_t* ring_state, int64_t ring_capacity, const void* next_positions, int32_t next_is64,
+    const int32_t* parents, int64_t capacity, int32_t* new_offsets, int32_t* slots,
+    int32_t* positions, int64_t* tree_mask, int32_t* block_table, int64_t table_stride,
+    int64_t table_columns, int32_t* totals, int32_t* status, uint32_t* workspace, int32_t commit,
+    void* stream) {
+  AKV_NVTX_RANGE("akv_map_slots");
+  using namespace akv;
+  if (batch < 0 || batch > 65535 || rows < 0 || columns < 0 || row_stride < columns ||
+      ring_capacity <= 0 || capacity < 0 || capacity > INT32_MAX || page_size <= 0 ||
+      page_size > 128 || (page_size & (page_size - 1)) || page_size == 2 ||
+      (block_table && (table_columns < 0 || table_stride < table_columns)))
+    return AKV_ERR_INVALID;
+  if (batch == 0) return AKV_OK;
+  if (!req_to_token || !row_ids || !raw_lens || !new_lens || !ring || !ring_state ||
+      !new_offsets || !totals || !status || !workspace || (capacity > 0 && (!slots || !positions)) ||
+      (parents && capacity > 0 && !tree_mask))
+    return AKV_ERR_INVALID;
+  int shift = 0;
+  while ((1 << shift) < page_size) ++shift;
+  SlotArgs a{req_to_token, row_stride, rows, columns, row_ids, row_ids_is64, raw_lens,
+             raw_lens_is64, new_lens, new_lens_is64, batch, shift, ring,
+             reinterpret_cast<long long*>(ring_state), ring_capacity, next_positions, next_is64,
+             parents, capacity, new_offsets, slots, positions, tree_mask, block_table,
+             table_stride, table_columns, totals, status, workspace, commit};
+  // Blocks per request: enough for about six per SM over the batch, no more
+  // than the request's share of tokens or its table row can use.
+  const long long longest =
+      std::max<long long>(parents ? 1 : capacity, block_table ? table_columns : 1);
+  const long long want = (longest + 4 * kSlotThreads - 1) / (4 * kSlotThreads);
+  const long long fit = std::max(1, kNumSMs * 6 / batch);
+  const dim3 grid((unsigned)std::max<long long>(1, std::min(want, fit)), batch);
+  map_slots_kernel<<<grid, kSlotThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return launch_status();
+}

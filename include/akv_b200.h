@@ -39,6 +39,13 @@ extern "C" {
 #define AKV_DROP_NO_ACTIVE 8      /* Reposition of a request with no token   */
 #define AKV_DROP_BAD_PAGE 16      /* page mode: a row breaks the page layout */
 
+/* Device-side status bits written by akv_map_slots into `status`. */
+#define AKV_SLOTS_RING_UNDERFLOW 1 /* not enough free pages in the ring       */
+#define AKV_SLOTS_CAPACITY 2       /* more new tokens than the outputs hold   */
+#define AKV_SLOTS_BAD_REQUEST 4    /* a row or a length out of range          */
+#define AKV_SLOTS_BAD_PAGE 8       /* a row's last slot is not at its offset  */
+#define AKV_SLOTS_BAD_PARENT 16    /* a draft node's parent is not before it  */
+
 /* Element types. */
 #define AKV_F16 0
 #define AKV_BF16 1
@@ -654,6 +661,86 @@ int akv_occurrence_advance_indices(const akv_advance_in* in, akv_advance_out* ou
 int64_t akv_gather_slots_chunk(void);
 int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chunks,
                      const int32_t* indices, int32_t* error_flag, void* stream);
+
+/*
+ * Slot maps, positions, draft-tree masks and block tables of the new tokens
+ * of a batch, from the requests' lengths, in one launch.  The reference
+ * allocates and writes them from the scheduler's Python
+ * (akv/system/sglang.patch:3133-3180).
+ *
+ * Request b owns row row_ids[b] of req_to_token (DEVICE int32 [rows,
+ * columns], row stride row_stride); its raw_lens[b] tokens fill the row's
+ * first columns and it receives new_lens[b] more.  page_size (1, or a power
+ * of two from 4 to 128): token t sits at offset t % page_size of its page.
+ * New tokens continue the row's last page, then take pages from the free ring
+ * (akv_drop_compact's: ring[ring_capacity], ring_state = {head, tail}) in
+ * request order.  With `commit` the ring's head moves past them; without it
+ * they are lent: the next call gives out the same pages.
+ *
+ * Outputs, new tokens in request order: new_offsets int32 [batch + 1]; slots
+ * and positions int32 [capacity]; the row's new columns; with parents, tree_mask
+ * int64 [capacity]: bit j of a token's word is set for itself and its
+ * ancestors j (token numbers of the request).  parents: int32, -1 for a root,
+ * otherwise an earlier token of the request; at most 64 new tokens per
+ * request.  A position is next_positions[b] (NULL: raw_lens[b]) plus the
+ * token's depth in the tree, or its number without one.  block_table (NULL:
+ * none) int32 [batch, table_columns]: the page ids of the row's pages, the new
+ * ones included; entries behind a request's last page are left as they
+ * were.  It describes whole rows: tokens dropped from a row are not left out.
+ * totals int32 [2] = {new tokens, pages taken}.
+ *
+ * status (int32): AKV_SLOTS_* bits of this call.  RING_UNDERFLOW and CAPACITY
+ * refuse the whole call (slots -1; rows, block table and ring untouched);
+ * BAD_REQUEST treats that request as one without new tokens; BAD_PAGE leaves
+ * that request's slots -1 and its row and block table untouched; BAD_PARENT
+ * makes the token a root.  Two requests of a call must not share a row, unless
+ * at most one of them has new tokens.  workspace: DEVICE uint32 [2], zero before the first call and
+ * left zero by every call; calls that share it must not overlap.
+ */
+int akv_map_slots(int32_t* req_to_token, int64_t row_stride, int64_t rows, int64_t columns,
+                  const void* row_ids, int32_t row_ids_is64, const void* raw_lens,
+                  int32_t raw_lens_is64, const void* new_lens, int32_t new_lens_is64,
+                  int32_t batch, int32_t page_size, const int32_t* ring, int64_t* ring_state,
+                  int64_t ring_capacity, const void* next_positions, int32_t next_is64,
+                  const int32_t* parents, int64_t capacity, int32_t* new_offsets, int32_t* slots,
+                  int32_t* positions, int64_t* tree_mask, int32_t* block_table,
+                  int64_t table_stride, int64_t table_columns, int32_t* totals, int32_t* status,
+                  uint32_t* workspace, int32_t commit, void* stream);
+
+/*
+ * Per-head RMS norms of Q and K, the position rotation, and the store of K
+ * and V into the cache, in one pass.  In the reference's runtime these are
+ * the model's norm and rotary modules and the pool's set_kv_buffer, called
+ * one after another (around akv/system/sglang.patch:2437-2445).
+ *
+ * q [tokens, num_q_heads, head_dim], k and v [tokens, num_kv_heads,
+ * head_dim], pools [num_slots, num_kv_heads, head_dim], all of `dtype`, unit
+ * last stride, strides in elements.  Per row: y = x * rsqrt(mean(x^2) + eps)
+ * * weight (weight NULL: y = x), then elements [0, rotary_dim) rotated by
+ * the position's table row (cos | sin) as akv_reposition_kv_layers rotates
+ * them; fp32 arithmetic, rounded once.  Q rows go to q_out (may be q); K
+ * rows to k_out (may be k; NULL: not) and, with k_pool, to
+ * k_pool[slots[token]]; V rows are copied to v_pool[slots[token]].  A
+ * negative slot marks a padding token, which is not stored.  A slot at or
+ * past num_slots, or a position outside [0, max_position) (rotated as
+ * position 0), is not stored and sets *error_flag (NULL: not reported).
+ * weight_dtype: `dtype` or AKV_F32.  head_dim and rotary_dim: multiples of
+ * 16, head_dim at most 512; every base address and stride a multiple of 16
+ * bytes.  Two tokens must not have the same slot.
+ */
+int akv_qk_norm_rope(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k,
+                     int64_t k_stride_token, int64_t k_stride_head, const void* v,
+                     int64_t v_stride_token, int64_t v_stride_head, int32_t dtype,
+                     int64_t tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t rotary_dim, int32_t is_neox_style, const void* q_weight,
+                     const void* k_weight, int32_t weight_dtype, float eps,
+                     const void* positions, int32_t positions_is64, const void* cos_sin_cache,
+                     int32_t cache_dtype, int64_t cache_stride, int64_t max_position, void* q_out,
+                     int64_t q_out_stride_token, int64_t q_out_stride_head, void* k_out,
+                     int64_t k_out_stride_token, int64_t k_out_stride_head, void* k_pool,
+                     int64_t k_pool_stride_slot, int64_t k_pool_stride_head, void* v_pool,
+                     int64_t v_pool_stride_slot, int64_t v_pool_stride_head, int64_t num_slots,
+                     const void* slots, int32_t slots_is64, int32_t* error_flag, void* stream);
 
 #ifdef __cplusplus
 }
