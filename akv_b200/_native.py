@@ -115,6 +115,12 @@ SIGNATURES = {
         _P, _P, _I32, ctypes.c_float, _P, _I32, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64,
         _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I32, _P, _P,
     ],
+    "akv_tree_attention_units": [_I32],
+    "akv_tree_attention": [
+        _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _P, _I64, _P,
+        ctypes.c_float, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, _P, _P, _P, _I64, _I64, _P, _P,
+        _P,
+    ],
     "akv_context_attention_query_block": [],
     "akv_context_attention": [
         _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P,
@@ -131,6 +137,7 @@ RESTYPES = {
     "akv_compile_layouts_workspace_bytes": _I64,
     "akv_compile_layouts_batch_bytes": _I64,
     "akv_decode_attention_ctas_per_sm": _I32,
+    "akv_tree_attention_units": _I32,
     "akv_context_attention_query_block": _I64,
     "akv_active_slots_chunk": _I64,
     "akv_gather_slots_chunk": _I64,

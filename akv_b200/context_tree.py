@@ -1,0 +1,240 @@
+"""Attention of drafted token trees over the paged cache (C ABI
+``akv_tree_attention``).
+
+Speculative decoding verifies, in one forward, a tree of drafted tokens per
+request: each sees the request's cached keys and, among the drafted tokens,
+itself and its ancestors.  The reference's runtime hands such a step to its
+native backends with a dense mask over all keys; ``TreeAttention`` takes the
+same paged inputs as ``DecodeAttention`` plus the drafted tokens' slots and one
+64-bit mask word per token (``context_slots.SlotMapper`` makes both).
+
+Like ``DecodeAttention``, ``plan`` cuts the batch into a work list on the host
+(one pinned copy to the device) and ``run`` launches on the current stream
+without host synchronisation: one kernel, and a second one that joins the
+pieces of requests that were cut.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+from . import _native
+
+MAX_DRAFT = 64      # drafted tokens per request: bits of a mask word
+TILE_ROWS = 128     # rows (drafted token x query head of the group) per tile
+TILE_KEYS = 64
+CTAS_PER_SM = 2
+MIN_TILES = 4       # key tiles per CTA, if the batch has as many
+
+
+def tree_work_list(kv_indptr, draft_indptr, group, num_kv_heads, units, ctas, min_tiles=MIN_TILES):
+    """(items int32 [n, 12], cta_items int32 [ctas + 1], merges int32 [m, 8],
+    partials) of a batch, as ``akv_tree_attention`` reads them.
+
+    A group of ``units`` (KV head, row tile) pairs shares its key tiles: heads
+    of one row tile for requests whose rows fill one tile, row tiles of one
+    head for the others.  The key tiles of all groups, one after another, are
+    cut into equal runs, one per CTA; a group whose tiles fall to several CTAs
+    gets a partial result for each and one merge."""
+    kv, dr = np.asarray(kv_indptr, np.int64), np.asarray(draft_indptr, np.int64)
+    if kv.ndim != 1 or kv.shape != dr.shape or len(kv) < 1 or kv[0] < 0 or dr[0] < 0:
+        raise ValueError("kv_indptr and draft_indptr must be CSR offsets of one batch")
+    prefix, n = np.diff(kv), np.diff(dr)
+    if np.any(prefix < 0) or np.any(n < 0):
+        raise ValueError("kv_indptr and draft_indptr must not decrease")
+    if kv[-1] >= 2**31 or dr[-1] >= 2**31:
+        raise ValueError("the batch has 2^31 keys or more")
+    if n.size and n.max() > MAX_DRAFT:
+        raise ValueError(f"a request has more than {MAX_DRAFT} drafted tokens")
+    row_tiles = -(-n * group // TILE_ROWS)
+    by_head = row_tiles <= 1
+    head_groups = np.where(by_head, -(-num_kv_heads // units), num_kv_heads)
+    tile_groups = np.where(by_head, np.minimum(row_tiles, 1), -(-row_tiles // units))
+    groups = head_groups * tile_groups  # 0 without drafted tokens
+    req = np.repeat(np.arange(len(n)), groups)
+    local = np.arange(len(req)) - np.repeat(np.cumsum(groups) - groups, groups)
+    tiles = -(-(prefix + n) // TILE_KEYS)
+    end = np.cumsum(tiles[req])
+    total = int(end[-1]) if len(end) else 0
+    ctas = min(int(ctas), -(-total // max(1, min_tiles)))
+    bounds = (np.arange(ctas + 1) * total) // max(1, ctas)
+    cuts = np.unique(np.concatenate((bounds, end, [0])))
+    first, last = cuts[:-1], cuts[1:]
+    g = np.searchsorted(end, first, side="right")
+    r, lg = req[g], local[g]
+    begin = first - (end[g] - tiles[r])
+    tile_group, head_group = lg // head_groups[r], lg % head_groups[r]
+    heads = by_head[r]
+    items = np.zeros((len(g), 12), np.int64)
+    items[:, 0], items[:, 1], items[:, 2], items[:, 3] = dr[r], n[r], kv[r], prefix[r]
+    items[:, 4] = begin * TILE_KEYS
+    items[:, 5] = np.minimum((begin + last - first) * TILE_KEYS, prefix[r] + n[r])
+    items[:, 6] = np.where(heads, head_group * units, head_group)
+    items[:, 7] = np.where(heads, 0, tile_group * units)
+    items[:, 8], items[:, 9] = heads, ~heads
+    items[:, 10] = np.minimum(units, np.where(heads, num_kv_heads - items[:, 6],
+                                              row_tiles[r] - items[:, 7]))
+    pieces = np.bincount(g, minlength=len(req))
+    cut = pieces[g] > 1
+    items[:, 11] = np.where(cut, (np.cumsum(cut) - 1) * units, -1)
+    lead = cut & np.concatenate(([True], g[1:] != g[:-1])) if len(g) else cut
+    merges = np.zeros((int(lead.sum()), 8), np.int64)
+    m = items[lead]
+    merges[:, :4] = m[:, [0, 1, 6, 7]]
+    merges[:, 4] = m[:, 8] | m[:, 9] << 1 | m[:, 10] << 2
+    merges[:, 5], merges[:, 6] = m[:, 11], pieces[g[lead]]
+    cta_items = np.searchsorted(first, bounds).astype(np.int32)
+    return items.astype(np.int32), cta_items, merges.astype(np.int32), int(cut.sum()) * units
+
+
+class TreeAttention:
+    """Plans and partial results live in the instance: runs of one instance,
+    replays of its graphs among them, must not overlap on the device, and a
+    captured run reads the plan that the device holds when it replays."""
+
+    def __init__(self, num_q_heads, num_kv_heads, head_dim, max_batch, device, *,
+                 dtype=torch.bfloat16, sm_scale=None, ctas=None):
+        if num_kv_heads <= 0 or num_q_heads <= 0 or num_q_heads % num_kv_heads:
+            raise ValueError("tree attention needs num_q_heads a multiple of num_kv_heads")
+        if head_dim not in (64, 128):
+            raise ValueError("tree attention supports head_dim 64 and 128")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("tree attention runs on bf16 or fp16")
+        if max_batch <= 0:
+            raise ValueError("max_batch must be positive")
+        device = torch.device(device)
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.device, self._index, self.dtype = device, device.index, dtype
+        self.hq, self.hkv, self.d = num_q_heads, num_kv_heads, head_dim
+        self.group = num_q_heads // num_kv_heads
+        self.sm_scale = 1.0 / math.sqrt(head_dim) if sm_scale is None else float(sm_scale)
+        self.max_batch = int(max_batch)
+        self.units = int(_native.lib.akv_tree_attention_units(head_dim))
+        if ctas is None:
+            ctas = CTAS_PER_SM * torch.cuda.get_device_properties(device).multi_processor_count
+        self.ctas = int(ctas)
+        # Every CTA boundary cuts at most one group.
+        row_tiles = -(-MAX_DRAFT * self.group // TILE_ROWS)
+        groups = max(-(-self.hkv // self.units), self.hkv * -(-row_tiles // self.units))
+        self.max_items = self.max_batch * groups + self.ctas
+        self.max_merges = min(self.max_batch * groups, self.ctas)
+        partials = 2 * self.ctas * self.units
+        self._at = (12 * self.max_items, 12 * self.max_items + 8 * self.max_merges)
+        size = self._at[1] + self.ctas + 1
+        self._host = torch.empty(size, dtype=torch.int32, pin_memory=True)
+        self._dev = torch.zeros(size, dtype=torch.int32, device=device)
+        self._acc = torch.empty((partials, TILE_ROWS, head_dim), dtype=torch.float32, device=device)
+        self._ml = torch.empty((partials, TILE_ROWS, 2), dtype=torch.float32, device=device)
+        # [0]: error bits kept until check(); [1]: the abort word of the current launch.
+        self.error_flag = torch.zeros(2, dtype=torch.int32, device=device)
+        self._copied = torch.cuda.Event()
+        self._copied.record(torch.cuda.current_stream(device))
+        self.tokens = self.keys = self.n_ctas = self.n_merges = 0
+
+    def plan(self, kv_indptr_host, draft_indptr_host):
+        """Work list from the host-known CSR offsets of the cached keys and of
+        the drafted tokens (at most ``MAX_DRAFT`` per request)."""
+        if len(kv_indptr_host) - 1 > self.max_batch:
+            raise ValueError("batch exceeds max_batch")
+        items, cta_items, merges, partials = tree_work_list(
+            kv_indptr_host, draft_indptr_host, self.group, self.hkv, self.units, self.ctas)
+        assert len(items) <= self.max_items and len(merges) <= self.max_merges and \
+            partials <= len(self._acc)
+        self._copied.synchronize()
+        stream = torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(stream):
+            for at, part in ((0, items), (self._at[0], merges), (self._at[1], cta_items)):
+                part = part.reshape(-1)
+                if len(part):
+                    self._host[at: at + len(part)].copy_(torch.from_numpy(part))
+                    self._dev[at: at + len(part)].copy_(self._host[at: at + len(part)],
+                                                        non_blocking=True)
+            self._copied.record(stream)
+        self.tokens, self.keys = int(draft_indptr_host[-1]), int(kv_indptr_host[-1])
+        self.n_ctas, self.n_merges = len(cta_items) - 1, len(merges)
+        return self
+
+    def run(self, q, k_pool, v_pool, kv_indices, draft_slots, tree_mask, sinks=None, window=None,
+            q_positions=None, kv_positions=None, out=None, return_lse=False):
+        """``q`` [drafted tokens, Hq, D]; pools [slots, Hkv, D]; ``kv_indices`` int32
+        [cached keys] and ``draft_slots`` int32 [drafted tokens], a negative
+        draft slot for a padding token (read as zeros); ``tree_mask`` int64
+        [drafted tokens]: bit j set for a visible drafted token j of the
+        request.  A token that sees no key gets zeros (and lse -inf, or the
+        sink).  ``window`` (None or negative: none) hides keys with
+        q_position - kv_position > window and needs both position vectors
+        (int32; those of the drafted keys are ``q_positions``).  Rows of
+        ``out`` past the planned tokens are left as they were.
+
+        The head's maximum, sum and accumulator are fp32; P is rounded to the
+        pools' type for P.V.  Returns out, or (out, lse fp32 [tokens, Hq])."""
+        index, tokens = self._index, self.tokens
+        if q.dtype != self.dtype or k_pool.dtype != self.dtype or v_pool.dtype != self.dtype:
+            raise ValueError("q / K / V must have the planned type")
+        if q.ndim != 3 or q.shape[0] < tokens or q.shape[1:] != (self.hq, self.d) or \
+                q.stride(-1) != 1:
+            raise ValueError("q must be [tokens, num_q_heads, head_dim] with unit last stride")
+        for pool in (k_pool, v_pool):
+            if pool.ndim != 3 or pool.shape[1:] != (self.hkv, self.d) or pool.stride(-1) != 1:
+                raise ValueError("KV pools must be [slots, num_kv_heads, head_dim]")
+        tensors = [q, k_pool, v_pool, kv_indices, draft_slots, tree_mask]
+        window = -1 if window is None or window < 0 else int(window)
+        vectors = [("kv_indices", kv_indices, self.keys, torch.int32),
+                   ("draft_slots", draft_slots, tokens, torch.int32),
+                   ("tree_mask", tree_mask, tokens, torch.int64)]
+        if window >= 0:
+            if q_positions is None or kv_positions is None:
+                raise ValueError("a window needs q_positions and kv_positions")
+            tensors += [q_positions, kv_positions]
+            vectors += [("q_positions", q_positions, tokens, torch.int32),
+                        ("kv_positions", kv_positions, self.keys, torch.int32)]
+        for name, t, n, dt in vectors:
+            if t.dtype != dt or t.ndim != 1 or t.shape[0] < n or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {dt} vector of the plan's length")
+        if sinks is not None:
+            if sinks.dtype != torch.float32 or sinks.shape != (self.hq,) or \
+                    not sinks.is_contiguous():
+                raise ValueError("sinks must be fp32 [num_q_heads]")
+            tensors.append(sinks)
+        if out is None:
+            out = torch.empty((tokens, self.hq, self.d), dtype=self.dtype, device=self.device)
+        else:
+            if out.dtype != self.dtype or out.ndim != 3 or out.shape[0] < tokens or \
+                    out.shape[1:] != (self.hq, self.d) or out.stride(-1) != 1:
+                raise ValueError("out must be [tokens, num_q_heads, head_dim] of the planned type")
+            tensors.append(out)
+        for t in tensors:
+            if t.get_device() != index:
+                raise ValueError("tree attention tensors must be on the plan's CUDA device")
+        lse = torch.empty((tokens, self.hq), dtype=torch.float32, device=self.device) \
+            if return_lse else None
+        dev = self._dev.data_ptr()
+        status = _native.launch(
+            index, _native.lib.akv_tree_attention, q.data_ptr(), q.stride(0), q.stride(1),
+            k_pool.data_ptr(), v_pool.data_ptr(), k_pool.stride(0), k_pool.stride(1),
+            v_pool.stride(0), v_pool.stride(1), min(k_pool.shape[0], v_pool.shape[0]),
+            _native.DTYPE_CODE[self.dtype], kv_indices.data_ptr() or dev, draft_slots.data_ptr(),
+            tree_mask.data_ptr(), None if window < 0 else q_positions.data_ptr(),
+            None if window < 0 else kv_positions.data_ptr() or dev, window,
+            None if sinks is None else sinks.data_ptr(), self.sm_scale, self.hq, self.hkv, self.d,
+            dev, dev + 4 * self._at[1], self.n_ctas, dev + 4 * self._at[0], self.n_merges,
+            self._acc.data_ptr(), self._ml.data_ptr(), out.data_ptr(), out.stride(0),
+            out.stride(1), None if lse is None else lse.data_ptr(), self.error_flag.data_ptr())
+        _native.check(status, "tree_attention")
+        return (out, lse) if return_lse else out
+
+    ERRORS = {1: "a key slot outside the KV pools was read as slot 0",
+              2: "a wait inside the kernel ran out; the output of that launch is invalid"}
+
+    def check(self):
+        """Raise RuntimeError if a launch since the last check reported an
+        error, and clear the error bits (synchronises)."""
+        bits = int(self.error_flag[0].item())
+        if bits:
+            self.error_flag[0].zero_()
+            why = "; ".join(msg for bit, msg in self.ERRORS.items() if bits & bit)
+            raise RuntimeError(f"tree attention: {why}")

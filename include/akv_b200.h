@@ -742,6 +742,56 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_token, int64_t q_stride_hea
                      int64_t v_pool_stride_slot, int64_t v_pool_stride_head, int64_t num_slots,
                      const void* slots, int32_t slots_is64, int32_t* error_flag, void* stream);
 
+/*
+ * Attention of drafted token trees over the paged cache, with learned sinks.
+ * The reference verifies drafts through native backends with dense masks
+ * (beside the decode call of akv/system/sglang.patch:2170-2183).
+ *
+ * Token i of a request (q row q0 + i) sees the request's cached keys (slots
+ * kv_indices[kv0 ..]) and its drafted tokens j (slots draft_slots[q0 + j];
+ * negative: padding, read as zeros) with bit j of tree_mask[q0 + i] set; with
+ * window >= 0 only keys with q_position - k_position <= window (drafted keys'
+ * positions are their q_positions).  The sink (NULL: none) is a term of the
+ * softmax denominator.  A token that sees nothing gets zeros.
+ *
+ * q, pools and out: dtype AKV_F16 or AKV_BF16, unit last stride, addresses and
+ * strides multiples of 16 bytes; num_q_heads any multiple of num_kv_heads;
+ * head_dim 64 or 128.  lse (NULL: none) fp32 [tokens, num_q_heads], natural
+ * log, of the scores and the sink.
+ *
+ * items: DEVICE int32 [n][12] = {q0, drafted tokens (at most 64), kv0, cached
+ * keys, first key, end key, head0, tile0, head_step, tile_step, units,
+ * partial}: keys [first, end) of the cached keys followed by the drafted
+ * tokens, first a multiple of 64; unit u < units <=
+ * akv_tree_attention_units(head_dim) is KV head head0 + u * head_step and rows
+ * [128 tile, 128 tile + 128), tile = tile0 + u * tile_step, row = token *
+ * group + query head of the group; partial -1 writes the output, otherwise
+ * unit u writes partial result partial + u.  cta_items: DEVICE int32 [n_ctas +
+ * 1], CTA c runs items [cta_items[c], cta_items[c + 1]).  merges: DEVICE
+ * int32 [n_merges][8] = {q0, tokens, head0, tile0, head_step | tile_step << 1
+ * | units << 2, first partial, pieces, 0}: the pieces' partials lie
+ * akv_tree_attention_units apart.  partial_acc fp32 [partials][128][head_dim],
+ * partial_ml fp32 [partials][128][2].  tree_work_list of
+ * akv_b200/context_tree.py builds all of them.
+ *
+ * error_flag: DEVICE int32 [2] or NULL: [0] collects 1 (a slot outside the
+ * pools, read as slot 0) and 2 (a wait ran out: the launch's output is
+ * invalid); [1] is the launch's abort word, cleared by every launch.
+ */
+int32_t akv_tree_attention_units(int32_t head_dim);
+int akv_tree_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head,
+                       const void* k_pool, const void* v_pool, int64_t k_stride_slot,
+                       int64_t k_stride_head, int64_t v_stride_slot, int64_t v_stride_head,
+                       int64_t num_slots, int32_t dtype, const int32_t* kv_indices,
+                       const int32_t* draft_slots, const int64_t* tree_mask,
+                       const int32_t* q_positions, const int32_t* kv_positions, int64_t window,
+                       const float* sinks, float sm_scale, int32_t num_q_heads,
+                       int32_t num_kv_heads, int32_t head_dim, const int32_t* items,
+                       const int32_t* cta_items, int32_t n_ctas, const int32_t* merges,
+                       int32_t n_merges, float* partial_acc, float* partial_ml, void* out,
+                       int64_t out_stride_token, int64_t out_stride_head, float* lse,
+                       int32_t* error_flag, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

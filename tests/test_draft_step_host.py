@@ -86,3 +86,92 @@ def test_wrappers_refuse_cpu_tensors():
     x = torch.zeros(2, 8, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA"):
         qk_norm_rope(x, x, torch.zeros(2, dtype=torch.int32), torch.zeros(4, 64))
+
+
+def tree_args(**change):
+    a = dict(q=BUF, q_st=512, q_sh=64, k=BUF, v=BUF, k_ss=128, k_sh=64, v_ss=128, v_sh=64, slots=8,
+             dtype=1, indices=BUF, draft=BUF, mask=BUF, qpos=None, kpos=None, window=-1, sinks=None,
+             scale=1.0, hq=8, hkv=2, dim=64, items=BUF, cta_items=BUF, n_ctas=1, merges=None, n_merges=0,
+             acc=None, ml=None, out=BUF, o_st=512, o_sh=64, lse=None, flag=None)
+    assert set(change) <= set(a)
+    return [*{**a, **change}.values(), None]
+
+
+@pytest.mark.parametrize("change", [
+    dict(hkv=0), dict(hq=0), dict(hq=9), dict(n_ctas=-1), dict(n_merges=-1), dict(slots=0), dict(dtype=2),
+    dict(q=None), dict(k=None), dict(v=None), dict(indices=None), dict(draft=None), dict(mask=None),
+    dict(items=None), dict(cta_items=None), dict(out=None), dict(n_merges=1), dict(window=3),
+    dict(window=3, qpos=BUF), dict(q=ODD), dict(k=ODD), dict(v=ODD), dict(out=ODD), dict(q_st=516),
+    dict(k_ss=130), dict(v_sh=60), dict(o_sh=63),
+])
+def test_tree_attention_refuses(change):
+    from akv_b200 import _native
+
+    assert _native.lib.akv_tree_attention(*tree_args(**change)) == _native.AKV_ERR_INVALID
+
+
+def test_tree_attention_of_nothing_is_ok_and_other_head_dims_are_unsupported():
+    from akv_b200 import _native
+
+    assert _native.lib.akv_tree_attention(*tree_args(n_ctas=0)) == _native.AKV_OK
+    assert _native.lib.akv_tree_attention(*tree_args(dim=96)) == _native.AKV_ERR_UNSUPPORTED
+    assert _native.lib.akv_tree_attention_units(64) > 0
+    assert _native.lib.akv_tree_attention_units(96) < 0
+
+
+@pytest.mark.parametrize("units", [1, 2, 4])
+@pytest.mark.parametrize("hkv,group", [(8, 8), (1, 8), (3, 5), (2, 40)])
+@pytest.mark.parametrize("ctas", [1, 7, 296])
+def test_tree_work_list_covers_every_key_of_every_row_once(units, hkv, group, ctas):
+    import numpy as np
+
+    from akv_b200.context_tree import tree_work_list
+
+    rng = np.random.default_rng(units * hkv + ctas)
+    cached = np.r_[0, 1, 64, rng.integers(0, 3000, 9)]
+    new = np.r_[1, 0, 64, rng.integers(0, 65, 9)]
+    kv, dr = (np.concatenate(([0], np.cumsum(x))) for x in (cached, new))
+    items, cta_items, merges, partials = tree_work_list(kv, dr, group, hkv, units, ctas)
+    seen, parts = {}, {}
+    for q0, n, kv0, prefix, lo, hi, h0, t0, hs, ts, u_n, partial in items.tolist():
+        b = int(np.searchsorted(dr, q0, side="right")) - 1
+        assert (q0, n, kv0, prefix) == (dr[b], new[b], kv[b], cached[b]) and n > 0
+        assert 0 < u_n <= units and hs + ts == 1 and lo % 64 == 0 and lo < hi <= prefix + n
+        for u in range(u_n):
+            key = (b, h0 + u * hs, t0 + u * ts)
+            assert key[1] < hkv and key[2] * 128 < n * group
+            seen.setdefault(key, []).append((lo, hi))
+            parts.setdefault(key, []).append(-1 if partial < 0 else partial + u)
+    for b in range(len(new)):
+        for h in range(hkv):
+            for t in range(-(-int(new[b]) * group // 128)):
+                runs = sorted(seen.pop((b, h, t)))
+                assert runs[0][0] == 0 and runs[-1][1] == cached[b] + new[b]
+                assert all(x[1] == y[0] for x, y in zip(runs, runs[1:]))
+    assert not seen
+    used = sorted(p for v in parts.values() for p in v if p >= 0)
+    assert len(set(used)) == len(used) and (not used or used[-1] < partials)
+    assert partials <= 2 * ctas * units
+    joined = set()
+    for q0, n, h0, t0, steps, first, count, _ in merges.tolist():
+        b = int(np.searchsorted(dr, q0, side="right")) - 1
+        assert n == new[b] and count > 1
+        for u in range(steps >> 2):
+            key = (b, h0 + u * (steps & 1), t0 + u * (steps >> 1 & 1))
+            assert sorted(parts[key]) == [first + u + i * units for i in range(count)]
+            joined.add(key)
+    assert joined == {k for k, v in parts.items() if v[0] >= 0}
+    assert all(len(v) == 1 for k, v in parts.items() if k not in joined)
+    assert cta_items[0] == 0 and cta_items[-1] == len(items) and np.all(np.diff(cta_items) >= 0)
+    tiles = -(-(items[:, 5] - items[:, 4]) // 64)
+    load = np.add.reduceat(tiles, cta_items[:-1]) if len(items) else tiles
+    assert load.max() - load.min() <= 1
+
+
+def test_tree_work_list_refuses():
+    from akv_b200.context_tree import tree_work_list
+
+    for kv, dr in (([0, 5], [0]), ([0, 5], [0, 65]), ([5, 0], [0, 1]), ([0, 5], [1, 0]), ([], []),
+                   ([0, 1 << 31], [0, 1])):
+        with pytest.raises(ValueError):
+            tree_work_list(kv, dr, 8, 8, 2, 10)
