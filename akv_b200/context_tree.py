@@ -105,6 +105,8 @@ class TreeAttention:
             raise ValueError("tree attention runs on bf16 or fp16")
         if max_batch <= 0:
             raise ValueError("max_batch must be positive")
+        if sm_scale is not None and not sm_scale > 0:
+            raise ValueError("sm_scale must be positive")
         device = torch.device(device)
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())

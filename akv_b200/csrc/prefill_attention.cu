@@ -27,7 +27,7 @@
 // K/V rows of the KV head (head_dim * 2 bytes per key) are gathered by
 // 16-byte cp.async into a 3-stage, XOR-swizzled shared-memory ring.
 
-#include "attention_common.cuh"
+#include "tcgen05.cuh"
 
 namespace akv {
 namespace {
@@ -380,146 +380,6 @@ constexpr int kTcBarOff = kTcRowOff + 4 * 128 * 4;
 // SM, which is all the tensor memory (2 x 256 columns) holds.
 constexpr int kTcSmemUsed = kTcBarOff + 64 + 1024;
 constexpr int kTcSmem = kTcSmemUsed > 80 * 1024 ? kTcSmemUsed : 80 * 1024;
-constexpr float kStaleMax = 8.f;      // log2 headroom before O is rescaled
-constexpr unsigned long long kWaitNs = 100000000ull;  // 100 ms per mbarrier wait
-
-// Shared-memory matrix descriptor, 128-byte swizzle (UMMA canonical layout):
-// start address >> 4, leading offset 16 B (unused for these shapes), stride
-// offset 1024 B between 8-row groups, version 1, layout SWIZZLE_128B.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-// The same for an MN-major operand wider than one 64-element swizzle atom:
-// lbo_bytes is the distance between consecutive atoms along MN.
-__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t smem_addr, uint32_t lbo_bytes) {
-  return (uint64_t)((smem_addr >> 4) & 0x3FFF) | ((uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-// Instruction descriptor, kind::f16: fp32 accumulate, bf16 A and B, A
-// K-major, B K-major (b_mn = 0) or MN-major (1), M = 128, N.
-__host__ __device__ constexpr uint32_t f16_idesc(int n, int b_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc,
-                                       uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
-}
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
-               : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void fence_async_smem() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_init(uint32_t bar, int count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ unsigned long long global_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-// Bounded wait on an mbarrier phase (kWaitNs of wall time); false when it
-// ran out.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = global_ns();
-  while (!mbar_try_wait(bar, parity))
-    if (global_ns() - t0 > kWaitNs) return false;
-  return true;
-}
-// TMEM access: each tcgen05.ld / tcgen05.st shares one asm statement with its
-// tcgen05.wait, so the compiler never sees a destination (or source)
-// register as settled while the asynchronous access is still in flight --
-// a register spilled or reused in between would otherwise be written (or
-// read) late.
-__device__ __forceinline__ void tmem_ld32_sync(uint32_t taddr, float* v) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31},"
-      " [%32];\n\ttcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void tmem_st32_sync(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
-      "%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      "\n\ttcgen05.wait::st.sync.aligned;" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-// One store of 16 columns (P's hi words alone) and its wait.
-__device__ __forceinline__ void tmem_st16_sync(uint32_t ta, const uint32_t* a) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,"
-      "%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-      "\n\ttcgen05.wait::st.sync.aligned;" ::"r"(ta),
-      "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(a[4]), "r"(a[5]), "r"(a[6]), "r"(a[7]),
-      "r"(a[8]), "r"(a[9]), "r"(a[10]), "r"(a[11]), "r"(a[12]), "r"(a[13]), "r"(a[14]),
-      "r"(a[15])
-      : "memory");
-}
-// Two stores of 16 columns (P's hi and lo words) and their wait.
-__device__ __forceinline__ void tmem_st16x2_sync(uint32_t ta, const uint32_t* a, uint32_t tb,
-                                                 const uint32_t* b) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%2,%3,%4,%5,%6,%7,%8,"
-      "%9,%10,%11,%12,%13,%14,%15,%16,%17};"
-      "\n\ttcgen05.st.sync.aligned.32x32b.x16.b32 [%1], {%18,%19,%20,%21,%22,%23,%24,%25,%26,"
-      "%27,%28,%29,%30,%31,%32,%33};"
-      "\n\ttcgen05.wait::st.sync.aligned;" ::"r"(ta), "r"(tb),
-      "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(a[4]), "r"(a[5]), "r"(a[6]), "r"(a[7]),
-      "r"(a[8]), "r"(a[9]), "r"(a[10]), "r"(a[11]), "r"(a[12]), "r"(a[13]), "r"(a[14]),
-      "r"(a[15]), "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3]), "r"(b[4]), "r"(b[5]), "r"(b[6]),
-      "r"(b[7]), "r"(b[8]), "r"(b[9]), "r"(b[10]), "r"(b[11]), "r"(b[12]), "r"(b[13]),
-      "r"(b[14]), "r"(b[15])
-      : "memory");
-}
 
 __global__ void __launch_bounds__(kTcThreads, 2) prefill_attention_tc_kernel(const PrefillParams p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -905,14 +765,6 @@ struct WsCfg {
   static_assert(kAhead >= 2, "the loop signals tile t+1 from copies issued a tile earlier");
   static_assert(kCpt >= 1 && kChunks % kTpk == 0, "K/V chunks split over the loaders");
 };
-// Byte offset of 16-byte chunk c of row r in a swizzled tile of `rows` rows.
-__device__ __forceinline__ uint32_t sw_chunk(int rows, int r, int c) {
-  return (uint32_t)((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 // 64-thread named barrier 1 + q of the two warps of pair q (query tile
 // q / 4, lane quadrant q % 4); immediate ids, so the kernel reserves only the
 // barriers it uses.
@@ -928,20 +780,6 @@ __device__ __forceinline__ void pair_sync(int q) {
     default: asm volatile("bar.sync 8, 64;" ::: "memory"); break;
   }
 }
-// Bounded wait that gives up at once after the CTA aborted.
-__device__ __forceinline__ bool ws_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = global_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (*abort) return false;
-    if (global_ns() - t0 > kWaitNs) {
-      *abort = 1;
-      return false;
-    }
-  }
-  return true;
-}
-
 // LO: P enters P.V as the bf16 pair hi + lo (two MMAs per key block, P to
 // about 16 bits); without it, as hi = RN_bf16(P) alone (one MMA), the
 // precision of FlashInfer's and most flash kernels' P.V.

@@ -16,9 +16,9 @@
 // host cuts the flat list of all key tiles into equal runs, one per CTA, and
 // a second kernel joins the pieces of requests that were cut.
 
-#include <algorithm>
+#include <type_traits>
 
-#include "attention_common.cuh"
+#include "tcgen05.cuh"
 
 namespace akv {
 namespace {
@@ -61,6 +61,19 @@ struct TreeParams {
   float* lse;
   int* error_flag;
 };
+
+// A pair of fp32 values as T, the lower address first.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  return pack_bf16(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 
 // Slot of key j of an item; -1: a padding token, read as zeros.
 __device__ __forceinline__ long long key_slot(const TreeParams& p, const TreeItem& w, int j) {
@@ -107,66 +120,480 @@ __device__ __forceinline__ RowEnd row_end(const float* sinks, int h, float m, fl
   return e;
 }
 
-// One thread per row, keys one after another.
+// ws_wait by a whole warp, which then takes one way.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, ws_wait(bar, parity, abort));
+}
+
+// Key j visible to a row: its token's mask word and position.
+__device__ __forceinline__ bool key_seen(const TreeParams& p, const TreeItem& w,
+                                         unsigned long long mask, long long pos, int j) {
+  if (j >= w.prefix) return mask >> (j - w.prefix) & 1;
+  return p.window < 0 || pos - p.kv_positions[w.kv0 + j] <= p.window;
+}
+
+constexpr int tree_units(int head_dim) { return head_dim == 64 ? 2 : 1; }
+
+// Two CTAs per SM, each with 256 tensor-memory columns: per unit, SB score
+// buffers of 64 columns and the accumulator of D (P overwrites its scores).
+// K and V tiles of 64 keys alternate in a ring of 16 KiB slots: at head_dim 64
+// two heads' rows (256 contiguous bytes a key in the usual pools), at 128 one.
+// 256-byte pieces gathered by cp.async from several CTAs per SM reach the
+// copy rate on random slots (6.9 TB/s in a bare gather, against 4.9 for
+// 128-byte pieces and 4.9 for TMA row gathers, whose issue is the limit).
+template <int D>
+struct TreeCfg {
+  static constexpr int kUnits = tree_units(D);
+  static constexpr int kBuffers = D == 64 ? 1 : 2;   // score buffers per unit
+  static constexpr int kSoftmax = 4 * kUnits;        // warps
+  static constexpr int kProducers = 2;               // warps
+  static constexpr int kThreads = 32 * (kSoftmax + kProducers + kUnits);
+  static constexpr int kHeadBytes = kTreeKeys * D * 2;  // one head's rows of a tile
+  static constexpr int kSlotBytes = 16384;
+  static constexpr int kSlots = 5;
+  static constexpr int kAhead = 3;                   // slots requested before the oldest is awaited
+  static constexpr int kQBytes = kTreeRows * D * 2;
+  static constexpr int kRingOff = kUnits * kQBytes;
+  static constexpr int kBarOff = kRingOff + kSlots * kSlotBytes;
+  static constexpr int kSmem = kBarOff + 256;
+  static constexpr int kUnitCols = 256 / kUnits;
+  static constexpr int kColO = kUnitCols - D;
+  static_assert(kHeadBytes * kUnits == kSlotBytes || kUnits == 1, "slot holds every unit's head");
+  static_assert(kAhead <= kSlots - 2, "a slot is signalled before its successors wait for room");
+};
+
+// Warps: 4 per unit run its softmax (warp w: rows 32 (w % 4) ..), then two
+// producers, then one MMA issuer per unit, so that units never wait for one
+// another.  Per slot: full (every producer thread's copies have landed), empty
+// (each unit's MMAs that read it are done).  Per unit: q (its Q tile is
+// stored), s[b] (scores done), p[b] (P stored), o (every P.V), done (the last
+// P.V of an item).  Waits are bounded; once one runs out the CTA's abort
+// flag ends every role's loop and *error_flag gets bit 2.
 template <typename T, int D>
-__global__ void __launch_bounds__(kTreeRows) tree_attention_kernel(const TreeParams p, int units) {
-  __shared__ float ks[16][D], vs[16][D];
-  __shared__ long long slots[16];
-  const int r = threadIdx.x;
-  for (int it = p.cta_items[blockIdx.x]; it < p.cta_items[blockIdx.x + 1]; ++it) {
-    const TreeItem w = p.items[it];
-    for (int u = 0; u < w.units; ++u) {
+__global__ void __launch_bounds__(TreeCfg<D>::kThreads, 2)
+tree_attention_kernel(const TreeParams p) {
+  using C = TreeCfg<D>;
+  constexpr int U = C::kUnits, SB = C::kBuffers;
+  constexpr int kHalf = std::is_same<T, __half>::value;  // fp16 operands
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const uint32_t base = smem_u32(smem);
+  const uint32_t bars = base + C::kBarOff;
+  auto bar_full = [&](uint32_t s) { return bars + 8u * s; };
+  auto bar_empty = [&](uint32_t s) { return bars + 8u * (C::kSlots + s); };
+  constexpr int kUnitBars = 3 + 2 * SB;
+  auto unit_bar = [&](int u, int i) { return bars + 8u * (2 * C::kSlots + u * kUnitBars + i); };
+  auto bar_q = [&](int u) { return unit_bar(u, 0); };
+  auto bar_o = [&](int u) { return unit_bar(u, 1); };
+  auto bar_done = [&](int u) { return unit_bar(u, 2); };
+  auto bar_s = [&](int u, uint32_t b) { return unit_bar(u, 3 + b); };
+  auto bar_p = [&](int u, uint32_t b) { return unit_bar(u, 3 + SB + b); };
+  static_assert(8 * (2 * C::kSlots + U * kUnitBars) + 16 <= 256, "barriers and flags");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOff + 240);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + C::kBarOff + 244);
+  volatile int* scrubbed = reinterpret_cast<volatile int*>(smem + C::kBarOff + 248);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(256));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (tid == 32) {
+    for (int s = 0; s < C::kSlots; ++s) {
+      mbar_init(bar_full(s), 32 * C::kProducers);
+      mbar_init(bar_empty(s), U);
+    }
+    for (int u = 0; u < U; ++u) {
+      mbar_init(bar_q(u), kTreeRows);
+      mbar_init(bar_o(u), 1);
+      mbar_init(bar_done(u), 1);
+      for (int b = 0; b < SB; ++b) {
+        mbar_init(bar_s(u, b), 1);
+        mbar_init(bar_p(u, b), 4);
+      }
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *abort = base & 1023 ? 1 : 0;  // the swizzled tiles need a 1024-byte aligned base
+    *scrubbed = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int it0 = p.cta_items[blockIdx.x], it1 = p.cta_items[blockIdx.x + 1];
+
+  if (warp >= C::kSoftmax + C::kProducers) {
+    // ---- one MMA issuer per unit ----
+    if (lane == 0) {
+      const int u = warp - C::kSoftmax - C::kProducers;
+      const uint32_t tu = tmem + u * C::kUnitCols;
+      const uint32_t sq = base + u * C::kQBytes;
+      uint32_t seq = 0, cnt = 0, items = 0;  // slots; this unit's tiles and items so far
+      for (int it = it0; it < it1; ++it) {
+        const TreeItem w = p.items[it];
+        const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
+        if (u >= w.units) {  // idle: give the slots back
+          bool ok = true;
+          for (int t = 0; t < 2 * n_tiles && ok; ++t, ++seq) {
+            ok = ws_wait(bar_full(seq % C::kSlots), seq / C::kSlots & 1, abort);
+            if (ok) mbar_arrive(bar_empty(seq % C::kSlots));
+          }
+          if (!ok) break;
+          continue;
+        }
+        if (!ws_wait(bar_q(u), items & 1, abort)) break;
+        const uint32_t head = w.head_step ? u * C::kHeadBytes : 0;
+        auto scores = [&](uint32_t c, uint32_t sk) {  // S(c) = Q K^T
+          tc_fence_after();
+          const uint32_t kb = base + C::kRingOff + sk % C::kSlots * C::kSlotBytes + head;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = 32u * (k & 3);
+            mma_ss(tu + c % SB * kTreeKeys,
+                   sw128_desc(sq + (k >> 2) * kTreeRows * 128 + off),
+                   sw128_desc(kb + (k >> 2) * kTreeKeys * 128 + off),
+                   f16_idesc(kTreeKeys, 0, kHalf), k > 0);
+          }
+          umma_commit(bar_s(u, c % SB));
+          umma_commit(bar_empty(sk % C::kSlots));
+        };
+        auto values = [&](uint32_t c, uint32_t sv, bool first, bool last) {  // O += P(c) V
+          tc_fence_after();
+          const uint32_t vb = base + C::kRingOff + sv % C::kSlots * C::kSlotBytes + head;
+#pragma unroll
+          for (int k = 0; k < kTreeKeys / 16; ++k) {  // 16 keys: 8 P columns, 2 KiB of V
+            const uint64_t vd = D == 64 ? sw128_desc(vb + 2048 * k)
+                                        : sw128_desc_mn(vb + 2048 * k, kTreeKeys * 128);
+            mma_ts(tu + C::kColO, tu + c % SB * kTreeKeys + 8 * k, vd, f16_idesc(D, 1, kHalf),
+                   !first || k > 0);
+          }
+          umma_commit(bar_o(u));
+          umma_commit(bar_empty(sv % C::kSlots));
+          if (last) umma_commit(bar_done(u));
+        };
+        bool ok = true;
+        // With two score buffers S(t) is issued before P(t-1).V(t-1), so the
+        // softmax never waits for a product; with one, after it is done.
+        for (int t = 0; t < n_tiles + SB - 1 && ok; ++t) {
+          if (t < n_tiles) {
+            const uint32_t sk = seq + 2 * t;
+            ok = ws_wait(bar_full(sk % C::kSlots), sk / C::kSlots & 1, abort);
+            // The buffer's last product is done: of SB tiles before or, as an
+            // item begins, the last one of the item before (all were issued).
+            if (ok && t >= SB) ok = ws_wait(bar_o(u), cnt + t - SB & 1, abort);
+            if (ok && t == 0 && cnt > 0) ok = ws_wait(bar_o(u), cnt - 1 & 1, abort);
+            if (!ok) break;
+            scores(cnt + t, sk);
+          }
+          const int v = t - (SB - 1);
+          if (v >= 0) {
+            const uint32_t c = cnt + v, sv = seq + 2 * v + 1;
+            ok = ws_wait(bar_full(sv % C::kSlots), sv / C::kSlots & 1, abort) &&
+                 ws_wait(bar_p(u, c % SB), c / SB & 1, abort);
+            if (!ok) break;
+            values(c, sv, v == 0, v == n_tiles - 1);
+          }
+        }
+        if (!ok) break;
+        seq += 2 * n_tiles;
+        cnt += n_tiles;
+        ++items;
+      }
+    }
+    __syncwarp();
+  } else if (warp >= C::kSoftmax) {
+    // ---- producers: warp pw gathers keys 32 pw .. of every tile ----
+    const int pw = warp - C::kSoftmax;
+    static_assert(kTreeKeys == 32 * C::kProducers, "one key per producer lane");
+    uint32_t seq = 0;
+    // Signals slot `s` (its copies have landed); a V slot of a guarded tile
+    // is first searched for infinities and NaN, which P = 0 would not mask.
+    uint32_t guard = 0;  // bit a: the slot requested a slots ago is a guarded V tile
+    int cpk = 0;         // 16-byte chunks per key of the current item, and of guarded slots
+    auto signal = [&](uint32_t s, bool guarded, int chunks) {
+      if (guarded) {
+        unsigned char* tile = smem + C::kRingOff + s % C::kSlots * C::kSlotBytes;
+        const int per = 32 / chunks;
+        for (int i = 0; i < 32 / per; ++i) {
+          const int key = 32 * pw + i * per + lane / chunks, c = lane % chunks;
+          uint4* at = reinterpret_cast<uint4*>(tile + c / (D / 8) * C::kHeadBytes +
+                                               sw_chunk(kTreeKeys, key, c % (D / 8)));
+          uint4 x = *at;
+          uint32_t* e = reinterpret_cast<uint32_t*>(&x);
+          bool hit = false;
+          constexpr uint32_t kExp = kHalf ? 0x7c00u : 0x7f80u;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if ((e[k] & kExp) == kExp) { e[k] &= 0xffff0000u; hit = true; }
+            if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0xffffu; hit = true; }
+          }
+          if (hit) {
+            *at = x;
+            *scrubbed = 1;
+          }
+        }
+      }
+      fence_async_smem();
+      mbar_arrive(bar_full(s % C::kSlots));
+    };
+    int old_cpk = 0;
+    bool ok = true;
+    for (int it = it0; it < it1; ++it) {
+      const TreeItem w = p.items[it];
+      const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
+      cpk = (w.head_step ? w.units : 1) * (D / 8);
+      auto fetch = [&](int t) {
+        const int j = w.lo + t * kTreeKeys + 32 * pw + lane;
+        return t < n_tiles && j < w.hi ? (int)key_slot(p, w, j) : -1;
+      };
+      int next = fetch(0);
+      for (int t = 0; t < n_tiles; ++t) {
+        const int slot = next;
+        next = fetch(t + 1);
+        const bool guarded = p.window >= 0 || w.lo + (t + 1) * kTreeKeys > w.prefix;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++seq) {
+          if (!warp_wait(bar_empty(seq % C::kSlots), (seq / C::kSlots & 1) ^ 1, abort)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = base + C::kRingOff + seq % C::kSlots * C::kSlotBytes;
+          const T* pool = static_cast<const T*>(kv ? p.v : p.k) +
+                          w.head0 * (kv ? p.v_sh : p.k_sh);
+          const long long ss = kv ? p.v_ss : p.k_ss, sh = kv ? p.v_sh : p.k_sh;
+          auto copy = [&](auto chunks) {
+            constexpr int kCpk = decltype(chunks)::value, kPer = 32 / kCpk;
+            const int c = lane % kCpk, hh = c / (D / 8), cc = c % (D / 8);
+            const T* src = pool + hh * sh + cc * 8;
+#pragma unroll
+            for (int i = 0; i < 32 / kPer; ++i) {
+              const int kk = i * kPer + lane / kCpk, key = 32 * pw + kk;
+              const int sl = __shfl_sync(0xffffffffu, slot, kk);
+              cp_async16(dst + hh * C::kHeadBytes + sw_chunk(kTreeKeys, key, cc),
+                         src + (sl < 0 ? 0 : sl) * ss, sl < 0 ? 0 : 16);
+            }
+          };
+          if (cpk == 16) copy(std::integral_constant<int, 16>());
+          else copy(std::integral_constant<int, 8>());
+          cp_async_commit();
+          guard = guard << 1 | (uint32_t)(kv && guarded);
+          if (seq >= C::kAhead - 1) {
+            cp_async_wait<C::kAhead - 1>();
+            const uint32_t ago = C::kAhead - 1;
+            // The slot of `ago` requests before: of this item, or of the one before it.
+            signal(seq - ago, guard >> ago & 1, 2 * t + kv >= (int)ago ? cpk : old_cpk);
+          }
+        }
+        if (!ok) break;
+      }
+      if (!ok) break;
+      // An item has at least one tile (two slots), so the slots still to be
+      // signalled are of the current item and, for one of them, the last.
+      old_cpk = cpk;
+    }
+    if (ok) {
+      cp_async_wait<0>();
+#pragma unroll
+      for (int ago = C::kAhead - 2; ago >= 0; --ago)
+        if (seq >= (uint32_t)ago + 1) signal(seq - 1 - ago, guard >> ago & 1, cpk);
+    }
+    cp_async_wait<0>();
+  } else {
+    // ---- softmax: warp w serves unit w / 4 and its rows 32 (w % 4) .. ----
+    const int u = warp >> 2, r = tid & (kTreeRows - 1);
+    const uint32_t tu = tmem + u * C::kUnitCols + ((uint32_t)(warp & 3) << 21);
+    uint32_t cnt = 0, items = 0;
+    for (int it = it0; it < it1; ++it) {
+      const TreeItem w = p.items[it];
+      if (u >= w.units) continue;
+      const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
       const int head = w.head0 + u * w.head_step;
-      const int row = (w.tile0 + u * w.tile_step) * kTreeRows + r;
-      const int i = row / p.group, h = head * p.group + row % p.group;
+      const int row0 = (w.tile0 + u * w.tile_step) * kTreeRows;
+      const int i = (row0 + r) / p.group, h = head * p.group + (row0 + r) - i * p.group;
       const bool live = i < w.n;
-      const T* q = static_cast<const T*>(p.q) + (long long)(w.q0 + (live ? i : 0)) * p.q_st +
-                   (long long)(live ? h : 0) * p.q_sh;
+      const bool warp_live = row0 + (warp & 3) * 32 < w.n * p.group;
+      if (live) {
+        const uint4* src = reinterpret_cast<const uint4*>(
+            static_cast<const T*>(p.q) + (long long)(w.q0 + i) * p.q_st + (long long)h * p.q_sh);
+        unsigned char* dst = smem + u * C::kQBytes;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          *reinterpret_cast<uint4*>(dst + sw_chunk(kTreeRows, r, c)) = src[c];
+      }
+      fence_async_smem();
+      mbar_arrive(bar_q(u));
       const unsigned long long mask = live ? row_mask(p, w, i) : 0;
       const long long pos = live && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
-      float acc[D], m = -INFINITY, l = 0.f;
-      for (int d = 0; d < D; ++d) acc[d] = 0.f;
-      for (int j0 = w.lo; j0 < w.hi; j0 += 16) {
-        __syncthreads();
-        if (r < 16) slots[r] = j0 + r < w.hi ? key_slot(p, w, j0 + r) : -1;
-        __syncthreads();
-        for (int e = r; e < 16 * D; e += kTreeRows) {
-          const long long s = slots[e / D];
-          const T* kp = static_cast<const T*>(p.k) + s * p.k_ss + head * p.k_sh;
-          const T* vp = static_cast<const T*>(p.v) + s * p.v_ss + head * p.v_sh;
-          ks[e / D][e % D] = s < 0 ? 0.f : Elem<T>::to_f32(kp[e % D]);
-          vs[e / D][e % D] = s < 0 ? 0.f : Elem<T>::to_f32(vp[e % D]);
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int t = 0; t < n_tiles; ++t) {
+        const uint32_t c = cnt + t, b = c % SB;
+        ok = warp_wait(bar_s(u, b), c / SB & 1, abort);
+        if (!ok) break;
+        if (warp_live) {
+          tc_fence_after();
+          const uint32_t ts = tu + b * kTreeKeys;
+          const int j0 = w.lo + t * kTreeKeys;
+          unsigned long long seen = ~0ull;
+          if (p.window >= 0 || j0 + kTreeKeys > w.prefix) {
+            const int cached = min(max(w.prefix - j0, 0), kTreeKeys);
+            seen = cached == 0          ? mask >> (j0 - w.prefix)
+                   : cached < kTreeKeys ? mask << cached
+                                        : 0;
+            if (p.window < 0) {
+              seen |= cached == kTreeKeys ? ~0ull : (1ull << cached) - 1;
+            } else {
+              const int* kp = p.kv_positions + w.kv0 + j0;
+              const int p0 = lane < cached ? kp[lane] : 0;
+              const int p1 = lane + 32 < cached ? kp[lane + 32] : 0;
+              for (int k = 0; k < cached; ++k) {
+                const int kpos = __shfl_sync(0xffffffffu, k < 32 ? p0 : p1, k & 31);
+                if (pos - kpos <= p.window) seen |= 1ull << k;
+              }
+            }
+            if (j0 + kTreeKeys > w.hi) seen &= (1ull << (w.hi - j0)) - 1;
+          }
+          const bool masked = __any_sync(0xffffffffu, seen != ~0ull);
+          // The scores stay in tensor memory and are read twice, 32 columns
+          // at a time (for the maximum, for P): 64 of them in registers
+          // spill at the 80 that two CTAs leave a thread.
+          auto scores32 = [&](int half, float(&s)[32]) {
+            tmem_ld32_sync(ts + 32 * half, s);
+            if (masked) {
+              const uint32_t bits = (uint32_t)(seen >> 32 * half);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) s[k] = bits >> k & 1 ? s[k] : -INFINITY;
+            }
+          };
+          float bm;
+          {
+            float s[32], m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              scores32(half, s);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], s[k]);
+            }
+            bm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+          }
+          // The base only moves when the tile exceeds it by 2^8; then l and
+          // O are rescaled.
+          float alpha = 1.f;
+          bool rescale = false;
+          if (bm > m + kStaleMax || (m == -INFINITY && bm != -INFINITY)) {
+            rescale = m != -INFINITY;
+            alpha = rescale ? fast_exp2(m - bm) : 0.f;
+            m = bm;
+          }
+          const float nb = m == -INFINITY ? 0.f : -m;
+          const f32x2 scale2 = f2_pack(p.scale_log2, p.scale_log2), nb2 = f2_pack(nb, nb);
+          f32x2 sum0 = f2_pack(0.f, 0.f), sum1 = sum0;
+          // P in two halves, each stored over the first columns of its
+          // scores, which this warp has read.
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t pk[16];
+            float s[32];
+            scores32(half, s);
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              float x0, x1;
+              f2_unpack(f2_fma(f2_pack(s[k], s[k + 1]), scale2, nb2), x0, x1);
+              x0 = fast_exp2(x0);
+              x1 = fast_exp2(x1);
+              if (k & 2) sum1 = f2_add(sum1, f2_pack(x0, x1));
+              else sum0 = f2_add(sum0, f2_pack(x0, x1));
+              pk[k / 2] = pack2<T>(x0, x1);
+            }
+            tmem_st16_sync(ts + 16 * half, pk);
+          }
+          float l0, l1;
+          f2_unpack(f2_add(sum0, sum1), l0, l1);
+          l = l * alpha + (l0 + l1);
+          if (__any_sync(0xffffffffu, rescale)) {
+            // With one score buffer S(t) came after P(t-1).V(t-1).
+            if (SB > 1) ok = warp_wait(bar_o(u), c - 1 & 1, abort);
+            tc_fence_after();
+#pragma unroll
+            for (int d = 0; d < D; d += 32) {
+              float o[32];
+              tmem_ld32_sync(tu + C::kColO + d, o);
+              uint32_t z[32];
+#pragma unroll
+              for (int k = 0; k < 32; ++k) z[k] = __float_as_uint(o[k] * alpha);
+              tmem_st32_sync(tu + C::kColO + d, z);
+            }
+          }
+          tc_fence_before();
         }
-        __syncthreads();
-        for (int c = 0; c < 16 && j0 + c < w.hi; ++c) {
-          const int j = j0 + c;
-          bool seen = live && (j < w.prefix || (mask >> (j - w.prefix) & 1));
-          if (seen && j < w.prefix && p.window >= 0)
-            seen = pos - p.kv_positions[w.kv0 + j] <= p.window;
-          if (!seen) continue;
-          float s = 0.f;
-          for (int d = 0; d < D; ++d) s += Elem<T>::to_f32(q[d]) * ks[c][d];
-          s *= p.scale_log2;
-          const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-          const float alpha = fast_exp2(m - base), e = fast_exp2(s - base);
-          m = mn;
-          l = l * alpha + e;
-          for (int d = 0; d < D; ++d) acc[d] = acc[d] * alpha + e * vs[c][d];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p(u, b));
+      }
+      if (!ok) break;
+      cnt += n_tiles;
+      if (!warp_wait(bar_done(u), items & 1, abort)) break;
+      ++items;
+      if (!warp_live) continue;
+      tc_fence_after();
+      const bool direct = w.partial < 0;
+      const long long at = ((long long)w.partial + u) * kTreeRows + r;
+      const RowEnd e = row_end(p.sinks, live ? h : 0, m, l);
+      T* dst = static_cast<T*>(p.out) + (long long)(w.q0 + i) * p.o_st + (long long)h * p.o_sh;
+#pragma unroll
+      for (int d = 0; d < D; d += 32) {
+        float o[32];
+        __syncwarp();
+        tmem_ld32_sync(tu + C::kColO + d, o);
+        if (!live) continue;
+        if (*scrubbed) {
+          // Infinities and NaN were taken out of guarded V tiles: the rows
+          // that see them get them here.
+          for (int j = p.window >= 0 ? w.lo : max(w.lo, w.prefix & ~(kTreeKeys - 1)); j < w.hi;
+               ++j) {
+            if (!key_seen(p, w, mask, pos, j)) continue;
+            const long long slot = key_slot(p, w, j);
+            if (slot < 0) continue;
+            const T* v = static_cast<const T*>(p.v) + slot * p.v_ss + head * p.v_sh + d;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float x = Elem<T>::to_f32(v[k]);
+              if (!isfinite(x)) o[k] += x;
+            }
+          }
+        }
+        if (direct) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint4 x;
+            x.x = pack2<T>(o[k] * e.scale, o[k + 1] * e.scale);
+            x.y = pack2<T>(o[k + 2] * e.scale, o[k + 3] * e.scale);
+            x.z = pack2<T>(o[k + 4] * e.scale, o[k + 5] * e.scale);
+            x.w = pack2<T>(o[k + 6] * e.scale, o[k + 7] * e.scale);
+            *reinterpret_cast<uint4*>(dst + d + k) = x;
+          }
+        } else {
+          float4* acc = reinterpret_cast<float4*>(p.part_acc + at * D + d);
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) acc[k / 4] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
       }
-      if (!live) continue;
-      if (w.partial >= 0) {
-        const long long at = (long long)(w.partial + u) * kTreeRows + r;
-        for (int d = 0; d < D; ++d) p.part_acc[at * D + d] = acc[d];
+      if (live && !direct) {
         p.part_ml[2 * at] = m;
         p.part_ml[2 * at + 1] = l;
-        continue;
+      } else if (live && p.lse) {
+        p.lse[(long long)(w.q0 + i) * p.num_q_heads + h] = e.lse;
       }
-      const RowEnd e = row_end(p.sinks, h, m, l);
-      T* o = static_cast<T*>(p.out) + (long long)(w.q0 + i) * p.o_st + (long long)h * p.o_sh;
-      for (int d = 0; d < D; ++d) o[d] = Elem<T>::from_f32(acc[d] * e.scale);
-      if (p.lse) p.lse[(long long)(w.q0 + i) * p.num_q_heads + h] = e.lse;
+      tc_fence_before();  // O's reads before the next item's products
     }
+  }
+  tc_fence_before();
+  __syncthreads();
+  pdl_launch_dependents();
+  if (tid == 0 && *abort && p.error_flag) atomicOr(p.error_flag, 2);
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
   }
 }
 
@@ -190,6 +617,7 @@ tree_merge_kernel(const TreeParams p, const TreeMerge* merges, int units) {
   const int row = (g.tile0 + u * (g.steps >> 1 & 1)) * kTreeRows + r;
   const int i = row / p.group, h = head * p.group + row % p.group;
   if (i >= g.n) return;
+  pdl_wait();
   const long long step = (long long)units * kTreeRows;  // rows between two pieces
   const long long at = ((long long)g.first + u) * kTreeRows + r;
   float m = -INFINITY;
@@ -215,16 +643,18 @@ tree_merge_kernel(const TreeParams p, const TreeMerge* merges, int units) {
   if (p.lse && lane == 0) p.lse[(long long)(g.q0 + i) * p.num_q_heads + h] = e.lse;
 }
 
-constexpr int tree_units(int head_dim) { return head_dim == 64 ? 2 : 1; }
-
 template <typename T, int D>
 int launch_tree(const TreeParams& p, int n_ctas, const TreeMerge* merges, int n_merges,
                 cudaStream_t s) {
-  constexpr int U = tree_units(D);
-  if (n_ctas > 0) tree_attention_kernel<T, D><<<n_ctas, kTreeRows, 0, s>>>(p, U);
-  if (n_merges > 0)
-    tree_merge_kernel<T, D><<<dim3(n_merges, U * (kTreeRows / kMergeWarps)), 32 * kMergeWarps, 0,
-                              s>>>(p, merges, U);
+  using C = TreeCfg<D>;
+  if (cudaFuncSetAttribute(tree_attention_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           C::kSmem) != cudaSuccess)
+    return AKV_ERR_CUDA;
+  tree_attention_kernel<T, D><<<n_ctas, C::kThreads, C::kSmem, s>>>(p);
+  if (n_merges > 0 &&
+      launch_pdl(tree_merge_kernel<T, D>, dim3(n_merges, C::kUnits * (kTreeRows / kMergeWarps)),
+                 dim3(32 * kMergeWarps), 0, s, p, merges, (int)C::kUnits) != cudaSuccess)
+    return AKV_ERR_CUDA;
   return launch_status();
 }
 
@@ -248,7 +678,7 @@ extern "C" int akv_tree_attention(
   AKV_NVTX_RANGE("akv_tree_attention");
   using namespace akv;
   if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || n_ctas < 0 ||
-      n_merges < 0 || num_slots <= 0 || (dtype != AKV_F16 && dtype != AKV_BF16))
+      n_merges < 0 || !(sm_scale > 0.f) || num_slots <= 0 || (dtype != AKV_F16 && dtype != AKV_BF16))
     return AKV_ERR_INVALID;
   if (head_dim != 64 && head_dim != 128) return AKV_ERR_UNSUPPORTED;
   if (n_ctas == 0) return AKV_OK;
