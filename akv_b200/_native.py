@@ -115,7 +115,7 @@ SIGNATURES = {
         _P, _P, _I32, ctypes.c_float, _P, _I32, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64,
         _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I32, _P, _P,
     ],
-    "akv_tree_attention_units": [_I32],
+    "akv_tree_attention_units": [],
     "akv_tree_attention": [
         _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _P, _I64, _P,
         ctypes.c_float, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, _P, _P, _P, _I64, _I64, _P, _P,

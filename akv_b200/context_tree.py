@@ -25,20 +25,23 @@ from . import _native
 
 MAX_DRAFT = 64      # drafted tokens per request: bits of a mask word
 TILE_ROWS = 128     # rows (drafted token x query head of the group) per tile
-TILE_KEYS = 64
-CTAS_PER_SM = 2
-MIN_TILES = 4       # key tiles per CTA, if the batch has as many
+TILE_KEYS = 128
+UNITS = int(_native.lib.akv_tree_attention_units())
+MIN_TILES = 1       # key tiles per CTA, if the batch has as many
 
 
-def tree_work_list(kv_indptr, draft_indptr, group, num_kv_heads, units, ctas, min_tiles=MIN_TILES):
+def tree_work_list(kv_indptr, draft_indptr, group, num_kv_heads, pair_heads, ctas,
+                   min_tiles=MIN_TILES):
     """(items int32 [n, 12], cta_items int32 [ctas + 1], merges int32 [m, 8],
     partials) of a batch, as ``akv_tree_attention`` reads them.
 
-    A group of ``units`` (KV head, row tile) pairs shares its key tiles: heads
-    of one row tile for requests whose rows fill one tile, row tiles of one
-    head for the others.  The key tiles of all groups, one after another, are
-    cut into equal runs, one per CTA; a group whose tiles fall to several CTAs
-    gets a partial result for each and one merge."""
+    A CTA has two units.  A pair of (KV head, row tile)s over the same key
+    tiles is one group: two heads of a request whose rows fill one tile (with
+    ``pair_heads``), or two row tiles of one head; what is left over is a
+    single, whose key tiles the units share out, at half the cost per tile.
+    The key tiles of all groups, one after another, are cut into runs of equal
+    cost, one per CTA; a group whose tiles fall to several CTAs gets a partial
+    result for each and one merge."""
     kv, dr = np.asarray(kv_indptr, np.int64), np.asarray(draft_indptr, np.int64)
     if kv.ndim != 1 or kv.shape != dr.shape or len(kv) < 1 or kv[0] < 0 or dr[0] < 0:
         raise ValueError("kv_indptr and draft_indptr must be CSR offsets of one batch")
@@ -50,44 +53,49 @@ def tree_work_list(kv_indptr, draft_indptr, group, num_kv_heads, units, ctas, mi
     if n.size and n.max() > MAX_DRAFT:
         raise ValueError(f"a request has more than {MAX_DRAFT} drafted tokens")
     row_tiles = -(-n * group // TILE_ROWS)
-    by_head = row_tiles <= 1
-    head_groups = np.where(by_head, -(-num_kv_heads // units), num_kv_heads)
-    tile_groups = np.where(by_head, np.minimum(row_tiles, 1), -(-row_tiles // units))
-    groups = head_groups * tile_groups  # 0 without drafted tokens
+    by_head = (row_tiles == 1) & bool(pair_heads)
+    # Groups of a request: over its heads in pairs, or per head over its row tiles in pairs.
+    per_head = np.where(by_head, 1, -(-row_tiles // 2))
+    groups = np.where(by_head, -(-num_kv_heads // 2), num_kv_heads * per_head)
     req = np.repeat(np.arange(len(n)), groups)
     local = np.arange(len(req)) - np.repeat(np.cumsum(groups) - groups, groups)
-    tiles = -(-(prefix + n) // TILE_KEYS)
-    end = np.cumsum(tiles[req])
-    total = int(end[-1]) if len(end) else 0
+    heads = by_head[req]
+    head = np.where(heads, 2 * local, local // per_head[req].clip(1))
+    tile = np.where(heads, 0, 2 * (local % per_head[req].clip(1)))
+    pair = np.where(heads, head + 1 < num_kv_heads, tile + 1 < row_tiles[req])
+    tiles = -(-(prefix + n) // TILE_KEYS)[req]
+    tile_end, weight = np.cumsum(tiles), 1 + pair
+    cost_end = np.cumsum(tiles * weight)
+    total, cost = (int(tile_end[-1]), int(cost_end[-1])) if len(req) else (0, 0)
     ctas = min(int(ctas), -(-total // max(1, min_tiles)))
-    bounds = (np.arange(ctas + 1) * total) // max(1, ctas)
-    cuts = np.unique(np.concatenate((bounds, end, [0])))
+    bounds = (np.arange(ctas + 1) * cost) // max(1, ctas)
+    if ctas:
+        g = np.minimum(np.searchsorted(cost_end, bounds, side="right"), len(req) - 1)
+        at = (bounds - (cost_end[g] - tiles[g] * weight[g])) // weight[g]
+        bounds = tile_end[g] - tiles[g] + at
+    cuts = np.unique(np.concatenate((bounds, tile_end, [0])))
     first, last = cuts[:-1], cuts[1:]
-    g = np.searchsorted(end, first, side="right")
-    r, lg = req[g], local[g]
-    begin = first - (end[g] - tiles[r])
-    tile_group, head_group = lg // head_groups[r], lg % head_groups[r]
-    heads = by_head[r]
+    g = np.searchsorted(tile_end, first, side="right")
+    r = req[g]
+    begin = first - (tile_end[g] - tiles[g])
     items = np.zeros((len(g), 12), np.int64)
     items[:, 0], items[:, 1], items[:, 2], items[:, 3] = dr[r], n[r], kv[r], prefix[r]
     items[:, 4] = begin * TILE_KEYS
     items[:, 5] = np.minimum((begin + last - first) * TILE_KEYS, prefix[r] + n[r])
-    items[:, 6] = np.where(heads, head_group * units, head_group)
-    items[:, 7] = np.where(heads, 0, tile_group * units)
-    items[:, 8], items[:, 9] = heads, ~heads
-    items[:, 10] = np.minimum(units, np.where(heads, num_kv_heads - items[:, 6],
-                                              row_tiles[r] - items[:, 7]))
+    items[:, 6], items[:, 7] = head[g], tile[g]
+    items[:, 8], items[:, 9] = pair[g] & heads[g], pair[g] & ~heads[g]
+    items[:, 10] = weight[g]
     pieces = np.bincount(g, minlength=len(req))
     cut = pieces[g] > 1
-    items[:, 11] = np.where(cut, (np.cumsum(cut) - 1) * units, -1)
+    items[:, 11] = np.where(cut, (np.cumsum(cut) - 1) * UNITS, -1)
     lead = cut & np.concatenate(([True], g[1:] != g[:-1])) if len(g) else cut
-    merges = np.zeros((int(lead.sum()), 8), np.int64)
     m = items[lead]
+    merges = np.zeros((len(m), 8), np.int64)
     merges[:, :4] = m[:, [0, 1, 6, 7]]
     merges[:, 4] = m[:, 8] | m[:, 9] << 1 | m[:, 10] << 2
     merges[:, 5], merges[:, 6] = m[:, 11], pieces[g[lead]]
     cta_items = np.searchsorted(first, bounds).astype(np.int32)
-    return items.astype(np.int32), cta_items, merges.astype(np.int32), int(cut.sum()) * units
+    return items.astype(np.int32), cta_items, merges.astype(np.int32), int(cut.sum()) * UNITS
 
 
 class TreeAttention:
@@ -115,16 +123,17 @@ class TreeAttention:
         self.group = num_q_heads // num_kv_heads
         self.sm_scale = 1.0 / math.sqrt(head_dim) if sm_scale is None else float(sm_scale)
         self.max_batch = int(max_batch)
-        self.units = int(_native.lib.akv_tree_attention_units(head_dim))
+        # Two heads' rows of head_dim 64 are 256 bytes a key, as one head's of 128.
+        self.pair_heads = head_dim == 64
         if ctas is None:
-            ctas = CTAS_PER_SM * torch.cuda.get_device_properties(device).multi_processor_count
+            ctas = torch.cuda.get_device_properties(device).multi_processor_count
         self.ctas = int(ctas)
         # Every CTA boundary cuts at most one group.
         row_tiles = -(-MAX_DRAFT * self.group // TILE_ROWS)
-        groups = max(-(-self.hkv // self.units), self.hkv * -(-row_tiles // self.units))
+        groups = self.hkv * -(-row_tiles // 2)
         self.max_items = self.max_batch * groups + self.ctas
         self.max_merges = min(self.max_batch * groups, self.ctas)
-        partials = 2 * self.ctas * self.units
+        partials = 2 * self.ctas * UNITS
         self._at = (12 * self.max_items, 12 * self.max_items + 8 * self.max_merges)
         size = self._at[1] + self.ctas + 1
         self._host = torch.empty(size, dtype=torch.int32, pin_memory=True)
@@ -143,7 +152,7 @@ class TreeAttention:
         if len(kv_indptr_host) - 1 > self.max_batch:
             raise ValueError("batch exceeds max_batch")
         items, cta_items, merges, partials = tree_work_list(
-            kv_indptr_host, draft_indptr_host, self.group, self.hkv, self.units, self.ctas)
+            kv_indptr_host, draft_indptr_host, self.group, self.hkv, self.pair_heads, self.ctas)
         assert len(items) <= self.max_items and len(merges) <= self.max_merges and \
             partials <= len(self._acc)
         self._copied.synchronize()

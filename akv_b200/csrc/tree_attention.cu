@@ -12,9 +12,9 @@
 //
 // Work: the rows of a KV head are (drafted token, query head of the group),
 // row = token * group + head, 128 rows to a tile.  A work item is a run of
-// 64-key tiles of one request for up to `units` (head, row tile) pairs; the
+// 128-key tiles of one request for one or two (head, row tile) units; the
 // host cuts the flat list of all key tiles into equal runs, one per CTA, and
-// a second kernel joins the pieces of requests that were cut.
+// a second kernel joins the pieces of units that were cut.
 
 #include <type_traits>
 
@@ -24,7 +24,8 @@ namespace akv {
 namespace {
 
 constexpr int kTreeRows = 128;
-constexpr int kTreeKeys = 64;
+constexpr int kTreeKeys = 128;
+constexpr int kTreeUnits = 2;
 
 struct TreeItem {   // 12 int32
   int q0, n;        // first drafted token of the request, and their number
@@ -32,8 +33,8 @@ struct TreeItem {   // 12 int32
   int lo, hi;       // keys [lo, hi) of prefix ++ drafted
   int head0, tile0; // unit u: head head0 + u * head_step, row tile tile0 + u * tile_step
   int head_step, tile_step;
-  int units;
-  int partial;      // first partial result (one per unit of the CTA), or -1
+  int units;        // 2: a pair; 1: both units share its keys
+  int partial;      // first partial result (kTreeUnits per item), or -1
 };
 
 struct TreeParams {
@@ -120,6 +121,26 @@ __device__ __forceinline__ RowEnd row_end(const float* sinks, int h, float m, fl
   return e;
 }
 
+// The thread's copies so far, once landed, arrive on an mbarrier.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Zeroes the infinities and NaN of eight elements; true if there were any.
+template <int HALF>
+__device__ __forceinline__ bool scrub(uint4& x) {
+  constexpr uint32_t kExp = HALF ? 0x7c00u : 0x7f80u;
+  uint32_t e[4] = {x.x, x.y, x.z, x.w};
+  bool hit = false;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if ((e[k] & kExp) == kExp) { e[k] &= 0xffff0000u; hit = true; }
+    if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0xffffu; hit = true; }
+  }
+  x = make_uint4(e[0], e[1], e[2], e[3]);
+  return hit;
+}
+
 // ws_wait by a whole warp, which then takes one way.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xffffffffu, ws_wait(bar, parity, abort));
@@ -132,62 +153,125 @@ __device__ __forceinline__ bool key_seen(const TreeParams& p, const TreeItem& w,
   return p.window < 0 || pos - p.kv_positions[w.kv0 + j] <= p.window;
 }
 
-constexpr int tree_units(int head_dim) { return head_dim == 64 ? 2 : 1; }
-
-// Two CTAs per SM, each with 256 tensor-memory columns: per unit, SB score
-// buffers of 64 columns and the accumulator of D (P overwrites its scores).
-// K and V tiles of 64 keys alternate in a ring of 16 KiB slots: at head_dim 64
-// two heads' rows (256 contiguous bytes a key in the usual pools), at 128 one.
-// 256-byte pieces gathered by cp.async from several CTAs per SM reach the
-// copy rate on random slots (6.9 TB/s in a bare gather, against 4.9 for
-// 128-byte pieces and 4.9 for TMA row gathers, whose issue is the limit).
+// One CTA per SM with two units, each with 256 tensor-memory columns: scores
+// of 128 keys, the accumulator of D and, at head_dim 64, P beside them (at 128
+// P overwrites the second half of its scores).  K and V tiles of 128 keys alternate in a ring of
+// 32 KiB slots, one or two heads' rows each.  256-byte pieces gathered by
+// cp.async are what reaches the copy rate on random slots (a bare gather: 6.9
+// TB/s with 256-byte pieces and 16 warps per SM, 5.8 with 8, 4.9 with 128-byte
+// pieces; TMA row gathers stop at 4.9, L2 prefetches cost more than they
+// bring), so at head_dim 64 two heads share a CTA.
 template <int D>
 struct TreeCfg {
-  static constexpr int kUnits = tree_units(D);
-  static constexpr int kBuffers = D == 64 ? 1 : 2;   // score buffers per unit
-  static constexpr int kSoftmax = 4 * kUnits;        // warps
-  static constexpr int kProducers = 2;               // warps
-  static constexpr int kThreads = 32 * (kSoftmax + kProducers + kUnits);
+  static constexpr int kSoftmax = 8, kProducers = 8;  // warps
+  static constexpr int kThreads = 32 * (kSoftmax + kProducers + 4);  // two issuers, two idle
   static constexpr int kHeadBytes = kTreeKeys * D * 2;  // one head's rows of a tile
-  static constexpr int kSlotBytes = 16384;
-  static constexpr int kSlots = 5;
-  static constexpr int kAhead = 3;                   // slots requested before the oldest is awaited
+  static constexpr int kSlotBytes = 32768;
+  static constexpr int kSlots = D == 64 ? 6 : 5;
   static constexpr int kQBytes = kTreeRows * D * 2;
-  static constexpr int kRingOff = kUnits * kQBytes;
-  static constexpr int kBarOff = kRingOff + kSlots * kSlotBytes;
+  static constexpr int kRingOff = 2 * kQBytes;
+  static constexpr int kRowOff = kRingOff + kSlots * kSlotBytes;  // [2][128] (maximum, sum)
+  static constexpr int kBarOff = kRowOff + 2 * kTreeRows * 8;
   static constexpr int kSmem = kBarOff + 256;
-  static constexpr int kUnitCols = 256 / kUnits;
-  static constexpr int kColO = kUnitCols - D;
-  static_assert(kHeadBytes * kUnits == kSlotBytes || kUnits == 1, "slot holds every unit's head");
-  static_assert(kAhead <= kSlots - 2, "a slot is signalled before its successors wait for room");
+  static constexpr int kColP = D == 64 ? 128 : 64, kColO = 256 - D;
+  static_assert(kSmem <= 232448, "shared memory of one CTA");
 };
 
-// Warps: 4 per unit run its softmax (warp w: rows 32 (w % 4) ..), then two
-// producers, then one MMA issuer per unit, so that units never wait for one
-// another.  Per slot: full (every producer thread's copies have landed), empty
-// (each unit's MMAs that read it are done).  Per unit: q (its Q tile is
-// stored), s[b] (scores done), p[b] (P stored), o (every P.V), done (the last
-// P.V of an item).  Waits are bounded; once one runs out the CTA's abort
-// flag ends every role's loop and *error_flag gets bit 2.
+// A position in the slot ring.
+template <int SLOTS>
+struct RingPos {
+  uint32_t slot = 0, phase = 0;
+  __device__ __forceinline__ void advance(uint32_t n) {  // n <= SLOTS
+    slot += n;
+    if (slot >= SLOTS) {
+      slot -= SLOTS;
+      phase ^= 1;
+    }
+  }
+};
+
+// Visible keys among the 64 from j0 on, as bits.  Every lane of the warp calls it.
+__device__ __forceinline__ unsigned long long seen64(const TreeParams& p, const TreeItem& w,
+                                                     unsigned long long mask, long long pos,
+                                                     int j0, int lane) {
+  if (j0 >= w.hi) return 0;
+  const int cached = min(max(w.prefix - j0, 0), 64);
+  unsigned long long seen;
+  if (cached == 0) {
+    seen = mask >> (j0 - w.prefix);  // j0 < hi <= prefix + 64
+  } else {
+    seen = cached < 64 ? mask << cached : 0;
+    if (p.window < 0) {
+      seen |= cached < 64 ? (1ull << cached) - 1 : ~0ull;
+    } else {
+      const int* kp = p.kv_positions + w.kv0 + j0;
+      const int p0 = lane < cached ? kp[lane] : 0;
+      const int p1 = lane + 32 < cached ? kp[lane + 32] : 0;
+      for (int k = 0; k < cached; ++k) {
+        const int kpos = __shfl_sync(0xffffffffu, k < 32 ? p0 : p1, k & 31);
+        if (pos - kpos <= p.window) seen |= 1ull << k;
+      }
+    }
+  }
+  if (w.hi - j0 < 64) seen &= (1ull << (w.hi - j0)) - 1;
+  return seen;
+}
+
+// Infinities and NaN were taken out of V tiles: adds those that a row sees to
+// columns [d0, d1) of its result (out, or the partial acc).
+template <typename T>
+__device__ __noinline__ void restore(const TreeParams& p, const TreeItem& w,
+                                     unsigned long long mask, long long pos, int head, T* out,
+                                     float* acc, int d0, int d1) {
+  for (int j = p.window >= 0 ? w.lo : max(w.lo, w.prefix / kTreeKeys * kTreeKeys); j < w.hi; ++j) {
+    if (!key_seen(p, w, mask, pos, j)) continue;
+    const long long slot = key_slot(p, w, j);
+    if (slot < 0) continue;
+    const T* v = static_cast<const T*>(p.v) + slot * p.v_ss + head * p.v_sh;
+    for (int d = d0; d < d1; ++d) {
+      const float x = Elem<T>::to_f32(v[d]);
+      if (isfinite(x)) continue;
+      if (out) out[d] = Elem<T>::from_f32(Elem<T>::to_f32(out[d]) + x);
+      else acc[d] += x;
+    }
+  }
+}
+
+// Warps 0-3 and 4-7 are the softmax of units 0 and 1 (warp w: rows 32 (w % 4)
+// .., one row per thread), 8-15 the producers,
+// 16 and 17 the MMA issuers, one per unit so that units never wait for one
+// another.  A pair item gives the units different heads or row tiles over
+// the same keys; a single one gives both the same rows and alternate key
+// tiles, and its accumulators are joined out of tensor memory at the end.
+// Barriers.  Per slot: full (every producer thread's copies have landed),
+// empty (the products of both units that read it are done; the unit that
+// reads a single item's slot signals twice).  Per unit: q (its Q tile is
+// stored), s (scores done), f (head_dim 64: the scores are read, so the
+// next product may overwrite them while P is made), p (P stored), o (P.V
+// done).  x: the units meet around the join.  A waiter is never two phases
+// behind: S(c + 1) needs f(c) or o(c), P(c + 1) is stored after o(c).  Waits are
+// bounded; once one runs out the CTA's abort flag ends every role's loop and
+// *error_flag gets bit 2.
 template <typename T, int D>
-__global__ void __launch_bounds__(TreeCfg<D>::kThreads, 2)
-tree_attention_kernel(const TreeParams p) {
+__global__ void __launch_bounds__(TreeCfg<D>::kThreads, 1)
+tree_attention_kernel(const __grid_constant__ TreeParams p) {
   using C = TreeCfg<D>;
-  constexpr int U = C::kUnits, SB = C::kBuffers;
+  using Pos = RingPos<C::kSlots>;
   constexpr int kHalf = std::is_same<T, __half>::value;  // fp16 operands
+  constexpr bool kFree = D == 64;                        // P has columns of its own
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
   const uint32_t bars = base + C::kBarOff;
   auto bar_full = [&](uint32_t s) { return bars + 8u * s; };
   auto bar_empty = [&](uint32_t s) { return bars + 8u * (C::kSlots + s); };
-  constexpr int kUnitBars = 3 + 2 * SB;
-  auto unit_bar = [&](int u, int i) { return bars + 8u * (2 * C::kSlots + u * kUnitBars + i); };
+  auto unit_bar = [&](int u, int i) { return bars + 8u * (2 * C::kSlots + 5 * u + i); };
   auto bar_q = [&](int u) { return unit_bar(u, 0); };
-  auto bar_o = [&](int u) { return unit_bar(u, 1); };
-  auto bar_done = [&](int u) { return unit_bar(u, 2); };
-  auto bar_s = [&](int u, uint32_t b) { return unit_bar(u, 3 + b); };
-  auto bar_p = [&](int u, uint32_t b) { return unit_bar(u, 3 + SB + b); };
-  static_assert(8 * (2 * C::kSlots + U * kUnitBars) + 16 <= 256, "barriers and flags");
+  auto bar_s = [&](int u) { return unit_bar(u, 1); };
+  auto bar_f = [&](int u) { return unit_bar(u, 2); };
+  auto bar_p = [&](int u) { return unit_bar(u, 3); };
+  auto bar_o = [&](int u) { return unit_bar(u, 4); };
+  const uint32_t bar_x = unit_bar(2, 0);
+  static_assert(8 * (2 * C::kSlots + 11) <= 240, "barriers and flags");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOff + 240);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + C::kBarOff + 244);
   volatile int* scrubbed = reinterpret_cast<volatile int*>(smem + C::kBarOff + 248);
@@ -196,23 +280,22 @@ tree_attention_kernel(const TreeParams p) {
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_slot)),
-                 "r"(256));
+                 "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (tid == 32) {
     for (int s = 0; s < C::kSlots; ++s) {
       mbar_init(bar_full(s), 32 * C::kProducers);
-      mbar_init(bar_empty(s), U);
+      mbar_init(bar_empty(s), 2);
     }
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < 2; ++u) {
       mbar_init(bar_q(u), kTreeRows);
+      mbar_init(bar_s(u), 1);
+      mbar_init(bar_f(u), 4);
+      mbar_init(bar_p(u), 4);
       mbar_init(bar_o(u), 1);
-      mbar_init(bar_done(u), 1);
-      for (int b = 0; b < SB; ++b) {
-        mbar_init(bar_s(u, b), 1);
-        mbar_init(bar_p(u, b), 4);
-      }
     }
+    mbar_init(bar_x, C::kSoftmax);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *abort = base & 1023 ? 1 : 0;  // the swizzled tiles need a 1024-byte aligned base
     *scrubbed = 0;
@@ -223,260 +306,226 @@ tree_attention_kernel(const TreeParams p) {
   const uint32_t tmem = *tmem_slot;
   const int it0 = p.cta_items[blockIdx.x], it1 = p.cta_items[blockIdx.x + 1];
 
+  // 640 threads launch with 96 registers; the softmax warps take 144
+  // (256 x 144 + 384 x 64 = 640 x 96).
+  static_assert(C::kSoftmax == 8 && C::kThreads == 640, "register split");
   if (warp >= C::kSoftmax + C::kProducers) {
-    // ---- one MMA issuer per unit ----
-    if (lane == 0) {
-      const int u = warp - C::kSoftmax - C::kProducers;
-      const uint32_t tu = tmem + u * C::kUnitCols;
-      const uint32_t sq = base + u * C::kQBytes;
-      uint32_t seq = 0, cnt = 0, items = 0;  // slots; this unit's tiles and items so far
-      for (int it = it0; it < it1; ++it) {
-        const TreeItem w = p.items[it];
-        const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
-        if (u >= w.units) {  // idle: give the slots back
-          bool ok = true;
-          for (int t = 0; t < 2 * n_tiles && ok; ++t, ++seq) {
-            ok = ws_wait(bar_full(seq % C::kSlots), seq / C::kSlots & 1, abort);
-            if (ok) mbar_arrive(bar_empty(seq % C::kSlots));
-          }
-          if (!ok) break;
-          continue;
-        }
-        if (!ws_wait(bar_q(u), items & 1, abort)) break;
-        const uint32_t head = w.head_step ? u * C::kHeadBytes : 0;
-        auto scores = [&](uint32_t c, uint32_t sk) {  // S(c) = Q K^T
-          tc_fence_after();
-          const uint32_t kb = base + C::kRingOff + sk % C::kSlots * C::kSlotBytes + head;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = 32u * (k & 3);
-            mma_ss(tu + c % SB * kTreeKeys,
-                   sw128_desc(sq + (k >> 2) * kTreeRows * 128 + off),
-                   sw128_desc(kb + (k >> 2) * kTreeKeys * 128 + off),
-                   f16_idesc(kTreeKeys, 0, kHalf), k > 0);
-          }
-          umma_commit(bar_s(u, c % SB));
-          umma_commit(bar_empty(sk % C::kSlots));
+    // ---- MMA issuers: one thread per unit ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const int u = warp - C::kSoftmax - C::kProducers;
+    if (u < 2 && lane == 0) {
+      const uint32_t tu = tmem + 256 * u;
+      const uint64_t qd = sw128_desc(base + u * C::kQBytes);
+      Pos at;  // the item's first K slot
+      uint32_t cnt = 0, n_q = 0;
+      bool ok = true;
+      for (int it = it0; it < it1 && ok; ++it) {
+        const int4 w1 = reinterpret_cast<const int4*>(p.items + it)[1];  // lo, hi, head0, tile0
+        const int4 w2 = reinterpret_cast<const int4*>(p.items + it)[2];  // steps, units, partial
+        const int n_tiles = (w1.y - w1.x + kTreeKeys - 1) / kTreeKeys;
+        const bool pair = w2.z == 2;
+        const int step = pair ? 1 : 2;
+        const int n = pair ? n_tiles : (n_tiles - u + 1) / 2;  // this unit's tiles
+        const uint32_t ring = base + C::kRingOff + (w2.x ? u * C::kHeadBytes : 0);
+        auto release = [&](uint32_t slot) {
+          umma_commit(bar_empty(slot));
+          if (!pair) umma_commit(bar_empty(slot));
         };
-        auto values = [&](uint32_t c, uint32_t sv, bool first, bool last) {  // O += P(c) V
+        // The copies are writes of the generic proxy that the full barrier
+        // has made visible to this thread; the fence orders them before the
+        // products that it issues.
+        auto scores = [&](uint32_t c, const Pos& k) {  // S(c) = Q K^T
+          ok = ok && ws_wait(bar_full(k.slot), k.phase, abort);
+          if (c > 0) ok = ok && ws_wait(kFree ? bar_f(u) : bar_o(u), c - 1 & 1, abort);
+          if (!ok) return;
+          fence_async_smem();
           tc_fence_after();
-          const uint32_t vb = base + C::kRingOff + sv % C::kSlots * C::kSlotBytes + head;
+          const uint64_t kd = sw128_desc(ring + k.slot * C::kSlotBytes);
 #pragma unroll
-          for (int k = 0; k < kTreeKeys / 16; ++k) {  // 16 keys: 8 P columns, 2 KiB of V
-            const uint64_t vd = D == 64 ? sw128_desc(vb + 2048 * k)
-                                        : sw128_desc_mn(vb + 2048 * k, kTreeKeys * 128);
-            mma_ts(tu + C::kColO, tu + c % SB * kTreeKeys + 8 * k, vd, f16_idesc(D, 1, kHalf),
-                   !first || k > 0);
+          for (int i = 0; i < D / 16; ++i) {  // 16 dims a step: 32 bytes of a 64-dim atom
+            const uint32_t off = ((i >> 2) * kTreeKeys * 128 + 32 * (i & 3)) >> 4;
+            mma_ss(tu, qd + off, kd + off, f16_idesc(kTreeKeys, 0, kHalf), i > 0);
           }
+          umma_commit(bar_s(u));
+          release(k.slot);
+        };
+        auto values = [&](uint32_t c, const Pos& v, bool first) {  // O += P(c) V
+          ok = ok && ws_wait(bar_full(v.slot), v.phase, abort) &&
+               ws_wait(bar_p(u), c & 1, abort);
+          if (!ok) return;
+          fence_async_smem();
+          tc_fence_after();
+          const uint32_t vb = ring + v.slot * C::kSlotBytes;
+          const uint64_t vd = D == 64 ? sw128_desc(vb) : sw128_desc_mn(vb, kTreeKeys * 128);
+#pragma unroll
+          for (int i = 0; i < kTreeKeys / 16; ++i)  // 16 keys: 8 P columns, 2 KiB of V
+            mma_ts(tu + C::kColO, tu + C::kColP + 8 * i, vd + (2048 * i >> 4),
+                   f16_idesc(D, 1, kHalf), !first || i > 0);
           umma_commit(bar_o(u));
-          umma_commit(bar_empty(sv % C::kSlots));
-          if (last) umma_commit(bar_done(u));
+          release(v.slot);
         };
-        bool ok = true;
-        // With two score buffers S(t) is issued before P(t-1).V(t-1), so the
-        // softmax never waits for a product; with one, after it is done.
-        for (int t = 0; t < n_tiles + SB - 1 && ok; ++t) {
-          if (t < n_tiles) {
-            const uint32_t sk = seq + 2 * t;
-            ok = ws_wait(bar_full(sk % C::kSlots), sk / C::kSlots & 1, abort);
-            // The buffer's last product is done: of SB tiles before or, as an
-            // item begins, the last one of the item before (all were issued).
-            if (ok && t >= SB) ok = ws_wait(bar_o(u), cnt + t - SB & 1, abort);
-            if (ok && t == 0 && cnt > 0) ok = ws_wait(bar_o(u), cnt - 1 & 1, abort);
-            if (!ok) break;
-            scores(cnt + t, sk);
+        if (n > 0) {
+          ok = ws_wait(bar_q(u), n_q++ & 1, abort);
+          Pos k = at;
+          if (!pair && u) k.advance(2);
+          if (kFree) scores(cnt, k);
+          for (int i = 0; i < n && ok; ++i) {
+            Pos v = k, next = k;
+            v.advance(1);
+            next.advance(2 * step);
+            // With P in columns of its own the next scores are made during
+            // this tile's softmax; otherwise once its P.V is done.
+            if (!kFree) scores(cnt + i, k);
+            else if (i + 1 < n) scores(cnt + i + 1, next);
+            values(cnt + i, v, i == 0);
+            k = next;
           }
-          const int v = t - (SB - 1);
-          if (v >= 0) {
-            const uint32_t c = cnt + v, sv = seq + 2 * v + 1;
-            ok = ws_wait(bar_full(sv % C::kSlots), sv / C::kSlots & 1, abort) &&
-                 ws_wait(bar_p(u, c % SB), c / SB & 1, abort);
-            if (!ok) break;
-            values(c, sv, v == 0, v == n_tiles - 1);
-          }
+          cnt += n;
         }
-        if (!ok) break;
-        seq += 2 * n_tiles;
-        cnt += n_tiles;
-        ++items;
+        const uint32_t end = at.slot + 2 * n_tiles;
+        at.phase ^= end / C::kSlots & 1;
+        at.slot = end % C::kSlots;
       }
     }
     __syncwarp();
   } else if (warp >= C::kSoftmax) {
-    // ---- producers: warp pw gathers keys 32 pw .. of every tile ----
+    // ---- producers: warp pw gathers keys 16 pw .. of every tile ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    constexpr int kKpw = kTreeKeys / C::kProducers;
     const int pw = warp - C::kSoftmax;
-    static_assert(kTreeKeys == 32 * C::kProducers, "one key per producer lane");
-    uint32_t seq = 0;
-    // Signals slot `s` (its copies have landed); a V slot of a guarded tile
-    // is first searched for infinities and NaN, which P = 0 would not mask.
-    uint32_t guard = 0;  // bit a: the slot requested a slots ago is a guarded V tile
-    int cpk = 0;         // 16-byte chunks per key of the current item, and of guarded slots
-    auto signal = [&](uint32_t s, bool guarded, int chunks) {
-      if (guarded) {
-        unsigned char* tile = smem + C::kRingOff + s % C::kSlots * C::kSlotBytes;
-        const int per = 32 / chunks;
-        for (int i = 0; i < 32 / per; ++i) {
-          const int key = 32 * pw + i * per + lane / chunks, c = lane % chunks;
-          uint4* at = reinterpret_cast<uint4*>(tile + c / (D / 8) * C::kHeadBytes +
-                                               sw_chunk(kTreeKeys, key, c % (D / 8)));
-          uint4 x = *at;
-          uint32_t* e = reinterpret_cast<uint32_t*>(&x);
-          bool hit = false;
-          constexpr uint32_t kExp = kHalf ? 0x7c00u : 0x7f80u;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if ((e[k] & kExp) == kExp) { e[k] &= 0xffff0000u; hit = true; }
-            if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0xffffu; hit = true; }
-          }
-          if (hit) {
-            *at = x;
-            *scrubbed = 1;
-          }
-        }
-      }
-      fence_async_smem();
-      mbar_arrive(bar_full(s % C::kSlots));
-    };
-    int old_cpk = 0;
+    Pos at;
     bool ok = true;
-    for (int it = it0; it < it1; ++it) {
+    for (int it = it0; it < it1 && ok; ++it) {
       const TreeItem w = p.items[it];
       const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
-      cpk = (w.head_step ? w.units : 1) * (D / 8);
+      const int heads = w.head_step ? 2 : 1;
       auto fetch = [&](int t) {
-        const int j = w.lo + t * kTreeKeys + 32 * pw + lane;
+        const int j = w.lo + t * kTreeKeys + kKpw * pw + lane % kKpw;
         return t < n_tiles && j < w.hi ? (int)key_slot(p, w, j) : -1;
       };
       int next = fetch(0);
-      for (int t = 0; t < n_tiles; ++t) {
+      for (int t = 0; t < n_tiles && ok; ++t) {
         const int slot = next;
         next = fetch(t + 1);
+        // An infinity or NaN of a V row that only some rows see would reach
+        // the others as 0 * V: tiles with drafted tokens or a window are
+        // searched for them before they are handed on.
         const bool guarded = p.window >= 0 || w.lo + (t + 1) * kTreeKeys > w.prefix;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++seq) {
-          if (!warp_wait(bar_empty(seq % C::kSlots), (seq / C::kSlots & 1) ^ 1, abort)) {
-            ok = false;
-            break;
-          }
-          const uint32_t dst = base + C::kRingOff + seq % C::kSlots * C::kSlotBytes;
-          const T* pool = static_cast<const T*>(kv ? p.v : p.k) +
-                          w.head0 * (kv ? p.v_sh : p.k_sh);
+        for (int kv = 0; kv < 2; ++kv) {
+          ok = warp_wait(bar_empty(at.slot), at.phase ^ 1, abort);
+          if (!ok) break;
           const long long ss = kv ? p.v_ss : p.k_ss, sh = kv ? p.v_sh : p.k_sh;
-          auto copy = [&](auto chunks) {
+          auto copy = [&](auto chunks) {  // chunks: 16-byte pieces per key
             constexpr int kCpk = decltype(chunks)::value, kPer = 32 / kCpk;
             const int c = lane % kCpk, hh = c / (D / 8), cc = c % (D / 8);
-            const T* src = pool + hh * sh + cc * 8;
+            const T* src = static_cast<const T*>(kv ? p.v : p.k) + (w.head0 + hh) * sh + cc * 8;
+            const uint32_t off = C::kRingOff + at.slot * C::kSlotBytes + hh * C::kHeadBytes;
 #pragma unroll
-            for (int i = 0; i < 32 / kPer; ++i) {
-              const int kk = i * kPer + lane / kCpk, key = 32 * pw + kk;
+            for (int i = 0; i < kKpw / kPer; ++i) {
+              const int kk = i * kPer + lane / kCpk;
               const int sl = __shfl_sync(0xffffffffu, slot, kk);
-              cp_async16(dst + hh * C::kHeadBytes + sw_chunk(kTreeKeys, key, cc),
+              cp_async16(base + off + sw_chunk(kTreeKeys, kKpw * pw + kk, cc),
                          src + (sl < 0 ? 0 : sl) * ss, sl < 0 ? 0 : 16);
             }
+            if (kv == 0 || !guarded) {
+              cp_async_arrive(bar_full(at.slot));
+              return;
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            bool hit = false;
+            for (int i = 0; i < kKpw / kPer; ++i) {  // the pieces that this thread copied
+              const int key = kKpw * pw + i * kPer + lane / kCpk;
+              uint4* v = reinterpret_cast<uint4*>(smem + off + sw_chunk(kTreeKeys, key, cc));
+              uint4 x = *v;
+              if (scrub<kHalf>(x)) {
+                *v = x;
+                hit = true;
+              }
+            }
+            if (hit) *scrubbed = 1;
+            fence_async_smem();
+            mbar_arrive(bar_full(at.slot));
           };
-          if (cpk == 16) copy(std::integral_constant<int, 16>());
+          if (heads * (D / 8) == 16) copy(std::integral_constant<int, 16>());
           else copy(std::integral_constant<int, 8>());
-          cp_async_commit();
-          guard = guard << 1 | (uint32_t)(kv && guarded);
-          if (seq >= C::kAhead - 1) {
-            cp_async_wait<C::kAhead - 1>();
-            const uint32_t ago = C::kAhead - 1;
-            // The slot of `ago` requests before: of this item, or of the one before it.
-            signal(seq - ago, guard >> ago & 1, 2 * t + kv >= (int)ago ? cpk : old_cpk);
-          }
+          at.advance(1);
         }
-        if (!ok) break;
       }
-      if (!ok) break;
-      // An item has at least one tile (two slots), so the slots still to be
-      // signalled are of the current item and, for one of them, the last.
-      old_cpk = cpk;
     }
-    if (ok) {
-      cp_async_wait<0>();
-#pragma unroll
-      for (int ago = C::kAhead - 2; ago >= 0; --ago)
-        if (seq >= (uint32_t)ago + 1) signal(seq - 1 - ago, guard >> ago & 1, cpk);
-    }
+    cp_async_commit();
     cp_async_wait<0>();
   } else {
-    // ---- softmax: warp w serves unit w / 4 and its rows 32 (w % 4) .. ----
+    // ---- softmax ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int u = warp >> 2, r = tid & (kTreeRows - 1);
-    const uint32_t tu = tmem + u * C::kUnitCols + ((uint32_t)(warp & 3) << 21);
-    uint32_t cnt = 0, items = 0;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's TMEM lanes
+    const uint32_t tu = tmem + 256 * u + lanes;
+    float2* rows = reinterpret_cast<float2*>(smem + C::kRowOff);
+    uint32_t cnt = 0, n_x = 0;
     for (int it = it0; it < it1; ++it) {
       const TreeItem w = p.items[it];
-      if (u >= w.units) continue;
       const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
+      const bool pair = w.units == 2;
+      const int n = pair ? n_tiles : (n_tiles - u + 1) / 2;
       const int head = w.head0 + u * w.head_step;
       const int row0 = (w.tile0 + u * w.tile_step) * kTreeRows;
       const int i = (row0 + r) / p.group, h = head * p.group + (row0 + r) - i * p.group;
       const bool live = i < w.n;
       const bool warp_live = row0 + (warp & 3) * 32 < w.n * p.group;
-      if (live) {
-        const uint4* src = reinterpret_cast<const uint4*>(
-            static_cast<const T*>(p.q) + (long long)(w.q0 + i) * p.q_st + (long long)h * p.q_sh);
-        unsigned char* dst = smem + u * C::kQBytes;
+      if (n > 0) {
+        if (live) {
+          const uint4* src = reinterpret_cast<const uint4*>(
+              static_cast<const T*>(p.q) + (long long)(w.q0 + i) * p.q_st + (long long)h * p.q_sh);
+          unsigned char* dst = smem + u * C::kQBytes;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-          *reinterpret_cast<uint4*>(dst + sw_chunk(kTreeRows, r, c)) = src[c];
+          for (int c = 0; c < D / 8; ++c)
+            *reinterpret_cast<uint4*>(dst + sw_chunk(kTreeRows, r, c)) = src[c];
+        }
+        fence_async_smem();
+        mbar_arrive(bar_q(u));
       }
-      fence_async_smem();
-      mbar_arrive(bar_q(u));
       const unsigned long long mask = live ? row_mask(p, w, i) : 0;
       const long long pos = live && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int t = 0; t < n_tiles; ++t) {
-        const uint32_t c = cnt + t, b = c % SB;
-        ok = warp_wait(bar_s(u, b), c / SB & 1, abort);
+      for (int v = 0; v < n && ok; ++v) {
+        const uint32_t c = cnt + v;
+        const int j0 = w.lo + (pair ? v : 2 * v + u) * kTreeKeys;
+        ok = warp_wait(bar_s(u), c & 1, abort);
         if (!ok) break;
         if (warp_live) {
           tc_fence_after();
-          const uint32_t ts = tu + b * kTreeKeys;
-          const int j0 = w.lo + t * kTreeKeys;
-          unsigned long long seen = ~0ull;
+          unsigned long long seen[2] = {~0ull, ~0ull};
           if (p.window >= 0 || j0 + kTreeKeys > w.prefix) {
-            const int cached = min(max(w.prefix - j0, 0), kTreeKeys);
-            seen = cached == 0          ? mask >> (j0 - w.prefix)
-                   : cached < kTreeKeys ? mask << cached
-                                        : 0;
-            if (p.window < 0) {
-              seen |= cached == kTreeKeys ? ~0ull : (1ull << cached) - 1;
-            } else {
-              const int* kp = p.kv_positions + w.kv0 + j0;
-              const int p0 = lane < cached ? kp[lane] : 0;
-              const int p1 = lane + 32 < cached ? kp[lane + 32] : 0;
-              for (int k = 0; k < cached; ++k) {
-                const int kpos = __shfl_sync(0xffffffffu, k < 32 ? p0 : p1, k & 31);
-                if (pos - kpos <= p.window) seen |= 1ull << k;
+            seen[0] = seen64(p, w, mask, pos, j0, lane);
+            seen[1] = seen64(p, w, mask, pos, j0 + 64, lane);
+          }
+          const bool masked = __any_sync(0xffffffffu, (seen[0] & seen[1]) != ~0ull);
+          // 64 scores at a time are in registers: the first half is read
+          // for the maximum, the second for both, then the first again.
+          float s[64];
+          auto half = [&](int b) {
+            tmem_ld64_sync(tu + 64 * b, s);
+            if (masked) {
+              const uint32_t lo = (uint32_t)seen[b], hi = (uint32_t)(seen[b] >> 32);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                s[k] = lo >> k & 1 ? s[k] : -INFINITY;
+                s[k + 32] = hi >> k & 1 ? s[k + 32] : -INFINITY;
               }
             }
-            if (j0 + kTreeKeys > w.hi) seen &= (1ull << (w.hi - j0)) - 1;
-          }
-          const bool masked = __any_sync(0xffffffffu, seen != ~0ull);
-          // The scores stay in tensor memory and are read twice, 32 columns
-          // at a time (for the maximum, for P): 64 of them in registers
-          // spill at the 80 that two CTAs leave a thread.
-          auto scores32 = [&](int half, float(&s)[32]) {
-            tmem_ld32_sync(ts + 32 * half, s);
-            if (masked) {
-              const uint32_t bits = (uint32_t)(seen >> 32 * half);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) s[k] = bits >> k & 1 ? s[k] : -INFINITY;
-            }
           };
-          float bm;
-          {
-            float s[32], m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              scores32(half, s);
+          for (int b = 0; b < 2; ++b) {
+            half(b);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], s[k]);
-            }
-            bm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+            for (int k = 0; k < 64; k += 2)
+              m4[k >> 1 & 3] = fmaxf(m4[k >> 1 & 3], fmaxf(s[k], s[k + 1]));
           }
+          const float bm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
           // The base only moves when the tile exceeds it by 2^8; then l and
           // O are rescaled.
           float alpha = 1.f;
@@ -488,32 +537,40 @@ tree_attention_kernel(const TreeParams p) {
           }
           const float nb = m == -INFINITY ? 0.f : -m;
           const f32x2 scale2 = f2_pack(p.scale_log2, p.scale_log2), nb2 = f2_pack(nb, nb);
-          f32x2 sum0 = f2_pack(0.f, 0.f), sum1 = sum0;
-          // P in two halves, each stored over the first columns of its
-          // scores, which this warp has read.
+          f32x2 sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t pk[16];
-            float s[32];
-            scores32(half, s);
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              float x0, x1;
-              f2_unpack(f2_fma(f2_pack(s[k], s[k + 1]), scale2, nb2), x0, x1);
-              x0 = fast_exp2(x0);
-              x1 = fast_exp2(x1);
-              if (k & 2) sum1 = f2_add(sum1, f2_pack(x0, x1));
-              else sum0 = f2_add(sum0, f2_pack(x0, x1));
-              pk[k / 2] = pack2<T>(x0, x1);
+          for (int b = 1; b >= 0; --b) {
+            if (b == 0) {
+              half(0);
+              if (kFree) {  // every score of the tile is read
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_f(u));
+              }
             }
-            tmem_st16_sync(ts + 16 * half, pk);
+#pragma unroll
+            for (int q = 0; q < 64; q += 32) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                float x0, x1;
+                f2_unpack(f2_fma(f2_pack(s[q + k], s[q + k + 1]), scale2, nb2), x0, x1);
+                x0 = fast_exp2(x0);
+                x1 = fast_exp2(x1);
+                sum[k >> 1 & 1] = f2_add(sum[k >> 1 & 1], f2_pack(x0, x1));
+                pk[k / 2] = pack2<T>(x0, x1);
+              }
+              // P's columns, and O's, are free once the product before is
+              // done (with P over the scores S(c) came after it).
+              if (b == 1 && q == 0 && kFree && c > 0)
+                ok = warp_wait(bar_o(u), c - 1 & 1, abort);
+              tmem_st16_sync(tu + C::kColP + (32 * b + q / 2), pk);
+            }
           }
           float l0, l1;
-          f2_unpack(f2_add(sum0, sum1), l0, l1);
+          f2_unpack(f2_add(sum[0], sum[1]), l0, l1);
           l = l * alpha + (l0 + l1);
           if (__any_sync(0xffffffffu, rescale)) {
-            // With one score buffer S(t) came after P(t-1).V(t-1).
-            if (SB > 1) ok = warp_wait(bar_o(u), c - 1 & 1, abort);
             tc_fence_after();
 #pragma unroll
             for (int d = 0; d < D; d += 32) {
@@ -526,65 +583,84 @@ tree_attention_kernel(const TreeParams p) {
             }
           }
           tc_fence_before();
+        } else if (kFree) {
+          if (lane == 0) mbar_arrive(bar_f(u));
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p(u, b));
+        if (lane == 0) mbar_arrive(bar_p(u));
       }
       if (!ok) break;
-      cnt += n_tiles;
-      if (!warp_wait(bar_done(u), items & 1, abort)) break;
-      ++items;
-      if (!warp_live) continue;
+      cnt += n;
+      if (n > 0 && !warp_wait(bar_o(u), cnt - 1 & 1, abort)) break;
       tc_fence_after();
-      const bool direct = w.partial < 0;
-      const long long at = ((long long)w.partial + u) * kTreeRows + r;
-      const RowEnd e = row_end(p.sinks, live ? h : 0, m, l);
-      T* dst = static_cast<T*>(p.out) + (long long)(w.q0 + i) * p.o_st + (long long)h * p.o_sh;
-#pragma unroll
-      for (int d = 0; d < D; d += 32) {
-        float o[32];
+      float f[2] = {1.f, 0.f};
+      if (!pair) {  // the two units' rows meet
+        rows[u * kTreeRows + r] = make_float2(m, l);
+        tc_fence_before();
         __syncwarp();
-        tmem_ld32_sync(tu + C::kColO + d, o);
-        if (!live) continue;
-        if (*scrubbed) {
-          // Infinities and NaN were taken out of guarded V tiles: the rows
-          // that see them get them here.
-          for (int j = p.window >= 0 ? w.lo : max(w.lo, w.prefix & ~(kTreeKeys - 1)); j < w.hi;
-               ++j) {
-            if (!key_seen(p, w, mask, pos, j)) continue;
-            const long long slot = key_slot(p, w, j);
-            if (slot < 0) continue;
-            const T* v = static_cast<const T*>(p.v) + slot * p.v_ss + head * p.v_sh + d;
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float x = Elem<T>::to_f32(v[k]);
-              if (!isfinite(x)) o[k] += x;
-            }
-          }
-        }
-        if (direct) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            uint4 x;
-            x.x = pack2<T>(o[k] * e.scale, o[k + 1] * e.scale);
-            x.y = pack2<T>(o[k + 2] * e.scale, o[k + 3] * e.scale);
-            x.z = pack2<T>(o[k + 4] * e.scale, o[k + 5] * e.scale);
-            x.w = pack2<T>(o[k + 6] * e.scale, o[k + 7] * e.scale);
-            *reinterpret_cast<uint4*>(dst + d + k) = x;
-          }
-        } else {
-          float4* acc = reinterpret_cast<float4*>(p.part_acc + at * D + d);
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) acc[k / 4] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-        }
+        if (lane == 0) mbar_arrive(bar_x);
+        if (!warp_wait(bar_x, n_x++ & 1, abort)) break;
+        tc_fence_after();
+        const float2 a = rows[r], b = rows[kTreeRows + r];
+        m = fmaxf(a.x, b.x);
+        const float top = m == -INFINITY ? 0.f : m;
+        f[0] = fast_exp2(a.x - top);
+        f[1] = fast_exp2(b.x - top);
+        l = a.y * f[0] + b.y * f[1];
       }
-      if (live && !direct) {
-        p.part_ml[2 * at] = m;
-        p.part_ml[2 * at + 1] = l;
-      } else if (live && p.lse) {
-        p.lse[(long long)(w.q0 + i) * p.num_q_heads + h] = e.lse;
+      if (warp_live) {
+        const bool direct = w.partial < 0;
+        const long long at = ((long long)w.partial + (pair ? u : 0)) * kTreeRows + r;
+        const RowEnd e = row_end(p.sinks, live ? h : 0, m, l);
+        T* dst = static_cast<T*>(p.out) + (long long)(w.q0 + i) * p.o_st + (long long)h * p.o_sh;
+        // A pair's units write all their columns, a single item's half each.
+        const int d0 = pair ? 0 : u * (D / 2), d1 = pair ? D : d0 + D / 2;
+        for (int d = d0; d < d1; d += 32) {
+          float o[32];
+          __syncwarp();
+          tmem_ld32_sync(tmem + lanes + (pair ? 256 * u : 0) + C::kColO + d, o);
+          if (!pair) {
+            float o1[32];
+            if (n_tiles > 1) tmem_ld32_sync(tmem + lanes + 256 + C::kColO + d, o1);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = o[k] * f[0] + (n_tiles > 1 ? o1[k] * f[1] : 0.f);
+          }
+          if (!live) continue;
+          if (direct) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              uint4 x;
+              x.x = pack2<T>(o[k] * e.scale, o[k + 1] * e.scale);
+              x.y = pack2<T>(o[k + 2] * e.scale, o[k + 3] * e.scale);
+              x.z = pack2<T>(o[k + 4] * e.scale, o[k + 5] * e.scale);
+              x.w = pack2<T>(o[k + 6] * e.scale, o[k + 7] * e.scale);
+              *reinterpret_cast<uint4*>(dst + d + k) = x;
+            }
+          } else {
+            float4* acc = reinterpret_cast<float4*>(p.part_acc + at * D + d);
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              acc[k / 4] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          }
+        }
+        if (live && *scrubbed)
+          restore<T>(p, w, mask, pos, head, direct ? dst : nullptr,
+                     direct ? nullptr : p.part_acc + at * D, d0, d1);
+        if (live && (pair || u == 0)) {
+          if (!direct) {
+            p.part_ml[2 * at] = m;
+            p.part_ml[2 * at + 1] = l;
+          } else if (p.lse) {
+            p.lse[(long long)(w.q0 + i) * p.num_q_heads + h] = e.lse;
+          }
+        }
       }
       tc_fence_before();  // O's reads before the next item's products
+      if (!pair) {        // of either unit
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_x);
+        if (!warp_wait(bar_x, n_x++ & 1, abort)) break;
+      }
     }
   }
   tc_fence_before();
@@ -593,7 +669,7 @@ tree_attention_kernel(const TreeParams p) {
   if (tid == 0 && *abort && p.error_flag) atomicOr(p.error_flag, 2);
   if (warp == 0) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
 }
 
@@ -607,7 +683,7 @@ constexpr int kMergeWarps = 8;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kMergeWarps)
-tree_merge_kernel(const TreeParams p, const TreeMerge* merges, int units) {
+tree_merge_kernel(const TreeParams p, const TreeMerge* merges) {
   const TreeMerge g = merges[blockIdx.x];
   const int lane = threadIdx.x & 31;
   const int u = blockIdx.y / (kTreeRows / kMergeWarps);
@@ -618,7 +694,7 @@ tree_merge_kernel(const TreeParams p, const TreeMerge* merges, int units) {
   const int i = row / p.group, h = head * p.group + row % p.group;
   if (i >= g.n) return;
   pdl_wait();
-  const long long step = (long long)units * kTreeRows;  // rows between two pieces
+  const long long step = (long long)kTreeUnits * kTreeRows;  // rows between two pieces
   const long long at = ((long long)g.first + u) * kTreeRows + r;
   float m = -INFINITY;
   for (int s = lane; s < g.count; s += 32) m = fmaxf(m, p.part_ml[2 * (at + s * step)]);
@@ -652,8 +728,8 @@ int launch_tree(const TreeParams& p, int n_ctas, const TreeMerge* merges, int n_
     return AKV_ERR_CUDA;
   tree_attention_kernel<T, D><<<n_ctas, C::kThreads, C::kSmem, s>>>(p);
   if (n_merges > 0 &&
-      launch_pdl(tree_merge_kernel<T, D>, dim3(n_merges, C::kUnits * (kTreeRows / kMergeWarps)),
-                 dim3(32 * kMergeWarps), 0, s, p, merges, (int)C::kUnits) != cudaSuccess)
+      launch_pdl(tree_merge_kernel<T, D>, dim3(n_merges, kTreeUnits * (kTreeRows / kMergeWarps)),
+                 dim3(32 * kMergeWarps), 0, s, p, merges) != cudaSuccess)
     return AKV_ERR_CUDA;
   return launch_status();
 }
@@ -661,9 +737,7 @@ int launch_tree(const TreeParams& p, int n_ctas, const TreeMerge* merges, int n_
 }  // namespace
 }  // namespace akv
 
-extern "C" int32_t akv_tree_attention_units(int32_t head_dim) {
-  return head_dim == 64 || head_dim == 128 ? akv::tree_units(head_dim) : -AKV_ERR_UNSUPPORTED;
-}
+extern "C" int32_t akv_tree_attention_units(void) { return akv::kTreeUnits; }
 
 extern "C" int akv_tree_attention(
     const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_pool,

@@ -762,10 +762,10 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_token, int64_t q_stride_hea
  * items: DEVICE int32 [n][12] = {q0, drafted tokens (at most 64), kv0, cached
  * keys, first key, end key, head0, tile0, head_step, tile_step, units,
  * partial}: keys [first, end) of the cached keys followed by the drafted
- * tokens, first a multiple of 64; unit u < units <=
- * akv_tree_attention_units(head_dim) is KV head head0 + u * head_step and rows
- * [128 tile, 128 tile + 128), tile = tile0 + u * tile_step, row = token *
- * group + query head of the group; partial -1 writes the output, otherwise
+ * tokens, first a multiple of 128; with units 2, unit u is KV head head0 + u *
+ * head_step and rows [128 tile, 128 tile + 128), tile = tile0 + u *
+ * tile_step, row = token * group + query head of the group; units 1 (both
+ * steps 0): that of unit 0 alone; partial -1 writes the output, otherwise
  * unit u writes partial result partial + u.  cta_items: DEVICE int32 [n_ctas +
  * 1], CTA c runs items [cta_items[c], cta_items[c + 1]).  merges: DEVICE
  * int32 [n_merges][8] = {q0, tokens, head0, tile0, head_step | tile_step << 1
@@ -778,7 +778,7 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_token, int64_t q_stride_hea
  * pools, read as slot 0) and 2 (a wait ran out: the launch's output is
  * invalid); [1] is the launch's abort word, cleared by every launch.
  */
-int32_t akv_tree_attention_units(int32_t head_dim);
+int32_t akv_tree_attention_units(void);
 int akv_tree_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head,
                        const void* k_pool, const void* v_pool, int64_t k_stride_slot,
                        int64_t k_stride_head, int64_t v_stride_slot, int64_t v_stride_head,

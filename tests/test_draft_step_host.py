@@ -115,28 +115,28 @@ def test_tree_attention_of_nothing_is_ok_and_other_head_dims_are_unsupported():
 
     assert _native.lib.akv_tree_attention(*tree_args(n_ctas=0)) == _native.AKV_OK
     assert _native.lib.akv_tree_attention(*tree_args(dim=96)) == _native.AKV_ERR_UNSUPPORTED
-    assert _native.lib.akv_tree_attention_units(64) > 0
-    assert _native.lib.akv_tree_attention_units(96) < 0
+    assert _native.lib.akv_tree_attention_units() == 2
 
 
-@pytest.mark.parametrize("units", [1, 2, 4])
+@pytest.mark.parametrize("pair_heads", [False, True])
 @pytest.mark.parametrize("hkv,group", [(8, 8), (1, 8), (3, 5), (2, 40)])
 @pytest.mark.parametrize("ctas", [1, 7, 296])
-def test_tree_work_list_covers_every_key_of_every_row_once(units, hkv, group, ctas):
+def test_tree_work_list_covers_every_key_of_every_row_once(pair_heads, hkv, group, ctas):
     import numpy as np
 
     from akv_b200.context_tree import tree_work_list
 
-    rng = np.random.default_rng(units * hkv + ctas)
-    cached = np.r_[0, 1, 64, rng.integers(0, 3000, 9)]
+    rng = np.random.default_rng(pair_heads + 2 * hkv + ctas)
+    cached = np.r_[0, 1, 128, rng.integers(0, 3000, 9)]
     new = np.r_[1, 0, 64, rng.integers(0, 65, 9)]
     kv, dr = (np.concatenate(([0], np.cumsum(x))) for x in (cached, new))
-    items, cta_items, merges, partials = tree_work_list(kv, dr, group, hkv, units, ctas)
+    items, cta_items, merges, partials = tree_work_list(kv, dr, group, hkv, pair_heads, ctas)
     seen, parts = {}, {}
     for q0, n, kv0, prefix, lo, hi, h0, t0, hs, ts, u_n, partial in items.tolist():
         b = int(np.searchsorted(dr, q0, side="right")) - 1
         assert (q0, n, kv0, prefix) == (dr[b], new[b], kv[b], cached[b]) and n > 0
-        assert 0 < u_n <= units and hs + ts == 1 and lo % 64 == 0 and lo < hi <= prefix + n
+        assert u_n in (1, 2) and hs + ts == u_n - 1 and lo % 128 == 0 and lo < hi <= prefix + n
+        assert pair_heads or not hs
         for u in range(u_n):
             key = (b, h0 + u * hs, t0 + u * ts)
             assert key[1] < hkv and key[2] * 128 < n * group
@@ -151,21 +151,21 @@ def test_tree_work_list_covers_every_key_of_every_row_once(units, hkv, group, ct
     assert not seen
     used = sorted(p for v in parts.values() for p in v if p >= 0)
     assert len(set(used)) == len(used) and (not used or used[-1] < partials)
-    assert partials <= 2 * ctas * units
+    assert partials <= 4 * ctas
     joined = set()
     for q0, n, h0, t0, steps, first, count, _ in merges.tolist():
         b = int(np.searchsorted(dr, q0, side="right")) - 1
         assert n == new[b] and count > 1
         for u in range(steps >> 2):
             key = (b, h0 + u * (steps & 1), t0 + u * (steps >> 1 & 1))
-            assert sorted(parts[key]) == [first + u + i * units for i in range(count)]
+            assert sorted(parts[key]) == [first + u + 2 * i for i in range(count)]
             joined.add(key)
     assert joined == {k for k, v in parts.items() if v[0] >= 0}
     assert all(len(v) == 1 for k, v in parts.items() if k not in joined)
     assert cta_items[0] == 0 and cta_items[-1] == len(items) and np.all(np.diff(cta_items) >= 0)
-    tiles = -(-(items[:, 5] - items[:, 4]) // 64)
-    load = np.add.reduceat(tiles, cta_items[:-1]) if len(items) else tiles
-    assert load.max() - load.min() <= 1
+    cost = -(-(items[:, 5] - items[:, 4]) // 128) * items[:, 10]
+    load = np.add.reduceat(cost, cta_items[:-1])
+    assert load.max() - load.min() <= 3
 
 
 def test_tree_work_list_refuses():
@@ -174,4 +174,4 @@ def test_tree_work_list_refuses():
     for kv, dr in (([0, 5], [0]), ([0, 5], [0, 65]), ([5, 0], [0, 1]), ([0, 5], [1, 0]), ([], []),
                    ([0, 1 << 31], [0, 1])):
         with pytest.raises(ValueError):
-            tree_work_list(kv, dr, 8, 8, 2, 10)
+            tree_work_list(kv, dr, 8, 8, True, 10)
