@@ -26,6 +26,7 @@ namespace {
 constexpr int kTreeRows = 128;
 constexpr int kTreeKeys = 128;
 constexpr int kTreeUnits = 2;
+constexpr uint32_t kPoly = 0x1111;  // pairs of sixteen whose exponentials are polynomials
 
 struct TreeItem {   // 12 int32
   int q0, n;        // first drafted token of the request, and their number
@@ -116,9 +117,46 @@ __device__ __forceinline__ RowEnd row_end(const float* sinks, int h, float m, fl
   const float f = fast_exp2(m - base);
   const float den = l * f + fast_exp2(sink - base);
   RowEnd e;
-  e.scale = den > 0.f ? f / den : 0.f;
-  e.lse = den > 0.f ? (base + log2f(den)) * kLn2 : -INFINITY;
+  e.scale = den == 0.f ? 0.f : f / den;  // NaN stays NaN
+  e.lse = den == 0.f ? -INFINITY : (base + log2f(den)) * kLn2;
   return e;
+}
+
+__device__ __forceinline__ void cp_async16_full(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
+}
+
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x for a pair on the FMA pipes, so that they share the exponentials with
+// the special-function unit: x = i + f with i the nearest integer (the low
+// bits of x + 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial of degree 5 with
+// constant term 1, fitted for the least relative error (9.1e-8), and i added to
+// the exponent field.  At x <= -127 the result is exactly 0.  A NaN is lost
+// (the caller's maximum sees it).
+__device__ __forceinline__ void exp2_pair(f32x2 x, float& e0, float& e1) {
+  float x0, x1;
+  f2_unpack(x, x0, x1);
+  x = f2_pack(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
+  const f32x2 magic = f2_pack(12582912.f, 12582912.f);
+  const f32x2 t = f2_add(x, magic);
+  const f32x2 f = f2_sub(x, f2_sub(t, magic));
+  f32x2 y = f2_pack(0x1.5bba14p-10f, 0x1.5bba14p-10f);
+  y = f2_fma(y, f, f2_pack(0x1.3cea88p-7f, 0x1.3cea88p-7f));
+  y = f2_fma(y, f, f2_pack(0x1.c6b752p-5f, 0x1.c6b752p-5f));
+  y = f2_fma(y, f, f2_pack(0x1.ebf9bcp-3f, 0x1.ebf9bcp-3f));
+  y = f2_fma(y, f, f2_pack(0x1.62e42ap-1f, 0x1.62e42ap-1f));
+  y = f2_fma(y, f, f2_pack(1.f, 1.f));
+  float t0, t1, y0, y1;
+  f2_unpack(t, t0, t1);
+  f2_unpack(y, y0, y1);
+  e0 = __int_as_float(__float_as_int(y0) + (__float_as_int(t0) << 23));
+  e1 = __int_as_float(__float_as_int(y1) + (__float_as_int(t1) << 23));
 }
 
 // The thread's copies so far, once landed, arrive on an mbarrier.
@@ -163,8 +201,8 @@ __device__ __forceinline__ bool key_seen(const TreeParams& p, const TreeItem& w,
 // bring), so at head_dim 64 two heads share a CTA.
 template <int D>
 struct TreeCfg {
-  static constexpr int kSoftmax = 8, kProducers = 8;  // warps
-  static constexpr int kThreads = 32 * (kSoftmax + kProducers + 4);  // two issuers, two idle
+  static constexpr int kSoftmax = 8, kProducers = 4;  // warps
+  static constexpr int kThreads = 32 * (kSoftmax + kProducers + 2);  // and two issuers
   static constexpr int kHeadBytes = kTreeKeys * D * 2;  // one head's rows of a tile
   static constexpr int kSlotBytes = 32768;
   static constexpr int kSlots = D == 64 ? 6 : 5;
@@ -220,14 +258,16 @@ __device__ __forceinline__ unsigned long long seen64(const TreeParams& p, const 
 // Infinities and NaN were taken out of V tiles: adds those that a row sees to
 // columns [d0, d1) of its result (out, or the partial acc).
 template <typename T>
-__device__ __noinline__ void restore(const TreeParams& p, const TreeItem& w,
+__device__ __forceinline__ void restore(const TreeParams& p, const TreeItem& w,
                                      unsigned long long mask, long long pos, int head, T* out,
                                      float* acc, int d0, int d1) {
+#pragma unroll 1
   for (int j = p.window >= 0 ? w.lo : max(w.lo, w.prefix / kTreeKeys * kTreeKeys); j < w.hi; ++j) {
     if (!key_seen(p, w, mask, pos, j)) continue;
     const long long slot = key_slot(p, w, j);
     if (slot < 0) continue;
     const T* v = static_cast<const T*>(p.v) + slot * p.v_ss + head * p.v_sh;
+#pragma unroll 1
     for (int d = d0; d < d1; ++d) {
       const float x = Elem<T>::to_f32(v[d]);
       if (isfinite(x)) continue;
@@ -306,14 +346,10 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
   const uint32_t tmem = *tmem_slot;
   const int it0 = p.cta_items[blockIdx.x], it1 = p.cta_items[blockIdx.x + 1];
 
-  // 640 threads launch with 96 registers; the softmax warps take 144
-  // (256 x 144 + 384 x 64 = 640 x 96).
-  static_assert(C::kSoftmax == 8 && C::kThreads == 640, "register split");
   if (warp >= C::kSoftmax + C::kProducers) {
     // ---- MMA issuers: one thread per unit ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int u = warp - C::kSoftmax - C::kProducers;
-    if (u < 2 && lane == 0) {
+    if (lane == 0) {
       const uint32_t tu = tmem + 256 * u;
       const uint64_t qd = sw128_desc(base + u * C::kQBytes);
       Pos at;  // the item's first K slot
@@ -390,7 +426,6 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     __syncwarp();
   } else if (warp >= C::kSoftmax) {
     // ---- producers: warp pw gathers keys 16 pw .. of every tile ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     constexpr int kKpw = kTreeKeys / C::kProducers;
     const int pw = warp - C::kSoftmax;
     Pos at;
@@ -407,6 +442,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
       for (int t = 0; t < n_tiles && ok; ++t) {
         const int slot = next;
         next = fetch(t + 1);
+        const bool whole = __all_sync(0xffffffffu, slot >= 0);
         // An infinity or NaN of a V row that only some rows see would reach
         // the others as 0 * V: tiles with drafted tokens or a window are
         // searched for them before they are handed on.
@@ -415,18 +451,32 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         for (int kv = 0; kv < 2; ++kv) {
           ok = warp_wait(bar_empty(at.slot), at.phase ^ 1, abort);
           if (!ok) break;
-          const long long ss = kv ? p.v_ss : p.k_ss, sh = kv ? p.v_sh : p.k_sh;
-          auto copy = [&](auto chunks) {  // chunks: 16-byte pieces per key
+          // kCpk 16-byte pieces per key, consecutive lanes on one key.  The
+          // swizzle moves piece cc of key k to cc ^ (k & 7); the keys of a
+          // lane differ in a constant, so one XOR each gives its address.
+          auto copy = [&](auto chunks) {
             constexpr int kCpk = decltype(chunks)::value, kPer = 32 / kCpk;
-            const int c = lane % kCpk, hh = c / (D / 8), cc = c % (D / 8);
-            const T* src = static_cast<const T*>(kv ? p.v : p.k) + (w.head0 + hh) * sh + cc * 8;
-            const uint32_t off = C::kRingOff + at.slot * C::kSlotBytes + hh * C::kHeadBytes;
+            const int c = lane % kCpk, hh = c / (D / 8), cc = c % (D / 8), sub = lane / kCpk;
+            const char* src = static_cast<const char*>(kv ? p.v : p.k) +
+                              2 * ((w.head0 + hh) * (kv ? p.v_sh : p.k_sh) + cc * 8);
+            const uint32_t stride = (uint32_t)(2 * (kv ? p.v_ss : p.k_ss));
+            const uint32_t off = C::kRingOff + at.slot * C::kSlotBytes + hh * C::kHeadBytes +
+                                 sw_chunk(kTreeKeys, kKpw * pw + sub, cc);
+            auto place = [&](int i) { return (off ^ (i * kPer & 7) << 4) + i * kPer * 128; };
+            if (whole) {
 #pragma unroll
-            for (int i = 0; i < kKpw / kPer; ++i) {
-              const int kk = i * kPer + lane / kCpk;
-              const int sl = __shfl_sync(0xffffffffu, slot, kk);
-              cp_async16(base + off + sw_chunk(kTreeKeys, kKpw * pw + kk, cc),
-                         src + (sl < 0 ? 0 : sl) * ss, sl < 0 ? 0 : 16);
+              for (int i = 0; i < kKpw / kPer; ++i) {
+                const uint32_t sl = __shfl_sync(0xffffffffu, (uint32_t)slot, i * kPer + sub);
+                cp_async16_full(base + place(i), src + (unsigned long long)sl * stride);
+              }
+            } else {  // some keys past the end or padding: zeros
+#pragma unroll
+              for (int i = 0; i < kKpw / kPer; ++i) {
+                const int sl = __shfl_sync(0xffffffffu, slot, i * kPer + sub);
+                cp_async16(base + place(i),
+                           src + (unsigned long long)(uint32_t)max(sl, 0) * stride,
+                           sl < 0 ? 0 : 16);
+              }
             }
             if (kv == 0 || !guarded) {
               cp_async_arrive(bar_full(at.slot));
@@ -436,8 +486,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
             cp_async_wait<0>();
             bool hit = false;
             for (int i = 0; i < kKpw / kPer; ++i) {  // the pieces that this thread copied
-              const int key = kKpw * pw + i * kPer + lane / kCpk;
-              uint4* v = reinterpret_cast<uint4*>(smem + off + sw_chunk(kTreeKeys, key, cc));
+              uint4* v = reinterpret_cast<uint4*>(smem + place(i));
               uint4 x = *v;
               if (scrub<kHalf>(x)) {
                 *v = x;
@@ -458,7 +507,6 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     cp_async_wait<0>();
   } else {
     // ---- softmax ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int u = warp >> 2, r = tid & (kTreeRows - 1);
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's TMEM lanes
     const uint32_t tu = tmem + 256 * u + lanes;
@@ -497,35 +545,39 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         if (!ok) break;
         if (warp_live) {
           tc_fence_after();
-          unsigned long long seen[2] = {~0ull, ~0ull};
           if (p.window >= 0 || j0 + kTreeKeys > w.prefix) {
-            seen[0] = seen64(p, w, mask, pos, j0, lane);
-            seen[1] = seen64(p, w, mask, pos, j0 + 64, lane);
-          }
-          const bool masked = __any_sync(0xffffffffu, (seen[0] & seen[1]) != ~0ull);
-          // 64 scores at a time are in registers: the first half is read
-          // for the maximum, the second for both, then the first again.
-          float s[64];
-          auto half = [&](int b) {
-            tmem_ld64_sync(tu + 64 * b, s);
-            if (masked) {
-              const uint32_t lo = (uint32_t)seen[b], hi = (uint32_t)(seen[b] >> 32);
+            // Hidden keys get a score of -inf in tensor memory, so that the
+            // ordinary path below has no mask (and no registers for one).
+#pragma unroll 1
+            for (int b = 0; b < kTreeKeys; b += 64) {
+              const unsigned long long seen = seen64(p, w, mask, pos, j0 + b, lane);
+              if (__all_sync(0xffffffffu, seen == ~0ull)) continue;
+#pragma unroll 1
+              for (int q = 0; q < 64; q += 32) {
+                const uint32_t bits = (uint32_t)(seen >> q);
+                float x[32];
+                tmem_ld32_sync(tu + b + q, x);
+                uint32_t y[32];
 #pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                s[k] = lo >> k & 1 ? s[k] : -INFINITY;
-                s[k + 32] = hi >> k & 1 ? s[k + 32] : -INFINITY;
+                for (int k = 0; k < 32; ++k)
+                  y[k] = __float_as_uint(bits >> k & 1 ? x[k] : -INFINITY);
+                tmem_st32_sync(tu + b + q, y);
               }
             }
-          };
+          }
+          // The scores are read twice, for the maximum and for P: more than
+          // 64 of them in registers cost spills.
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            half(b);
+          for (int b = 0; b < kTreeKeys; b += 64) {
+            float s[64];
+            tmem_ld64_sync(tu + b, s);
 #pragma unroll
             for (int k = 0; k < 64; k += 2)
-              m4[k >> 1 & 3] = fmaxf(m4[k >> 1 & 3], fmaxf(s[k], s[k + 1]));
+              m4[k >> 1 & 3] = max3_nan(m4[k >> 1 & 3], s[k], s[k + 1]);
           }
-          const float bm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+          const float bm =
+              max3_nan(max3_nan(m4[0], m4[1], m4[2]), m4[3], -INFINITY) * p.scale_log2;
           // The base only moves when the tile exceeds it by 2^8; then l and
           // O are rescaled.
           float alpha = 1.f;
@@ -538,38 +590,41 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
           const float nb = m == -INFINITY ? 0.f : -m;
           const f32x2 scale2 = f2_pack(p.scale_log2, p.scale_log2), nb2 = f2_pack(nb, nb);
           f32x2 sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+          // The last columns come first: P overwrites the second half of its
+          // scores at head_dim 128, each piece of it columns that are read.
 #pragma unroll
-          for (int b = 1; b >= 0; --b) {
-            if (b == 0) {
-              half(0);
-              if (kFree) {  // every score of the tile is read
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_f(u));
-              }
+          for (int b = kTreeKeys - 32; b >= 0; b -= 32) {
+            float s[32];
+            tmem_ld32_sync(tu + b, s);
+            if (kFree && b == 0) {  // every score of the tile is read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar_f(u));
             }
+            uint32_t pk[16];
 #pragma unroll
-            for (int q = 0; q < 64; q += 32) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                float x0, x1;
-                f2_unpack(f2_fma(f2_pack(s[q + k], s[q + k + 1]), scale2, nb2), x0, x1);
+            for (int k = 0; k < 32; k += 2) {
+              float x0, x1;
+              const f32x2 x = f2_fma(f2_pack(s[k], s[k + 1]), scale2, nb2);
+              if (kPoly >> (k / 2) & 1) {
+                exp2_pair(x, x0, x1);
+              } else {
+                f2_unpack(x, x0, x1);
                 x0 = fast_exp2(x0);
                 x1 = fast_exp2(x1);
-                sum[k >> 1 & 1] = f2_add(sum[k >> 1 & 1], f2_pack(x0, x1));
-                pk[k / 2] = pack2<T>(x0, x1);
               }
-              // P's columns, and O's, are free once the product before is
-              // done (with P over the scores S(c) came after it).
-              if (b == 1 && q == 0 && kFree && c > 0)
-                ok = warp_wait(bar_o(u), c - 1 & 1, abort);
-              tmem_st16_sync(tu + C::kColP + (32 * b + q / 2), pk);
+              sum[k >> 1 & 1] = f2_add(sum[k >> 1 & 1], f2_pack(x0, x1));
+              pk[k / 2] = pack2<T>(x0, x1);
             }
+            // P's columns, and O's, are free once the product before is done
+            // (with P over the scores S(c) came after it).
+            if (b == kTreeKeys - 32 && kFree && c > 0) ok = warp_wait(bar_o(u), c - 1 & 1, abort);
+            tmem_st16_sync(tu + C::kColP + b / 2, pk);
           }
           float l0, l1;
           f2_unpack(f2_add(sum[0], sum[1]), l0, l1);
           l = l * alpha + (l0 + l1);
+          if (!(bm < INFINITY)) l = NAN;  // an infinite or NaN score: the row is NaN
           if (__any_sync(0xffffffffu, rescale)) {
             tc_fence_after();
 #pragma unroll
@@ -584,7 +639,10 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
           }
           tc_fence_before();
         } else if (kFree) {
+          // A warp without rows keeps the others' pace: with S(c + 1) made
+          // early it would otherwise arrive on p twice before they do once.
           if (lane == 0) mbar_arrive(bar_f(u));
+          if (c > 0) ok = warp_wait(bar_o(u), c - 1 & 1, abort);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_p(u));
@@ -763,6 +821,9 @@ extern "C" int akv_tree_attention(
   const void* bases[] = {q, k_pool, v_pool, out};
   for (const void* b : bases)
     if (reinterpret_cast<uintptr_t>(b) & 15) return AKV_ERR_INVALID;
+  if (k_stride_slot < 0 || v_stride_slot < 0 || k_stride_slot >= (1ll << 31) ||
+      v_stride_slot >= (1ll << 31))
+    return AKV_ERR_INVALID;  // bytes between slots in 32 bits
   const int64_t strides[] = {q_stride_token, q_stride_head,    k_stride_slot,  k_stride_head,
                              v_stride_slot,  v_stride_head,    out_stride_token, out_stride_head};
   for (int64_t s : strides)
