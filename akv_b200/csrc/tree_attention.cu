@@ -439,7 +439,10 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         return t < n_tiles && j < w.hi ? (int)key_slot(p, w, j) : -1;
       };
       int next = fetch(0);
-      for (int t = 0; t < n_tiles && ok; ++t) {
+      // chunks: 16-byte pieces per key, consecutive lanes on one key.
+      auto tile = [&](int t, auto chunks) {
+        constexpr int kCpk = decltype(chunks)::value, kPer = 32 / kCpk, kRounds = kKpw / kPer;
+        const int c = lane % kCpk, hh = c / (D / 8), cc = c % (D / 8), sub = lane / kCpk;
         const int slot = next;
         next = fetch(t + 1);
         const bool whole = __all_sync(0xffffffffu, slot >= 0);
@@ -447,45 +450,39 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         // the others as 0 * V: tiles with drafted tokens or a window are
         // searched for them before they are handed on.
         const bool guarded = p.window >= 0 || w.lo + (t + 1) * kTreeKeys > w.prefix;
+        // The slots of the keys that this lane copies a piece of, all before
+        // the first copy: between the copies each would wait for its shuffle.
+        int sl[kRounds];
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) sl[i] = __shfl_sync(0xffffffffu, slot, i * kPer + sub);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           ok = warp_wait(bar_empty(at.slot), at.phase ^ 1, abort);
-          if (!ok) break;
-          // kCpk 16-byte pieces per key, consecutive lanes on one key.  The
-          // swizzle moves piece cc of key k to cc ^ (k & 7); the keys of a
-          // lane differ in a constant, so one XOR each gives its address.
-          auto copy = [&](auto chunks) {
-            constexpr int kCpk = decltype(chunks)::value, kPer = 32 / kCpk;
-            const int c = lane % kCpk, hh = c / (D / 8), cc = c % (D / 8), sub = lane / kCpk;
-            const char* src = static_cast<const char*>(kv ? p.v : p.k) +
-                              2 * ((w.head0 + hh) * (kv ? p.v_sh : p.k_sh) + cc * 8);
-            const uint32_t stride = (uint32_t)(2 * (kv ? p.v_ss : p.k_ss));
-            const uint32_t off = C::kRingOff + at.slot * C::kSlotBytes + hh * C::kHeadBytes +
-                                 sw_chunk(kTreeKeys, kKpw * pw + sub, cc);
-            auto place = [&](int i) { return (off ^ (i * kPer & 7) << 4) + i * kPer * 128; };
-            if (whole) {
+          if (!ok) return;
+          const char* src = static_cast<const char*>(kv ? p.v : p.k) +
+                            2 * ((w.head0 + hh) * (kv ? p.v_sh : p.k_sh) + cc * 8);
+          const uint32_t stride = (uint32_t)(2 * (kv ? p.v_ss : p.k_ss));
+          // The swizzle moves piece cc of key k to cc ^ (k & 7); the keys of
+          // a lane differ in a constant, so one XOR each gives its address.
+          const uint32_t off = C::kRingOff + at.slot * C::kSlotBytes + hh * C::kHeadBytes +
+                               sw_chunk(kTreeKeys, kKpw * pw + sub, cc);
+          auto place = [&](int i) { return (off ^ (i * kPer & 7) << 4) + i * kPer * 128; };
+          if (whole) {
 #pragma unroll
-              for (int i = 0; i < kKpw / kPer; ++i) {
-                const uint32_t sl = __shfl_sync(0xffffffffu, (uint32_t)slot, i * kPer + sub);
-                cp_async16_full(base + place(i), src + (unsigned long long)sl * stride);
-              }
-            } else {  // some keys past the end or padding: zeros
+            for (int i = 0; i < kRounds; ++i)
+              cp_async16_full(base + place(i), src + (unsigned long long)(uint32_t)sl[i] * stride);
+          } else {  // some keys past the end or padding: zeros
 #pragma unroll
-              for (int i = 0; i < kKpw / kPer; ++i) {
-                const int sl = __shfl_sync(0xffffffffu, slot, i * kPer + sub);
-                cp_async16(base + place(i),
-                           src + (unsigned long long)(uint32_t)max(sl, 0) * stride,
-                           sl < 0 ? 0 : 16);
-              }
-            }
-            if (kv == 0 || !guarded) {
-              cp_async_arrive(bar_full(at.slot));
-              return;
-            }
+            for (int i = 0; i < kRounds; ++i)
+              cp_async16(base + place(i),
+                         src + (unsigned long long)(uint32_t)max(sl[i], 0) * stride,
+                         sl[i] < 0 ? 0 : 16);
+          }
+          if (kv == 1 && guarded) {
             cp_async_commit();
             cp_async_wait<0>();
             bool hit = false;
-            for (int i = 0; i < kKpw / kPer; ++i) {  // the pieces that this thread copied
+            for (int i = 0; i < kRounds; ++i) {  // the pieces that this thread copied
               uint4* v = reinterpret_cast<uint4*>(smem + place(i));
               uint4 x = *v;
               if (scrub<kHalf>(x)) {
@@ -496,11 +493,15 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
             if (hit) *scrubbed = 1;
             fence_async_smem();
             mbar_arrive(bar_full(at.slot));
-          };
-          if (heads * (D / 8) == 16) copy(std::integral_constant<int, 16>());
-          else copy(std::integral_constant<int, 8>());
+          } else {
+            cp_async_arrive(bar_full(at.slot));
+          }
           at.advance(1);
         }
+      };
+      for (int t = 0; t < n_tiles && ok; ++t) {
+        if (heads * (D / 8) == 16) tile(t, std::integral_constant<int, 16>());
+        else tile(t, std::integral_constant<int, 8>());
       }
     }
     cp_async_commit();
