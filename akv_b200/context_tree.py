@@ -72,6 +72,10 @@ def tree_work_list(kv_indptr, draft_indptr, group, num_kv_heads, pair_heads, cta
     if ctas:
         g = np.minimum(np.searchsorted(cost_end, bounds, side="right"), len(req) - 1)
         at = (bounds - (cost_end[g] - tiles[g] * weight[g])) // weight[g]
+        # A cut one tile off a group's end moves there: a piece of one tile
+        # costs more (its own start, a partial result, a merge) than it evens.
+        at = np.where((at == 1) & (tiles[g] > 1), 0, at)
+        at = np.where((at == tiles[g] - 1) & (tiles[g] > 2), tiles[g], at)
         bounds = tile_end[g] - tiles[g] + at
     cuts = np.unique(np.concatenate((bounds, tile_end, [0])))
     first, last = cuts[:-1], cuts[1:]

@@ -56,7 +56,7 @@ struct TreeParams {
   int group, num_q_heads;
   const TreeItem* items;
   const int* cta_items;
-  float* part_acc;  // [partials][kTreeRows][D]
+  float* part_acc;  // [partials][D / 4][kTreeRows][4]: a warp's rows side by side
   float* part_ml;   // [partials][kTreeRows][2]: maximum in base 2, sum
   void* out;
   long long o_st, o_sh;
@@ -228,9 +228,10 @@ struct RingPos {
   }
 };
 
-// Visible keys among the 64 from j0 on, as bits.  Every lane of the warp calls it.
+// Visible keys among the 64 from j0 on, as bits, of this lane's row of token i
+// (position pos).  Every lane of the warp calls it; tokens rise with the lane.
 __device__ __forceinline__ unsigned long long seen64(const TreeParams& p, const TreeItem& w,
-                                                     unsigned long long mask, long long pos,
+                                                     unsigned long long mask, int i, int pos,
                                                      int j0, int lane) {
   if (j0 >= w.hi) return 0;
   const int cached = min(max(w.prefix - j0, 0), 64);
@@ -242,12 +243,18 @@ __device__ __forceinline__ unsigned long long seen64(const TreeParams& p, const 
     if (p.window < 0) {
       seen |= cached < 64 ? (1ull << cached) - 1 : ~0ull;
     } else {
+      // Each lane tests two keys, for one of the warp's tokens after another.
       const int* kp = p.kv_positions + w.kv0 + j0;
-      const int p0 = lane < cached ? kp[lane] : 0;
-      const int p1 = lane + 32 < cached ? kp[lane + 32] : 0;
-      for (int k = 0; k < cached; ++k) {
-        const int kpos = __shfl_sync(0xffffffffu, k < 32 ? p0 : p1, k & 31);
-        if (pos - kpos <= p.window) seen |= 1ull << k;
+      const bool in0 = lane < cached, in1 = lane + 32 < cached;
+      const long long p0 = in0 ? kp[lane] : 0, p1 = in1 ? kp[lane + 32] : 0;
+      for (unsigned left = 0xffffffffu; left;) {
+        const int src = __ffs(left) - 1;
+        const int token = __shfl_sync(0xffffffffu, i, src);
+        const long long at = __shfl_sync(0xffffffffu, pos, src);
+        const unsigned lo = __ballot_sync(0xffffffffu, in0 && at - p0 <= p.window);
+        const unsigned hi = __ballot_sync(0xffffffffu, in1 && at - p1 <= p.window);
+        if (i == token) seen |= (unsigned long long)hi << 32 | lo;
+        left = __ballot_sync(0xffffffffu, i > token);
       }
     }
   }
@@ -272,7 +279,7 @@ __device__ __forceinline__ void restore(const TreeParams& p, const TreeItem& w,
       const float x = Elem<T>::to_f32(v[d]);
       if (isfinite(x)) continue;
       if (out) out[d] = Elem<T>::from_f32(Elem<T>::to_f32(out[d]) + x);
-      else acc[d] += x;
+      else acc[(d >> 2) * 4 * kTreeRows + (d & 3)] += x;
     }
   }
 }
@@ -513,6 +520,24 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     const uint32_t tu = tmem + 256 * u + lanes;
     float2* rows = reinterpret_cast<float2*>(smem + C::kRowOff);
     uint32_t cnt = 0, n_x = 0;
+    // Copies this thread's row of an item's Q: for the first item here, for
+    // the next one once the last scores of the one before are made.
+    auto load_q = [&](int it) {
+      if (it < it1) {
+        const TreeItem w = p.items[it];
+        const int row = (w.tile0 + u * w.tile_step) * kTreeRows + r;
+        const int i = row / p.group, h = (w.head0 + u * w.head_step) * p.group + row - i * p.group;
+        if (i < w.n) {
+          const T* src = static_cast<const T*>(p.q) + (long long)(w.q0 + i) * p.q_st +
+                         (long long)h * p.q_sh;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            cp_async16_full(base + u * C::kQBytes + sw_chunk(kTreeRows, r, c), src + 8 * c);
+        }
+      }
+      cp_async_commit();
+    };
+    load_q(it0);
     for (int it = it0; it < it1; ++it) {
       const TreeItem w = p.items[it];
       const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
@@ -523,20 +548,15 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
       const int i = (row0 + r) / p.group, h = head * p.group + (row0 + r) - i * p.group;
       const bool live = i < w.n;
       const bool warp_live = row0 + (warp & 3) * 32 < w.n * p.group;
+      const unsigned long long mask = live ? row_mask(p, w, i) : 0;
+      const int pos = live && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
+      cp_async_wait<0>();
       if (n > 0) {
-        if (live) {
-          const uint4* src = reinterpret_cast<const uint4*>(
-              static_cast<const T*>(p.q) + (long long)(w.q0 + i) * p.q_st + (long long)h * p.q_sh);
-          unsigned char* dst = smem + u * C::kQBytes;
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c)
-            *reinterpret_cast<uint4*>(dst + sw_chunk(kTreeRows, r, c)) = src[c];
-        }
         fence_async_smem();
         mbar_arrive(bar_q(u));
+      } else {
+        load_q(it + 1);
       }
-      const unsigned long long mask = live ? row_mask(p, w, i) : 0;
-      const long long pos = live && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
       for (int v = 0; v < n && ok; ++v) {
@@ -544,6 +564,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         const int j0 = w.lo + (pair ? v : 2 * v + u) * kTreeKeys;
         ok = warp_wait(bar_s(u), c & 1, abort);
         if (!ok) break;
+        if (v == n - 1) load_q(it + 1);
         if (warp_live) {
           tc_fence_after();
           if (p.window >= 0 || j0 + kTreeKeys > w.prefix) {
@@ -551,7 +572,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
             // ordinary path below has no mask (and no registers for one).
 #pragma unroll 1
             for (int b = 0; b < kTreeKeys; b += 64) {
-              const unsigned long long seen = seen64(p, w, mask, pos, j0 + b, lane);
+              const unsigned long long seen = seen64(p, w, mask, i, pos, j0 + b, lane);
               if (__all_sync(0xffffffffu, seen == ~0ull)) continue;
 #pragma unroll 1
               for (int q = 0; q < 64; q += 32) {
@@ -669,8 +690,10 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
       }
       if (warp_live) {
         const bool direct = w.partial < 0;
-        const long long at = ((long long)w.partial + (pair ? u : 0)) * kTreeRows + r;
-        const RowEnd e = row_end(p.sinks, live ? h : 0, m, l);
+        const long long part = (long long)w.partial + (pair ? u : 0);
+        float* acc = p.part_acc + part * D * kTreeRows + 4 * r;
+        RowEnd e = {0.f, 0.f};
+        if (direct) e = row_end(p.sinks, live ? h : 0, m, l);
         T* dst = static_cast<T*>(p.out) + (long long)(w.q0 + i) * p.o_st + (long long)h * p.o_sh;
         // A pair's units write all their columns, a single item's half each.
         const int d0 = pair ? 0 : u * (D / 2), d1 = pair ? D : d0 + D / 2;
@@ -696,19 +719,18 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
               *reinterpret_cast<uint4*>(dst + d + k) = x;
             }
           } else {
-            float4* acc = reinterpret_cast<float4*>(p.part_acc + at * D + d);
 #pragma unroll
             for (int k = 0; k < 32; k += 4)
-              acc[k / 4] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              *reinterpret_cast<float4*>(acc + (d + k) * kTreeRows) =
+                  make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
           }
         }
         if (live && *scrubbed)
           restore<T>(p, w, mask, pos, head, direct ? dst : nullptr,
-                     direct ? nullptr : p.part_acc + at * D, d0, d1);
+                     direct ? nullptr : acc, d0, d1);
         if (live && (pair || u == 0)) {
           if (!direct) {
-            p.part_ml[2 * at] = m;
-            p.part_ml[2 * at + 1] = l;
+            reinterpret_cast<float2*>(p.part_ml)[part * kTreeRows + r] = make_float2(m, l);
           } else if (p.lse) {
             p.lse[(long long)(w.q0 + i) * p.num_q_heads + h] = e.lse;
           }
@@ -737,45 +759,52 @@ struct TreeMerge {  // 8 int32
   int first, count, unused;
 };
 
-// Joins the pieces of one unit: one warp per row.
-constexpr int kMergeWarps = 8;
+// Joins the pieces of units that were cut.  A block takes kRows rows of one
+// unit, a thread four columns of a row; neighbouring threads have
+// neighbouring rows, as the partial results lie.
+constexpr int kMergeThreads = 256;
+template <int D>
+constexpr int merge_rows() { return kMergeThreads / (D / 4); }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kMergeWarps)
+__global__ void __launch_bounds__(kMergeThreads)
 tree_merge_kernel(const TreeParams p, const TreeMerge* merges) {
+  constexpr int kRows = merge_rows<D>();
   const TreeMerge g = merges[blockIdx.x];
-  const int lane = threadIdx.x & 31;
-  const int u = blockIdx.y / (kTreeRows / kMergeWarps);
-  const int r = blockIdx.y % (kTreeRows / kMergeWarps) * kMergeWarps + (threadIdx.x >> 5);
+  const int u = blockIdx.y / (kTreeRows / kRows);
+  const int r = blockIdx.y % (kTreeRows / kRows) * kRows + threadIdx.x % kRows;
+  const int d = threadIdx.x / kRows * 4;
   if (u >= g.steps >> 2) return;
   const int head = g.head0 + u * (g.steps & 1);
   const int row = (g.tile0 + u * (g.steps >> 1 & 1)) * kTreeRows + r;
   const int i = row / p.group, h = head * p.group + row % p.group;
   if (i >= g.n) return;
   pdl_wait();
-  const long long step = (long long)kTreeUnits * kTreeRows;  // rows between two pieces
-  const long long at = ((long long)g.first + u) * kTreeRows + r;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) +
+                     ((long long)g.first + u) * kTreeRows + r;
+  const float* acc = p.part_acc + (((long long)g.first + u) * D + d) * kTreeRows + 4 * r;
   float m = -INFINITY;
-  for (int s = lane; s < g.count; s += 32) m = fmaxf(m, p.part_ml[2 * (at + s * step)]);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+#pragma unroll 4
+  for (int s = 0; s < g.count; ++s) m = fmaxf(m, ml[s * kTreeUnits * kTreeRows].x);
   const float base = m == -INFINITY ? 0.f : m;
-  float den = 0.f, num[D / 32];
-#pragma unroll
-  for (int d = 0; d < D / 32; ++d) num[d] = 0.f;
+  float den = 0.f, num[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int s = 0; s < g.count; ++s) {
-    const long long a = at + s * step;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * a);
-    const float f = fast_exp2(ml.x - base);
-    den += ml.y * f;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d) num[d] += p.part_acc[a * D + lane + 32 * d] * f;
+    const float2 x = ml[s * kTreeUnits * kTreeRows];
+    const float4 a =
+        *reinterpret_cast<const float4*>(acc + (long long)s * kTreeUnits * D * kTreeRows);
+    const float f = fast_exp2(x.x - base);
+    den += x.y * f;
+    num[0] += a.x * f;
+    num[1] += a.y * f;
+    num[2] += a.z * f;
+    num[3] += a.w * f;
   }
   const RowEnd e = row_end(p.sinks, h, m, den);
-  T* o = static_cast<T*>(p.out) + (long long)(g.q0 + i) * p.o_st + (long long)h * p.o_sh + lane;
-#pragma unroll
-  for (int d = 0; d < D / 32; ++d) o[32 * d] = Elem<T>::from_f32(num[d] * e.scale);
-  if (p.lse && lane == 0) p.lse[(long long)(g.q0 + i) * p.num_q_heads + h] = e.lse;
+  T* o = static_cast<T*>(p.out) + (long long)(g.q0 + i) * p.o_st + (long long)h * p.o_sh + d;
+  *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(num[0] * e.scale, num[1] * e.scale),
+                                            pack2<T>(num[2] * e.scale, num[3] * e.scale));
+  if (p.lse && d == 0) p.lse[(long long)(g.q0 + i) * p.num_q_heads + h] = e.lse;
 }
 
 template <typename T, int D>
@@ -787,8 +816,8 @@ int launch_tree(const TreeParams& p, int n_ctas, const TreeMerge* merges, int n_
     return AKV_ERR_CUDA;
   tree_attention_kernel<T, D><<<n_ctas, C::kThreads, C::kSmem, s>>>(p);
   if (n_merges > 0 &&
-      launch_pdl(tree_merge_kernel<T, D>, dim3(n_merges, kTreeUnits * (kTreeRows / kMergeWarps)),
-                 dim3(32 * kMergeWarps), 0, s, p, merges) != cudaSuccess)
+      launch_pdl(tree_merge_kernel<T, D>, dim3(n_merges, kTreeUnits * kTreeRows / merge_rows<D>()),
+                 dim3(kMergeThreads), 0, s, p, merges) != cudaSuccess)
     return AKV_ERR_CUDA;
   return launch_status();
 }

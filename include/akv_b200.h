@@ -770,8 +770,8 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_token, int64_t q_stride_hea
  * 1], CTA c runs items [cta_items[c], cta_items[c + 1]).  merges: DEVICE
  * int32 [n_merges][8] = {q0, tokens, head0, tile0, head_step | tile_step << 1
  * | units << 2, first partial, pieces, 0}: the pieces' partials lie
- * akv_tree_attention_units apart.  partial_acc fp32 [partials][128][head_dim],
- * partial_ml fp32 [partials][128][2].  tree_work_list of
+ * akv_tree_attention_units apart.  partial_acc fp32 [partials][head_dim /
+ * 4][128][4], partial_ml fp32 [partials][128][2].  tree_work_list of
  * akv_b200/context_tree.py builds all of them.
  *
  * error_flag: DEVICE int32 [2] or NULL: [0] collects 1 (a slot outside the

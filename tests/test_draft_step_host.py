@@ -164,8 +164,9 @@ def test_tree_work_list_covers_every_key_of_every_row_once(pair_heads, hkv, grou
     assert all(len(v) == 1 for k, v in parts.items() if k not in joined)
     assert cta_items[0] == 0 and cta_items[-1] == len(items) and np.all(np.diff(cta_items) >= 0)
     cost = -(-(items[:, 5] - items[:, 4]) // 128) * items[:, 10]
-    load = np.add.reduceat(cost, cta_items[:-1])
-    assert load.max() - load.min() <= 3
+    load = [cost[a:b].sum() for a, b in zip(cta_items, cta_items[1:])]
+    # Equal shares, each end off by less than two tiles of a pair.
+    assert max(load) <= -(-cost.sum() // len(load)) + 6
 
 
 def test_tree_work_list_refuses():
