@@ -18,18 +18,17 @@ import torch
 
 from . import _native
 
-_launch = _native.launch
+_NONE = (0, 0, 0)
 
 
 def _heads(name, t, dtype, index, shape):
-    if t.ndim != 3 or t.dtype != dtype or t.get_device() != index or t.stride(2) != 1 or \
+    """(address, stride of the first dimension, of the second)."""
+    s = t.stride()
+    if t.dtype != dtype or t.get_device() != index or len(s) != 3 or s[2] != 1 or \
             (shape is not None and t.shape != shape):
         raise ValueError(f"{name} must be [tokens, heads, head_dim] of the type and device of q, "
                          "with unit last stride")
-    return t.data_ptr(), t.stride(0), t.stride(1)
-
-
-_NONE = (None, 0, 0)
+    return t.data_ptr(), s[0], s[1]
 
 
 def qk_norm_rope(q, k, positions, cos_sin_cache, *, q_weight=None, k_weight=None, eps=1e-6,
@@ -67,15 +66,16 @@ def qk_norm_rope(q, k, positions, cos_sin_cache, *, q_weight=None, k_weight=None
     qa = _heads("q", q, dtype, index, None)
     tokens, hq, d = q.shape
     ka = _heads("k", k, dtype, index, None)
-    hkv = k.shape[1]
-    if k.shape[0] != tokens or k.shape[2] != d:
+    k_tokens, hkv, k_dim = k.shape
+    if k_tokens != tokens or k_dim != d:
         raise ValueError("k must have q's tokens and head_dim")
-    if cos_sin_cache.ndim != 2 or cos_sin_cache.stride(1) != 1 or \
-            cos_sin_cache.get_device() != index:
+    if cos_sin_cache.ndim != 2 or cos_sin_cache.get_device() != index:
         raise ValueError("cos_sin_cache must be [max_position, rotary_dim] on the device of q")
-    rotary = cos_sin_cache.shape[1] if rotary_dim is None else rotary_dim
+    max_position, width = cos_sin_cache.shape
+    cache_stride, unit = cos_sin_cache.stride()
+    rotary = width if rotary_dim is None else rotary_dim
     cache_code = _native.DTYPE_CODE.get(cos_sin_cache.dtype)
-    if cache_code is None or rotary != cos_sin_cache.shape[1]:
+    if cache_code is None or rotary != width or unit != 1:
         raise ValueError("cos_sin_cache must be floating point and rotary_dim wide")
     if d % 16 or d > 512 or rotary % 16 or not 0 < rotary <= d:
         raise ValueError("head_dim and rotary_dim must be multiples of 16, at most 512")
@@ -93,38 +93,41 @@ def qk_norm_rope(q, k, positions, cos_sin_cache, *, q_weight=None, k_weight=None
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError("norm weights must have one type")
     if q_out is None:
-        q_out = torch.empty((tokens, hq, d), dtype=dtype, device=q.device)
-    qo = _heads("q_out", q_out, dtype, index, (tokens, hq, d))
+        q_out = torch.empty_like(q)
+    qo = _heads("q_out", q_out, dtype, index, q.shape)
     va = kp = vp = _NONE
-    num_slots, slots_ptr, slots64 = 0, None, 0
+    num_slots = slots_ptr = slots64 = 0
     if k_pool is not None:
         if v is None or v_pool is None or slots is None:
             raise ValueError("a store needs v, k_pool, v_pool and slots")
-        va = _heads("v", v, dtype, index, (tokens, hkv, d))
+        va = _heads("v", v, dtype, index, k.shape)
         kp = _heads("k_pool", k_pool, dtype, index, None)
         vp = _heads("v_pool", v_pool, dtype, index, None)
-        if k_pool.shape[1:] != (hkv, d) or v_pool.shape[1:] != (hkv, d):
+        k_shape, v_shape = k_pool.shape, v_pool.shape
+        if k_shape[1:] != (hkv, d) or v_shape[1:] != (hkv, d):
             raise ValueError("KV pools must be [slots, num_kv_heads, head_dim]")
-        num_slots = min(k_pool.shape[0], v_pool.shape[0])
+        num_slots = min(k_shape[0], v_shape[0])
         if slots.shape != (tokens,) or slots.get_device() != index or not slots.is_contiguous():
             raise ValueError("slots must be a contiguous vector of one entry per token")
         slots_ptr, slots64 = slots.data_ptr(), _native.is64(slots)
     elif v is not None or v_pool is not None or slots is not None:
         raise ValueError("a store needs v, k_pool, v_pool and slots")
     elif k_out is None:
-        k_out = torch.empty((tokens, hkv, d), dtype=dtype, device=q.device)
-    ko = _NONE if k_out is None else _heads("k_out", k_out, dtype, index, (tokens, hkv, d))
-    if error_flag is not None and (error_flag.get_device() != index or
-                                   error_flag.dtype != torch.int32):
-        raise ValueError("error_flag must be an int32 tensor on the device of q")
+        k_out = torch.empty_like(k)
+    ko = _NONE if k_out is None else _heads("k_out", k_out, dtype, index, k.shape)
+    flag = 0
+    if error_flag is not None:
+        if error_flag.get_device() != index or error_flag.dtype != torch.int32:
+            raise ValueError("error_flag must be an int32 tensor on the device of q")
+        flag = error_flag.data_ptr()
+    positions64 = _native.is64(positions)
     if tokens == 0:
         return q_out, k_out
-    status = _launch(
-        index, _native.lib.akv_qk_norm_rope, *qa, *ka, *va, code, tokens, hq, hkv, d, rotary,
-        1 if is_neox_style else 0, None if q_weight is None else q_weight.data_ptr(),
-        None if k_weight is None else k_weight.data_ptr(), weight_code, eps,
-        positions.data_ptr(), _native.is64(positions), cos_sin_cache.data_ptr(), cache_code,
-        cos_sin_cache.stride(0), cos_sin_cache.shape[0], *qo, *ko, *kp, *vp, num_slots, slots_ptr,
-        slots64, None if error_flag is None else error_flag.data_ptr())
+    status = _native.launch(index, _native.lib.akv_qk_norm_rope, _native.QK_NORM_ROPE.pack(
+        *qa, *ka, *va, code, tokens, hq, hkv, d, rotary, 1 if is_neox_style else 0,
+        0 if q_weight is None else q_weight.data_ptr(),
+        0 if k_weight is None else k_weight.data_ptr(), weight_code, eps, positions.data_ptr(),
+        positions64, cos_sin_cache.data_ptr(), cache_code, cache_stride, max_position, *qo, *ko,
+        *kp, *vp, num_slots, slots_ptr, slots64, flag))
     _native.check(status, "qk_norm_rope")
     return q_out, k_out

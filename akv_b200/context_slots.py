@@ -55,6 +55,14 @@ class SlotMap:
             raise RuntimeError(f"slot map: {why}")
 
 
+def _vector(name, t, n, index):
+    """1 for an int64 vector of n entries on the device, 0 for int32."""
+    if t.shape != (n,) or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{name} must be a contiguous vector of one entry per request, on the "
+                         "mapper's device")
+    return _native.is64(t)
+
+
 class SlotMapper:
     """Outputs are allocated once, for up to ``max_batch`` requests with
     ``max_new_tokens`` new tokens in all; a call allocates nothing, so it can
@@ -80,6 +88,9 @@ class SlotMapper:
         self._slots, self._positions = vector(self.max_new_tokens), vector(self.max_new_tokens)
         self._mask = vector(self.max_new_tokens, torch.int64)
         self._totals, self._status, self._work = vector(2), vector(1), vector(2)
+        self._outputs = tuple(t.data_ptr() for t in (self._offsets, self._slots, self._positions,
+                                                     self._mask))
+        self._words = tuple(t.data_ptr() for t in (self._totals, self._status, self._work))
 
     def run(self, req_to_token, row_ids, raw_lens, new_lens, ring, *, next_positions=None,
             parents=None, block_table=None, commit=True) -> SlotMap:
@@ -94,56 +105,51 @@ class SlotMapper:
         page ids of whole rows.  Two requests of one call must not share a
         row, unless at most one of them has new tokens.  Failures that only
         the device sees are bits of ``status`` (``SlotMap.check``)."""
-        batch, index = len(row_ids), self._index
+        batch, index = row_ids.shape[0], self._index
         if batch > self.max_batch:
             raise ValueError("batch exceeds max_batch")
-        if req_to_token.dtype != torch.int32 or req_to_token.ndim != 2 or \
-                req_to_token.stride(1) != 1:
-            raise ValueError("req_to_token must be int32 [rows, columns] with unit last stride")
-        for name, t in (("row_ids", row_ids), ("raw_lens", raw_lens), ("new_lens", new_lens),
-                        ("next_positions", next_positions)):
-            if t is not None and (t.shape != (batch,) or not t.is_contiguous()):
-                raise ValueError(f"{name} must be a contiguous vector of one entry per request")
-        tensors = [req_to_token, row_ids, raw_lens, new_lens, ring.ring, ring.state]
+        rows, columns = req_to_token.shape
+        row_stride, unit = req_to_token.stride()
+        if req_to_token.dtype != torch.int32 or unit != 1 or req_to_token.get_device() != index:
+            raise ValueError("req_to_token must be int32 [rows, columns] with unit last stride, "
+                             "on the mapper's device")
+        is64 = [_vector(name, t, batch, index) for name, t in
+                (("row_ids", row_ids), ("raw_lens", raw_lens), ("new_lens", new_lens))]
+        next_ptr = next64 = parents_ptr = table_ptr = table_stride = table_columns = 0
         if next_positions is not None:
-            tensors.append(next_positions)
+            next64 = _vector("next_positions", next_positions, batch, index)
+            next_ptr = next_positions.data_ptr()
         if parents is not None:
-            if parents.dtype != torch.int32 or parents.ndim != 1 or not parents.is_contiguous():
-                raise ValueError("parents must be a contiguous int32 vector")
-            if parents.numel() < self.max_new_tokens:
-                raise ValueError("parents must hold max_new_tokens entries")
-            tensors.append(parents)
-        table_stride = table_columns = 0
+            if parents.dtype != torch.int32 or parents.ndim != 1 or \
+                    not parents.is_contiguous() or parents.get_device() != index or \
+                    parents.shape[0] < self.max_new_tokens:
+                raise ValueError("parents must be a contiguous int32 vector of max_new_tokens "
+                                 "entries on the mapper's device")
+            parents_ptr = parents.data_ptr()
         if block_table is not None:
-            if block_table.dtype != torch.int32 or block_table.ndim != 2 or \
-                    block_table.stride(1) != 1 or block_table.shape[0] < batch:
-                raise ValueError("block_table must be int32 [>= batch, columns] with unit last stride")
-            table_stride, table_columns = block_table.stride(0), block_table.shape[1]
-            tensors.append(block_table)
-        for t in tensors:
-            if t.get_device() != index:
-                raise ValueError("slot map tensors must be on the mapper's CUDA device")
-        is64 = _native.is64
-        flags = (is64(row_ids), is64(raw_lens), is64(new_lens),
-                 is64(next_positions) if next_positions is not None else 0)
-        result = SlotMap(self._offsets[: batch + 1], self._slots, self._positions,
+            table_rows, table_columns = block_table.shape
+            table_stride, unit = block_table.stride()
+            if block_table.dtype != torch.int32 or unit != 1 or table_rows < batch or \
+                    block_table.get_device() != index:
+                raise ValueError("block_table must be int32 [>= batch, columns] with unit last "
+                                 "stride, on the mapper's device")
+            table_ptr = block_table.data_ptr()
+        free, state = ring.ring, ring.state
+        if free.get_device() != index or state.get_device() != index:
+            raise ValueError("the free ring must be on the mapper's device")
+        offsets = self._offsets if batch == self.max_batch else self._offsets[: batch + 1]
+        result = SlotMap(offsets, self._slots, self._positions,
                          self._mask if parents is not None else None, block_table, self._totals,
                          self._status)
         if batch == 0:
             for t in (result.new_offsets, result.totals, result.status):
                 t.zero_()
             return result
-        status = _native.launch(
-            index, _native.lib.akv_map_slots,
-            req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[0],
-            req_to_token.shape[1], row_ids.data_ptr(), flags[0], raw_lens.data_ptr(), flags[1],
-            new_lens.data_ptr(), flags[2], batch, self.page_size, ring.ring.data_ptr(),
-            ring.state.data_ptr(), ring.capacity,
-            None if next_positions is None else next_positions.data_ptr(), flags[3],
-            None if parents is None else parents.data_ptr(), self.max_new_tokens,
-            self._offsets.data_ptr(), self._slots.data_ptr(), self._positions.data_ptr(),
-            self._mask.data_ptr(), None if block_table is None else block_table.data_ptr(),
-            table_stride, table_columns, self._totals.data_ptr(), self._status.data_ptr(),
-            self._work.data_ptr(), int(bool(commit)))
+        status = _native.launch(index, _native.lib.akv_map_slots, _native.MAP_SLOTS.pack(
+            req_to_token.data_ptr(), row_stride, rows, columns, row_ids.data_ptr(), is64[0],
+            raw_lens.data_ptr(), is64[1], new_lens.data_ptr(), is64[2], batch, self.page_size,
+            free.data_ptr(), state.data_ptr(), ring.capacity, next_ptr, next64, parents_ptr,
+            self.max_new_tokens, *self._outputs, table_ptr, table_stride, table_columns,
+            *self._words, 1 if commit else 0))
         _native.check(status, "map_slots")
         return result

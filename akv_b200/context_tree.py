@@ -102,6 +102,27 @@ def tree_work_list(kv_indptr, draft_indptr, group, num_kv_heads, pair_heads, cta
     return items.astype(np.int32), cta_items, merges.astype(np.int32), int(cut.sum()) * UNITS
 
 
+def _rows(name, t, dtype, index, tokens, shape):
+    """The first two strides of a [>= tokens, heads, head_dim] tensor."""
+    n, *rest = t.shape
+    s = t.stride()
+    if tuple(rest) != shape or n < tokens or t.dtype != dtype or s[2] != 1 or \
+            t.get_device() != index:
+        raise ValueError(f"{name} must be [tokens or slots, heads, head_dim] = [>= {tokens}, "
+                         f"{shape[0]}, {shape[1]}] {dtype} with unit last stride, on the plan's "
+                         "device")
+    return s[0], s[1]
+
+
+def _vector(name, t, dtype, index, n):
+    """The address of a contiguous vector of at least n entries."""
+    if t.dtype != dtype or t.ndim != 1 or t.shape[0] < n or not t.is_contiguous() or \
+            t.get_device() != index:
+        raise ValueError(f"{name} must be a contiguous {dtype} vector of the plan's length, on "
+                         "the plan's device")
+    return t.data_ptr()
+
+
 class TreeAttention:
     """Plans and partial results live in the instance: runs of one instance,
     replays of its graphs among them, must not overlap on the device, and a
@@ -146,6 +167,9 @@ class TreeAttention:
         self._ml = torch.empty((partials, TILE_ROWS, 2), dtype=torch.float32, device=device)
         # [0]: error bits kept until check(); [1]: the abort word of the current launch.
         self.error_flag = torch.zeros(2, dtype=torch.int32, device=device)
+        self._plan_ptr, self._flag_ptr = self._dev.data_ptr(), self.error_flag.data_ptr()
+        self._partial_ptrs = self._acc.data_ptr(), self._ml.data_ptr()
+        self._code = _native.DTYPE_CODE[dtype]
         self._copied = torch.cuda.Event()
         self._copied.record(torch.cuda.current_stream(device))
         self.tokens = self.keys = self.n_ctas = self.n_merges = 0
@@ -187,58 +211,40 @@ class TreeAttention:
 
         The head's maximum, sum and accumulator are fp32; P is rounded to the
         pools' type for P.V.  Returns out, or (out, lse fp32 [tokens, Hq])."""
-        index, tokens = self._index, self.tokens
-        if q.dtype != self.dtype or k_pool.dtype != self.dtype or v_pool.dtype != self.dtype:
-            raise ValueError("q / K / V must have the planned type")
-        if q.ndim != 3 or q.shape[0] < tokens or q.shape[1:] != (self.hq, self.d) or \
-                q.stride(-1) != 1:
-            raise ValueError("q must be [tokens, num_q_heads, head_dim] with unit last stride")
-        for pool in (k_pool, v_pool):
-            if pool.ndim != 3 or pool.shape[1:] != (self.hkv, self.d) or pool.stride(-1) != 1:
-                raise ValueError("KV pools must be [slots, num_kv_heads, head_dim]")
-        tensors = [q, k_pool, v_pool, kv_indices, draft_slots, tree_mask]
+        index, tokens, dtype = self._index, self.tokens, self.dtype
+        q_token, q_head = _rows("q", q, dtype, index, tokens, (self.hq, self.d))
+        k_slot, k_head = _rows("k_pool", k_pool, dtype, index, 1, (self.hkv, self.d))
+        v_slot, v_head = _rows("v_pool", v_pool, dtype, index, 1, (self.hkv, self.d))
         window = -1 if window is None or window < 0 else int(window)
-        vectors = [("kv_indices", kv_indices, self.keys, torch.int32),
-                   ("draft_slots", draft_slots, tokens, torch.int32),
-                   ("tree_mask", tree_mask, tokens, torch.int64)]
+        ints = torch.int32
+        kv_ptr = _vector("kv_indices", kv_indices, ints, index, self.keys)
+        draft_ptr = _vector("draft_slots", draft_slots, ints, index, tokens)
+        mask_ptr = _vector("tree_mask", tree_mask, torch.int64, index, tokens)
+        dev = self._plan_ptr
+        q_pos = kv_pos = sinks_ptr = lse_ptr = 0
         if window >= 0:
             if q_positions is None or kv_positions is None:
                 raise ValueError("a window needs q_positions and kv_positions")
-            tensors += [q_positions, kv_positions]
-            vectors += [("q_positions", q_positions, tokens, torch.int32),
-                        ("kv_positions", kv_positions, self.keys, torch.int32)]
-        for name, t, n, dt in vectors:
-            if t.dtype != dt or t.ndim != 1 or t.shape[0] < n or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous {dt} vector of the plan's length")
+            q_pos = _vector("q_positions", q_positions, ints, index, tokens)
+            kv_pos = _vector("kv_positions", kv_positions, ints, index, self.keys) or dev
         if sinks is not None:
-            if sinks.dtype != torch.float32 or sinks.shape != (self.hq,) or \
-                    not sinks.is_contiguous():
+            if sinks.shape != (self.hq,):
                 raise ValueError("sinks must be fp32 [num_q_heads]")
-            tensors.append(sinks)
+            sinks_ptr = _vector("sinks", sinks, torch.float32, index, self.hq)
         if out is None:
-            out = torch.empty((tokens, self.hq, self.d), dtype=self.dtype, device=self.device)
-        else:
-            if out.dtype != self.dtype or out.ndim != 3 or out.shape[0] < tokens or \
-                    out.shape[1:] != (self.hq, self.d) or out.stride(-1) != 1:
-                raise ValueError("out must be [tokens, num_q_heads, head_dim] of the planned type")
-            tensors.append(out)
-        for t in tensors:
-            if t.get_device() != index:
-                raise ValueError("tree attention tensors must be on the plan's CUDA device")
-        lse = torch.empty((tokens, self.hq), dtype=torch.float32, device=self.device) \
-            if return_lse else None
-        dev = self._dev.data_ptr()
-        status = _native.launch(
-            index, _native.lib.akv_tree_attention, q.data_ptr(), q.stride(0), q.stride(1),
-            k_pool.data_ptr(), v_pool.data_ptr(), k_pool.stride(0), k_pool.stride(1),
-            v_pool.stride(0), v_pool.stride(1), min(k_pool.shape[0], v_pool.shape[0]),
-            _native.DTYPE_CODE[self.dtype], kv_indices.data_ptr() or dev, draft_slots.data_ptr(),
-            tree_mask.data_ptr(), None if window < 0 else q_positions.data_ptr(),
-            None if window < 0 else kv_positions.data_ptr() or dev, window,
-            None if sinks is None else sinks.data_ptr(), self.sm_scale, self.hq, self.hkv, self.d,
-            dev, dev + 4 * self._at[1], self.n_ctas, dev + 4 * self._at[0], self.n_merges,
-            self._acc.data_ptr(), self._ml.data_ptr(), out.data_ptr(), out.stride(0),
-            out.stride(1), None if lse is None else lse.data_ptr(), self.error_flag.data_ptr())
+            out = torch.empty((tokens, self.hq, self.d), dtype=dtype, device=self.device)
+        o_token, o_head = _rows("out", out, dtype, index, tokens, (self.hq, self.d))
+        lse = None
+        if return_lse:
+            lse = torch.empty((tokens, self.hq), dtype=torch.float32, device=self.device)
+            lse_ptr = lse.data_ptr()
+        status = _native.launch(index, _native.lib.akv_tree_attention, _native.TREE_ATTENTION.pack(
+            q.data_ptr(), q_token, q_head, k_pool.data_ptr(), v_pool.data_ptr(), k_slot, k_head,
+            v_slot, v_head, min(k_pool.shape[0], v_pool.shape[0]), self._code, kv_ptr or dev,
+            draft_ptr, mask_ptr, q_pos, kv_pos, window, sinks_ptr, self.sm_scale, self.hq,
+            self.hkv, self.d, dev, dev + 4 * self._at[1], self.n_ctas, dev + 4 * self._at[0],
+            self.n_merges, *self._partial_ptrs, out.data_ptr(), o_token, o_head, lse_ptr,
+            self._flag_ptr))
         _native.check(status, "tree_attention")
         return (out, lse) if return_lse else out
 

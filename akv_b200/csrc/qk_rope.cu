@@ -267,55 +267,52 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 }  // namespace
 }  // namespace akv
 
-extern "C" int akv_qk_norm_rope(
-    const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k,
-    int64_t k_stride_token, int64_t k_stride_head, const void* v, int64_t v_stride_token,
-    int64_t v_stride_head, int32_t dtype, int64_t tokens, int32_t num_q_heads,
-    int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim, int32_t is_neox_style,
-    const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
-    const void* positions, int32_t positions_is64, const void* cos_sin_cache, int32_t cache_dtype,
-    int64_t cache_stride, int64_t max_position, void* q_out, int64_t q_out_stride_token,
-    int64_t q_out_stride_head, void* k_out, int64_t k_out_stride_token, int64_t k_out_stride_head,
-    void* k_pool, int64_t k_pool_stride_slot, int64_t k_pool_stride_head, void* v_pool,
-    int64_t v_pool_stride_slot, int64_t v_pool_stride_head, int64_t num_slots, const void* slots,
-    int32_t slots_is64, int32_t* error_flag, void* stream) {
+extern "C" int64_t akv_qk_norm_rope_args_bytes(void) { return sizeof(akv_qk_norm_rope_args); }
+
+extern "C" int akv_qk_norm_rope(const akv_qk_norm_rope_args* args, void* stream) {
   AKV_NVTX_RANGE("akv_qk_norm_rope");
   using namespace akv;
-  if (tokens < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
-      head_dim < 16 || head_dim > 512 || head_dim % 16 || rotary_dim <= 0 ||
-      rotary_dim > head_dim || rotary_dim % 16 || dtype < AKV_F16 || dtype > AKV_F32 ||
-      cache_dtype < AKV_F16 || cache_dtype > AKV_F32 ||
-      ((q_weight || k_weight) && weight_dtype != dtype && weight_dtype != AKV_F32))
+  if (args == nullptr) return AKV_ERR_INVALID;
+  const akv_qk_norm_rope_args& x = *args;
+  if (x.tokens < 0 || x.num_q_heads <= 0 || x.num_kv_heads <= 0 || x.num_q_heads > INT32_MAX / 2 ||
+      x.num_kv_heads > INT32_MAX / 2 || x.head_dim < 16 || x.head_dim > 512 || x.head_dim % 16 ||
+      x.rotary_dim <= 0 || x.rotary_dim > x.head_dim || x.rotary_dim % 16 || x.dtype < AKV_F16 ||
+      x.dtype > AKV_F32 || x.cache_dtype < AKV_F16 || x.cache_dtype > AKV_F32 ||
+      ((x.q_weight || x.k_weight) && x.weight_dtype != x.dtype && x.weight_dtype != AKV_F32))
     return AKV_ERR_INVALID;
-  if (tokens == 0) return AKV_OK;
-  if (!q || !k || !q_out || !positions || !cos_sin_cache || max_position <= 0 || (!k_out && !k_pool) ||
-      (k_pool && (!v || !v_pool || !slots || num_slots <= 0)) || (v && !k_pool))
+  if (x.tokens == 0) return AKV_OK;
+  if (!x.q || !x.k || !x.q_out || !x.positions || !x.cos_sin_cache || x.max_position <= 0 ||
+      (!x.k_out && !x.k_pool) ||
+      (x.k_pool && (!x.v || !x.v_pool || !x.slots || x.num_slots <= 0)) || (x.v && !x.k_pool))
     return AKV_ERR_INVALID;
-  const int64_t vec = dtype == AKV_F32 ? 4 : 8;  // elements of a 16-byte access
-  const int64_t cache_vec = cache_dtype == AKV_F32 ? 4 : 8;
-  const int64_t strides[] = {q_stride_token,     q_stride_head,      k_stride_token,
-                             k_stride_head,      v_stride_token,     v_stride_head,
-                             q_out_stride_token, q_out_stride_head,  k_out_stride_token,
-                             k_out_stride_head,  k_pool_stride_slot, k_pool_stride_head,
-                             v_pool_stride_slot, v_pool_stride_head};
+  const int64_t vec = x.dtype == AKV_F32 ? 4 : 8;  // elements of a 16-byte access
+  const int64_t cache_vec = x.cache_dtype == AKV_F32 ? 4 : 8;
+  const int64_t strides[] = {
+      x.q_stride_token,     x.q_stride_head,      x.k_stride_token,     x.k_stride_head,
+      x.v_stride_token,     x.v_stride_head,      x.q_out_stride_token, x.q_out_stride_head,
+      x.k_out_stride_token, x.k_out_stride_head,  x.k_pool_stride_slot, x.k_pool_stride_head,
+      x.v_pool_stride_slot, x.v_pool_stride_head};
   for (int64_t s : strides)
     if (s % vec) return AKV_ERR_INVALID;
-  const void* bases[] = {q,      k,        v,        q_out,        k_out,
-                         k_pool, v_pool,   q_weight, k_weight,     cos_sin_cache};
+  const void* bases[] = {x.q,      x.k,      x.v,        x.q_out,    x.k_out,
+                         x.k_pool, x.v_pool, x.q_weight, x.k_weight, x.cos_sin_cache};
   for (const void* p : bases)
     if (!aligned16(p)) return AKV_ERR_INVALID;
-  if (cache_stride % cache_vec) return AKV_ERR_INVALID;
-  RopeArgs a{q, q_stride_token, q_stride_head, k, k_stride_token, k_stride_head, v,
-             v_stride_token, v_stride_head, q_out, q_out_stride_token, q_out_stride_head, k_out,
-             k_out_stride_token, k_out_stride_head, k_pool, k_pool_stride_slot,
-             k_pool_stride_head, v_pool, v_pool_stride_slot, v_pool_stride_head, q_weight,
-             k_weight, weight_dtype == AKV_F32, eps, positions, positions_is64, slots, slots_is64,
-             cos_sin_cache, cache_dtype, cache_stride, max_position, num_slots, tokens,
-             num_q_heads, num_kv_heads, head_dim, rotary_dim, 0, 0, 0, error_flag};
+  if (x.cache_stride % cache_vec) return AKV_ERR_INVALID;
+  RopeArgs a{x.q, x.q_stride_token, x.q_stride_head, x.k, x.k_stride_token, x.k_stride_head, x.v,
+             x.v_stride_token, x.v_stride_head, x.q_out, x.q_out_stride_token,
+             x.q_out_stride_head, x.k_out, x.k_out_stride_token, x.k_out_stride_head, x.k_pool,
+             x.k_pool_stride_slot, x.k_pool_stride_head, x.v_pool, x.v_pool_stride_slot,
+             x.v_pool_stride_head, x.q_weight, x.k_weight, x.weight_dtype == AKV_F32,
+             (float)x.eps, x.positions, x.positions_is64 != 0, x.slots, x.slots_is64 != 0,
+             x.cos_sin_cache, (int)x.cache_dtype, x.cache_stride, x.max_position, x.num_slots,
+             x.tokens, (int)x.num_q_heads, (int)x.num_kv_heads, (int)x.head_dim,
+             (int)x.rotary_dim, 0, 0, 0, x.error_flag};
+  const int neox = x.is_neox_style != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case AKV_F16: return launch_rope_lanes<__half>(a, is_neox_style, s);
-    case AKV_BF16: return launch_rope_lanes<__nv_bfloat16>(a, is_neox_style, s);
-    default: return launch_rope_lanes<float>(a, is_neox_style, s);
+  switch (x.dtype) {
+    case AKV_F16: return launch_rope_lanes<__half>(a, neox, s);
+    case AKV_BF16: return launch_rope_lanes<__nv_bfloat16>(a, neox, s);
+    default: return launch_rope_lanes<float>(a, neox, s);
   }
 }

@@ -269,38 +269,38 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
 }  // namespace
 }  // namespace akv
 
-extern "C" int akv_map_slots(
-    int32_t* req_to_token, int64_t row_stride, int64_t rows, int64_t columns, const void* row_ids,
-    int32_t row_ids_is64, const void* raw_lens, int32_t raw_lens_is64, const void* new_lens,
-    int32_t new_lens_is64, int32_t batch, int32_t page_size, const int32_t* ring,
-    int64_t* ring_state, int64_t ring_capacity, const void* next_positions, int32_t next_is64,
-    const int32_t* parents, int64_t capacity, int32_t* new_offsets, int32_t* slots,
-    int32_t* positions, int64_t* tree_mask, int32_t* block_table, int64_t table_stride,
-    int64_t table_columns, int32_t* totals, int32_t* status, uint32_t* workspace, int32_t commit,
-    void* stream) {
+extern "C" int64_t akv_map_slots_args_bytes(void) { return sizeof(akv_map_slots_args); }
+
+extern "C" int akv_map_slots(const akv_map_slots_args* args, void* stream) {
   AKV_NVTX_RANGE("akv_map_slots");
   using namespace akv;
-  if (batch < 0 || batch > 65535 || rows < 0 || columns < 0 || row_stride < columns ||
-      ring_capacity <= 0 || capacity < 0 || capacity > INT32_MAX || page_size <= 0 ||
-      page_size > 128 || (page_size & (page_size - 1)) || page_size == 2 ||
-      (block_table && (table_columns < 0 || table_stride < table_columns)))
+  if (args == nullptr) return AKV_ERR_INVALID;
+  const akv_map_slots_args& x = *args;
+  const int64_t page = x.page_size;
+  if (x.batch < 0 || x.batch > 65535 || x.rows < 0 || x.columns < 0 || x.row_stride < x.columns ||
+      x.ring_capacity <= 0 || x.capacity < 0 || x.capacity > INT32_MAX || page <= 0 ||
+      page > 128 || (page & (page - 1)) || page == 2 ||
+      (x.block_table && (x.table_columns < 0 || x.table_stride < x.table_columns)))
     return AKV_ERR_INVALID;
-  if (batch == 0) return AKV_OK;
-  if (!req_to_token || !row_ids || !raw_lens || !new_lens || !ring || !ring_state ||
-      !new_offsets || !totals || !status || !workspace || (capacity > 0 && (!slots || !positions)) ||
-      (parents && capacity > 0 && !tree_mask))
+  if (x.batch == 0) return AKV_OK;
+  if (!x.req_to_token || !x.row_ids || !x.raw_lens || !x.new_lens || !x.ring || !x.ring_state ||
+      !x.new_offsets || !x.totals || !x.status || !x.workspace ||
+      (x.capacity > 0 && (!x.slots || !x.positions)) ||
+      (x.parents && x.capacity > 0 && !x.tree_mask))
     return AKV_ERR_INVALID;
   int shift = 0;
-  while ((1 << shift) < page_size) ++shift;
-  SlotArgs a{req_to_token, row_stride, rows, columns, row_ids, row_ids_is64, raw_lens,
-             raw_lens_is64, new_lens, new_lens_is64, batch, shift, ring,
-             reinterpret_cast<long long*>(ring_state), ring_capacity, next_positions, next_is64,
-             parents, capacity, new_offsets, slots, positions, tree_mask, block_table,
-             table_stride, table_columns, totals, status, workspace, commit};
+  while ((1 << shift) < page) ++shift;
+  const int batch = (int)x.batch;
+  SlotArgs a{x.req_to_token, x.row_stride, x.rows, x.columns, x.row_ids, x.row_ids_is64 != 0,
+             x.raw_lens, x.raw_lens_is64 != 0, x.new_lens, x.new_lens_is64 != 0, batch, shift,
+             x.ring, reinterpret_cast<long long*>(x.ring_state), x.ring_capacity,
+             x.next_positions, x.next_is64 != 0, x.parents, x.capacity, x.new_offsets, x.slots,
+             x.positions, x.tree_mask, x.block_table, x.table_stride, x.table_columns, x.totals,
+             x.status, x.workspace, x.commit != 0};
   // Blocks per request: enough for about six per SM over the batch, no more
   // than the request's share of tokens or its table row can use.
   const long long longest =
-      std::max<long long>(parents ? 1 : capacity, block_table ? table_columns : 1);
+      std::max<long long>(x.parents ? 1 : x.capacity, x.block_table ? x.table_columns : 1);
   const long long want = (longest + 4 * kSlotThreads - 1) / (4 * kSlotThreads);
   const long long fit = std::max(1, kNumSMs * 6 / batch);
   const dim3 grid((unsigned)std::max<long long>(1, std::min(want, fit)), batch);

@@ -827,48 +827,49 @@ int launch_tree(const TreeParams& p, int n_ctas, const TreeMerge* merges, int n_
 
 extern "C" int32_t akv_tree_attention_units(void) { return akv::kTreeUnits; }
 
-extern "C" int akv_tree_attention(
-    const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_pool,
-    const void* v_pool, int64_t k_stride_slot, int64_t k_stride_head, int64_t v_stride_slot,
-    int64_t v_stride_head, int64_t num_slots, int32_t dtype, const int32_t* kv_indices,
-    const int32_t* draft_slots, const int64_t* tree_mask, const int32_t* q_positions,
-    const int32_t* kv_positions, int64_t window, const float* sinks, float sm_scale,
-    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const int32_t* items,
-    const int32_t* cta_items, int32_t n_ctas, const int32_t* merges, int32_t n_merges,
-    float* partial_acc, float* partial_ml, void* out, int64_t out_stride_token,
-    int64_t out_stride_head, float* lse, int32_t* error_flag, void* stream) {
+extern "C" int64_t akv_tree_attention_args_bytes(void) { return sizeof(akv_tree_attention_args); }
+
+extern "C" int akv_tree_attention(const akv_tree_attention_args* args, void* stream) {
   AKV_NVTX_RANGE("akv_tree_attention");
   using namespace akv;
-  if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || n_ctas < 0 ||
-      n_merges < 0 || !(sm_scale > 0.f) || num_slots <= 0 || (dtype != AKV_F16 && dtype != AKV_BF16))
+  if (args == nullptr) return AKV_ERR_INVALID;
+  const akv_tree_attention_args& x = *args;
+  if (x.num_kv_heads <= 0 || x.num_q_heads <= 0 || x.num_q_heads > INT32_MAX / 64 ||
+      x.num_q_heads % x.num_kv_heads || x.n_ctas < 0 || x.n_ctas > INT32_MAX || x.n_merges < 0 ||
+      x.n_merges > INT32_MAX || !(x.sm_scale > 0.) || x.num_slots <= 0 ||
+      x.num_slots > INT32_MAX || (x.dtype != AKV_F16 && x.dtype != AKV_BF16))
     return AKV_ERR_INVALID;
-  if (head_dim != 64 && head_dim != 128) return AKV_ERR_UNSUPPORTED;
-  if (n_ctas == 0) return AKV_OK;
-  if (!q || !k_pool || !v_pool || !draft_slots || !tree_mask || !items || !cta_items || !out ||
-      !kv_indices || (n_merges > 0 && (!merges || !partial_acc || !partial_ml)) ||
-      (window >= 0 && (!q_positions || !kv_positions)))
+  if (x.head_dim != 64 && x.head_dim != 128) return AKV_ERR_UNSUPPORTED;
+  if (x.n_ctas == 0) return AKV_OK;
+  if (!x.q || !x.k_pool || !x.v_pool || !x.draft_slots || !x.tree_mask || !x.items ||
+      !x.cta_items || !x.out || !x.kv_indices ||
+      (x.n_merges > 0 && (!x.merges || !x.partial_acc || !x.partial_ml)) ||
+      (x.window >= 0 && (!x.q_positions || !x.kv_positions)))
     return AKV_ERR_INVALID;
-  const void* bases[] = {q, k_pool, v_pool, out};
+  const void* bases[] = {x.q, x.k_pool, x.v_pool, x.out};
   for (const void* b : bases)
     if (reinterpret_cast<uintptr_t>(b) & 15) return AKV_ERR_INVALID;
-  if (k_stride_slot < 0 || v_stride_slot < 0 || k_stride_slot >= (1ll << 31) ||
-      v_stride_slot >= (1ll << 31))
+  if (x.k_stride_slot < 0 || x.v_stride_slot < 0 || x.k_stride_slot >= (1ll << 31) ||
+      x.v_stride_slot >= (1ll << 31))
     return AKV_ERR_INVALID;  // bytes between slots in 32 bits
-  const int64_t strides[] = {q_stride_token, q_stride_head,    k_stride_slot,  k_stride_head,
-                             v_stride_slot,  v_stride_head,    out_stride_token, out_stride_head};
+  const int64_t strides[] = {x.q_stride_token, x.q_stride_head,    x.k_stride_slot,
+                             x.k_stride_head,  x.v_stride_slot,    x.v_stride_head,
+                             x.out_stride_token, x.out_stride_head};
   for (int64_t s : strides)
     if (s % 8) return AKV_ERR_INVALID;  // 16-byte rows
-  TreeParams p{q, q_stride_token, q_stride_head, k_pool, v_pool, k_stride_slot, k_stride_head,
-               v_stride_slot, v_stride_head, num_slots, kv_indices, draft_slots,
-               reinterpret_cast<const unsigned long long*>(tree_mask), q_positions, kv_positions,
-               window, sinks, sm_scale * kLog2e, num_q_heads / num_kv_heads, num_q_heads,
-               reinterpret_cast<const TreeItem*>(items), cta_items, partial_acc, partial_ml, out,
-               out_stride_token, out_stride_head, lse, error_flag};
-  const TreeMerge* m = reinterpret_cast<const TreeMerge*>(merges);
+  TreeParams p{x.q, x.q_stride_token, x.q_stride_head, x.k_pool, x.v_pool, x.k_stride_slot,
+               x.k_stride_head, x.v_stride_slot, x.v_stride_head, x.num_slots, x.kv_indices,
+               x.draft_slots, reinterpret_cast<const unsigned long long*>(x.tree_mask),
+               x.q_positions, x.kv_positions, x.window, x.sinks, (float)x.sm_scale * kLog2e,
+               (int)(x.num_q_heads / x.num_kv_heads), (int)x.num_q_heads,
+               reinterpret_cast<const TreeItem*>(x.items), x.cta_items, x.partial_acc,
+               x.partial_ml, x.out, x.out_stride_token, x.out_stride_head, x.lse, x.error_flag};
+  const TreeMerge* m = reinterpret_cast<const TreeMerge*>(x.merges);
+  const int n = (int)x.n_ctas, nm = (int)x.n_merges;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == AKV_BF16)
-    return head_dim == 64 ? launch_tree<__nv_bfloat16, 64>(p, n_ctas, m, n_merges, s)
-                          : launch_tree<__nv_bfloat16, 128>(p, n_ctas, m, n_merges, s);
-  return head_dim == 64 ? launch_tree<__half, 64>(p, n_ctas, m, n_merges, s)
-                        : launch_tree<__half, 128>(p, n_ctas, m, n_merges, s);
+  if (x.dtype == AKV_BF16)
+    return x.head_dim == 64 ? launch_tree<__nv_bfloat16, 64>(p, n, m, nm, s)
+                            : launch_tree<__nv_bfloat16, 128>(p, n, m, nm, s);
+  return x.head_dim == 64 ? launch_tree<__half, 64>(p, n, m, nm, s)
+                          : launch_tree<__half, 128>(p, n, m, nm, s);
 }

@@ -663,6 +663,10 @@ int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chun
                      const int32_t* indices, int32_t* error_flag, void* stream);
 
 /*
+ * The three entry points of a drafted-token step take their arguments in one
+ * HOST struct, every member 8 bytes (pointers, int64_t, double), read before
+ * the call returns; <name>_args_bytes() is its size.
+ *
  * Slot maps, positions, draft-tree masks and block tables of the new tokens
  * of a batch, from the requests' lengths, in one launch.  The reference
  * allocates and writes them from the scheduler's Python
@@ -697,15 +701,40 @@ int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chun
  * at most one of them has new tokens.  workspace: DEVICE uint32 [2], zero before the first call and
  * left zero by every call; calls that share it must not overlap.
  */
-int akv_map_slots(int32_t* req_to_token, int64_t row_stride, int64_t rows, int64_t columns,
-                  const void* row_ids, int32_t row_ids_is64, const void* raw_lens,
-                  int32_t raw_lens_is64, const void* new_lens, int32_t new_lens_is64,
-                  int32_t batch, int32_t page_size, const int32_t* ring, int64_t* ring_state,
-                  int64_t ring_capacity, const void* next_positions, int32_t next_is64,
-                  const int32_t* parents, int64_t capacity, int32_t* new_offsets, int32_t* slots,
-                  int32_t* positions, int64_t* tree_mask, int32_t* block_table,
-                  int64_t table_stride, int64_t table_columns, int32_t* totals, int32_t* status,
-                  uint32_t* workspace, int32_t commit, void* stream);
+typedef struct akv_map_slots_args {
+  int32_t* req_to_token;
+  int64_t row_stride;
+  int64_t rows;
+  int64_t columns;
+  const void* row_ids;
+  int64_t row_ids_is64;
+  const void* raw_lens;
+  int64_t raw_lens_is64;
+  const void* new_lens;
+  int64_t new_lens_is64;
+  int64_t batch;
+  int64_t page_size;
+  const int32_t* ring;
+  int64_t* ring_state;
+  int64_t ring_capacity;
+  const void* next_positions;
+  int64_t next_is64;
+  const int32_t* parents;
+  int64_t capacity;
+  int32_t* new_offsets;
+  int32_t* slots;
+  int32_t* positions;
+  int64_t* tree_mask;
+  int32_t* block_table;
+  int64_t table_stride;
+  int64_t table_columns;
+  int32_t* totals;
+  int32_t* status;
+  uint32_t* workspace;
+  int64_t commit;
+} akv_map_slots_args;
+int64_t akv_map_slots_args_bytes(void);
+int akv_map_slots(const akv_map_slots_args* args, void* stream);
 
 /*
  * Per-head RMS norms of Q and K, the position rotation, and the store of K
@@ -728,19 +757,52 @@ int akv_map_slots(int32_t* req_to_token, int64_t row_stride, int64_t rows, int64
  * 16, head_dim at most 512; every base address and stride a multiple of 16
  * bytes.  Two tokens must not have the same slot.
  */
-int akv_qk_norm_rope(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k,
-                     int64_t k_stride_token, int64_t k_stride_head, const void* v,
-                     int64_t v_stride_token, int64_t v_stride_head, int32_t dtype,
-                     int64_t tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                     int32_t rotary_dim, int32_t is_neox_style, const void* q_weight,
-                     const void* k_weight, int32_t weight_dtype, float eps,
-                     const void* positions, int32_t positions_is64, const void* cos_sin_cache,
-                     int32_t cache_dtype, int64_t cache_stride, int64_t max_position, void* q_out,
-                     int64_t q_out_stride_token, int64_t q_out_stride_head, void* k_out,
-                     int64_t k_out_stride_token, int64_t k_out_stride_head, void* k_pool,
-                     int64_t k_pool_stride_slot, int64_t k_pool_stride_head, void* v_pool,
-                     int64_t v_pool_stride_slot, int64_t v_pool_stride_head, int64_t num_slots,
-                     const void* slots, int32_t slots_is64, int32_t* error_flag, void* stream);
+typedef struct akv_qk_norm_rope_args {
+  const void* q;
+  int64_t q_stride_token;
+  int64_t q_stride_head;
+  const void* k;
+  int64_t k_stride_token;
+  int64_t k_stride_head;
+  const void* v;
+  int64_t v_stride_token;
+  int64_t v_stride_head;
+  int64_t dtype;
+  int64_t tokens;
+  int64_t num_q_heads;
+  int64_t num_kv_heads;
+  int64_t head_dim;
+  int64_t rotary_dim;
+  int64_t is_neox_style;
+  const void* q_weight;
+  const void* k_weight;
+  int64_t weight_dtype;
+  double eps;
+  const void* positions;
+  int64_t positions_is64;
+  const void* cos_sin_cache;
+  int64_t cache_dtype;
+  int64_t cache_stride;
+  int64_t max_position;
+  void* q_out;
+  int64_t q_out_stride_token;
+  int64_t q_out_stride_head;
+  void* k_out;
+  int64_t k_out_stride_token;
+  int64_t k_out_stride_head;
+  void* k_pool;
+  int64_t k_pool_stride_slot;
+  int64_t k_pool_stride_head;
+  void* v_pool;
+  int64_t v_pool_stride_slot;
+  int64_t v_pool_stride_head;
+  int64_t num_slots;
+  const void* slots;
+  int64_t slots_is64;
+  int32_t* error_flag;
+} akv_qk_norm_rope_args;
+int64_t akv_qk_norm_rope_args_bytes(void);
+int akv_qk_norm_rope(const akv_qk_norm_rope_args* args, void* stream);
 
 /*
  * Attention of drafted token trees over the paged cache, with learned sinks.
@@ -779,18 +841,44 @@ int akv_qk_norm_rope(const void* q, int64_t q_stride_token, int64_t q_stride_hea
  * invalid); [1] is the launch's abort word, cleared by every launch.
  */
 int32_t akv_tree_attention_units(void);
-int akv_tree_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head,
-                       const void* k_pool, const void* v_pool, int64_t k_stride_slot,
-                       int64_t k_stride_head, int64_t v_stride_slot, int64_t v_stride_head,
-                       int64_t num_slots, int32_t dtype, const int32_t* kv_indices,
-                       const int32_t* draft_slots, const int64_t* tree_mask,
-                       const int32_t* q_positions, const int32_t* kv_positions, int64_t window,
-                       const float* sinks, float sm_scale, int32_t num_q_heads,
-                       int32_t num_kv_heads, int32_t head_dim, const int32_t* items,
-                       const int32_t* cta_items, int32_t n_ctas, const int32_t* merges,
-                       int32_t n_merges, float* partial_acc, float* partial_ml, void* out,
-                       int64_t out_stride_token, int64_t out_stride_head, float* lse,
-                       int32_t* error_flag, void* stream);
+typedef struct akv_tree_attention_args {
+  const void* q;
+  int64_t q_stride_token;
+  int64_t q_stride_head;
+  const void* k_pool;
+  const void* v_pool;
+  int64_t k_stride_slot;
+  int64_t k_stride_head;
+  int64_t v_stride_slot;
+  int64_t v_stride_head;
+  int64_t num_slots;
+  int64_t dtype;
+  const int32_t* kv_indices;
+  const int32_t* draft_slots;
+  const int64_t* tree_mask;
+  const int32_t* q_positions;
+  const int32_t* kv_positions;
+  int64_t window;
+  const float* sinks;
+  double sm_scale;
+  int64_t num_q_heads;
+  int64_t num_kv_heads;
+  int64_t head_dim;
+  const int32_t* items;
+  const int32_t* cta_items;
+  int64_t n_ctas;
+  const int32_t* merges;
+  int64_t n_merges;
+  float* partial_acc;
+  float* partial_ml;
+  void* out;
+  int64_t out_stride_token;
+  int64_t out_stride_head;
+  float* lse;
+  int32_t* error_flag;
+} akv_tree_attention_args;
+int64_t akv_tree_attention_args_bytes(void);
+int akv_tree_attention(const akv_tree_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

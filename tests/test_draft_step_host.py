@@ -9,6 +9,14 @@ _HOST = (ctypes.c_int64 * 64)()  # only its address is used
 BUF = ctypes.c_void_p((ctypes.addressof(_HOST) + 15) & ~15)
 
 
+def packed(struct, args, change):
+    """The argument struct of ``args``, given in its members' order."""
+    from akv_b200 import _native
+
+    values = [getattr(v, "value", v) or 0 for v in {**args, **change}.values()]
+    return getattr(_native, struct).pack(*values), None
+
+
 def slots_args(**change):
     a = dict(req_to_token=BUF, row_stride=8, rows=2, columns=8, row_ids=BUF, row_ids_is64=1,
              raw_lens=BUF, raw_lens_is64=1, new_lens=BUF, new_lens_is64=1, batch=2, page_size=4,
@@ -17,7 +25,7 @@ def slots_args(**change):
              block_table=None, table_stride=0, table_columns=0, totals=BUF, status=BUF,
              workspace=BUF, commit=1)
     assert set(change) <= set(a)
-    return [*{**a, **change}.values(), None]
+    return packed("MAP_SLOTS", a, change)
 
 
 @pytest.mark.parametrize("change", [
@@ -49,7 +57,7 @@ def rope_args(**change):
              k_pool=None, kp_ss=0, kp_sh=0, v_pool=None, vp_ss=0, vp_sh=0, num_slots=0, slots=None,
              slots_is64=0, flag=None)
     assert set(change) <= set(a)
-    return [*{**a, **change}.values(), None]
+    return packed("QK_NORM_ROPE", a, change)
 
 
 ODD = ctypes.c_void_p(BUF.value + 8)  # not on a 16-byte boundary
@@ -78,6 +86,29 @@ def test_qk_norm_rope_of_no_token_is_ok():
     assert _native.lib.akv_qk_norm_rope(*rope_args(tokens=0)) == _native.AKV_OK
 
 
+def test_argument_structs_match_the_header():
+    """Members in the header's order, doubles where it has doubles, its size;
+    no struct is refused."""
+    import os
+    import re
+
+    from akv_b200 import _native
+    from conftest import ROOT
+
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "akv_b200.h")).read(),
+                  flags=re.S)
+    for name, mirror in (("akv_map_slots", _native.MAP_SLOTS),
+                         ("akv_qk_norm_rope", _native.QK_NORM_ROPE),
+                         ("akv_tree_attention", _native.TREE_ATTENTION)):
+        end = text.index("} %s_args;" % name)
+        members = text[text.rindex("{", 0, end) + 1: end].split(";")[:-1]
+        assert [re.sub(r".*[ *]", "", m.strip()) for m in members] == mirror.names
+        assert "".join("d" if m.split()[0] == "double" else "q" for m in members) == \
+            mirror.struct.format
+        assert getattr(_native.lib, name + "_args_bytes")() == mirror.struct.size
+        assert getattr(_native.lib, name)(None, None) == _native.AKV_ERR_INVALID
+
+
 def test_wrappers_refuse_cpu_tensors():
     import torch
 
@@ -94,7 +125,7 @@ def tree_args(**change):
              scale=1.0, hq=8, hkv=2, dim=64, items=BUF, cta_items=BUF, n_ctas=1, merges=None, n_merges=0,
              acc=None, ml=None, out=BUF, o_st=512, o_sh=64, lse=None, flag=None)
     assert set(change) <= set(a)
-    return [*{**a, **change}.values(), None]
+    return packed("TREE_ATTENTION", a, change)
 
 
 @pytest.mark.parametrize("change", [
