@@ -13,18 +13,23 @@
 //   modules around akv/system/sglang.patch:2437-2445).
 //
 // Bound: HBM.  Each element is read and written once.  A row is shared by
-// D / 16 lanes, each with two 16-byte pieces that rotate into one another
-// (elements [8j, 8j + 8) and [R/2 + 8j, ..) with halves, [16j, 16j + 16) with
-// pairs), so the rotation needs no exchange and the norm's sum is log2(D/16)
-// shuffles.  A lane keeps its 8 cos, 8 sin and 16 weights in registers over
-// kRows rows of its token, all of which it requests before it uses the first.
+// D / 16 lanes, each with two 8-element pieces: with halves the two that
+// rotate into one another ([8j, 8j + 8) and [R/2 + 8j, ..)), with pairs j and
+// j + D/16, which rotate within themselves.  So the rotation needs no exchange,
+// the lanes of an access are neighbours, and the norm's sum is log2(D/16)
+// shuffles.  A lane keeps its 8 cos, 8 sin and 16 weights in registers for the
+// two rows (one in fp32) that it requests before it uses the first.  Measured on
+// 16,411 tokens of 64 + 8 + 8 heads of 128, bf16 (681 MB): 142 us, 4.8 TB/s,
+// 0.73 of the copy rate, at 8 blocks of 128 threads per SM; four rows per lane
+// (102 registers, 5 blocks) 156-179 us, one row 177 us, two rows at a time
+// in a loop that keeps the table row 160 us (spills): residency counts most.
 
 #include "common.cuh"
 
 namespace akv {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 
 struct RopeArgs {
   const void* q;
@@ -86,15 +91,37 @@ __device__ __forceinline__ void load8(const void* base, long long at, float (&ou
   for (int i = 0; i < 8; ++i) out[i] = e.get(i);
 }
 
+// Four consecutive elements (8 or 16 bytes), as fp32.
+template <typename T>
+__device__ __forceinline__ void load4(const void* base, long long at, float* out) {
+  struct alignas(4 * sizeof(T)) Four { T e[4]; };
+  const Four f = *reinterpret_cast<const Four*>(static_cast<const T*>(base) + at);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = Elem<T>::to_f32(f.e[i]);
+}
+
+// The eight cosines (or sines) of a lane's two runs: at a one run of eight
+// (halves), or four at a and, if `both`, four at b (pairs).
+template <typename T, bool NEOX>
+__device__ __forceinline__ void load_turn(const void* base, long long a, long long b, bool both,
+                                          float (&out)[8]) {
+  if (NEOX) {
+    load8<T>(base, a, out);
+  } else {
+    load4<T>(base, a, out);
+    if (both) load4<T>(base, b, out + 4);
+  }
+}
+
 // T: element type; LANES: lanes per row (D / 16 rounded up to a power of
 // two); NEOX: halves or adjacent pairs; ROWS: rows per lane group.
 template <typename T, int LANES, bool NEOX, int ROWS>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeArgs a) {
-  const long long group =
-      ((long long)blockIdx.x * kRopeThreads + threadIdx.x) / LANES;
+__global__ void __launch_bounds__(kRopeThreads, 8) qk_norm_rope_kernel(const RopeArgs a) {
+  const uint32_t group = blockIdx.x * (kRopeThreads / LANES) + threadIdx.x / LANES;
   const int j = threadIdx.x % LANES;
-  const long long token = group / a.units;
-  const int unit = (int)(group - token * a.units);
+  const uint32_t token32 = group / (uint32_t)a.units;
+  const int unit = (int)(group - token32 * a.units);
+  const long long token = token32;
   if (token >= a.tokens) return;  // whole lane groups leave together
   // Shuffles stay inside the lane group, whose lanes all take the same path.
   const unsigned lanes =
@@ -104,11 +131,15 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeAr
   const int first =
       (kind == 0 ? unit : kind == 1 ? unit - a.q_units : unit - a.q_units - a.k_units) * ROWS;
   const int heads = kind == 0 ? a.hq : a.hkv;
-  const bool live = 16 * j < a.dim;  // D / 16 need not be a power of two
-  const bool turned = 16 * j < a.rotary;
-  // This lane's two runs of eight elements.
-  const int e0 = NEOX && turned ? 8 * j : 16 * j;
-  const int e1 = NEOX && turned ? a.rotary / 2 + 8 * j : 16 * j + 8;
+  // This lane's two runs of eight elements.  Halves: [8j, 8j + 8) of the
+  // first half and of the second, and past the rotation the same of the rest.
+  // Pairs: pieces j and j + LANES of the row, each turning within itself.
+  const int half = a.rotary / 2, t = j - a.rotary / 16;
+  const bool turned = NEOX ? t < 0 : 8 * j < a.rotary;
+  const bool turned1 = NEOX ? turned : 8 * (j + LANES) < a.rotary;
+  const int e0 = NEOX && t >= 0 ? a.rotary + 8 * t : 8 * j;
+  const int e1 = !NEOX ? 8 * (j + LANES) : t >= 0 ? (a.rotary + a.dim) / 2 + 8 * t : half + 8 * j;
+  const bool live = NEOX ? 16 * j < a.dim : 8 * j < a.dim, live1 = NEOX ? live : e1 < a.dim;
 
   const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v);
   const long long st = kind == 0 ? a.q_st : kind == 1 ? a.k_st : a.v_st;
@@ -117,9 +148,9 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeAr
   Eight<T> x0[ROWS], x1[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
-    if (live && first + r < heads) {
-      x0[r].load(src + r * sh + e0);
-      x1[r].load(src + r * sh + e1);
+    if (first + r < heads) {
+      if (live) x0[r].load(src + r * sh + e0);
+      if (live1) x1[r].load(src + r * sh + e1);
     }
 
   long long slot = -1;
@@ -137,46 +168,45 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeAr
     slot = -1;
   }
   if (kind == 2) {
-    if (slot < 0 || !live) return;
+    if (slot < 0) return;
     T* dst = static_cast<T*>(a.v_pool) + slot * a.vp_ss + first * a.vp_sh;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
       if (first + r < heads) {
-        x0[r].store(dst + r * a.vp_sh + e0);
-        x1[r].store(dst + r * a.vp_sh + e1);
+        if (live) x0[r].store(dst + r * a.vp_sh + e0);
+        if (live1) x1[r].store(dst + r * a.vp_sh + e1);
       }
     return;
   }
 
   float c[8], s[8];
-  if (turned) {
-    const long long at = pos * a.table_stride + 8 * j;
-    if (a.table_dtype == AKV_F32) {
-      load8<float>(a.table, at, c);
-      load8<float>(a.table, at + a.rotary / 2, s);
-    } else if (a.table_dtype == AKV_BF16) {
-      load8<__nv_bfloat16>(a.table, at, c);
-      load8<__nv_bfloat16>(a.table, at + a.rotary / 2, s);
-    } else {
-      load8<__half>(a.table, at, c);
-      load8<__half>(a.table, at + a.rotary / 2, s);
-    }
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] = 1.f;
-      s[i] = 0.f;
+  for (int i = 0; i < 8; ++i) {
+    c[i] = 1.f;
+    s[i] = 0.f;
+  }
+  if (turned) {
+    const long long at = pos * a.table_stride + (NEOX ? 8 : 4) * j, at1 = at + 4 * LANES;
+    if (a.table_dtype == AKV_F32) {
+      load_turn<float, NEOX>(a.table, at, at1, turned1, c);
+      load_turn<float, NEOX>(a.table, at + half, at1 + half, turned1, s);
+    } else if (a.table_dtype == AKV_BF16) {
+      load_turn<__nv_bfloat16, NEOX>(a.table, at, at1, turned1, c);
+      load_turn<__nv_bfloat16, NEOX>(a.table, at + half, at1 + half, turned1, s);
+    } else {
+      load_turn<__half, NEOX>(a.table, at, at1, turned1, c);
+      load_turn<__half, NEOX>(a.table, at + half, at1 + half, turned1, s);
     }
   }
   const void* weight = kind == 0 ? a.q_weight : a.k_weight;
   float w0[8], w1[8];
-  if (weight != nullptr && live) {
+  if (weight != nullptr) {
     if (a.weight_f32) {
-      load8<float>(weight, e0, w0);
-      load8<float>(weight, e1, w1);
+      if (live) load8<float>(weight, e0, w0);
+      if (live1) load8<float>(weight, e1, w1);
     } else {
-      load8<T>(weight, e0, w0);
-      load8<T>(weight, e1, w1);
+      if (live) load8<T>(weight, e0, w0);
+      if (live1) load8<T>(weight, e1, w1);
     }
   }
 
@@ -194,7 +224,7 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeAr
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       y0[i] = live ? x0[r].get(i) : 0.f;
-      y1[i] = live ? x1[r].get(i) : 0.f;
+      y1[i] = live1 ? x1[r].get(i) : 0.f;
     }
     if (weight != nullptr) {
       float ss = 0.f;
@@ -203,21 +233,18 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeAr
 #pragma unroll
       for (int d = LANES / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(lanes, ss, d);
       const float inv = rsqrtf(ss / (float)a.dim + a.eps);
-      if (live) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          y0[i] *= inv * w0[i];
-          y1[i] *= inv * w1[i];
-        }
+      for (int i = 0; i < 8; ++i) {
+        if (live) y0[i] *= inv * w0[i];
+        if (live1) y1[i] *= inv * w1[i];
       }
     }
-    if (!live) continue;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (NEOX) {
         x0[r].set(i, y0[i] * c[i] - y1[i] * s[i]);
         x1[r].set(i, y1[i] * c[i] + y0[i] * s[i]);
-      } else if (i < 4) {  // pairs 0-3 of the lane's run in y0, 4-7 in y1
+      } else if (i < 4) {
         x0[r].set(2 * i, y0[2 * i] * c[i] - y0[2 * i + 1] * s[i]);
         x0[r].set(2 * i + 1, y0[2 * i + 1] * c[i] + y0[2 * i] * s[i]);
         x1[r].set(2 * i, y1[2 * i] * c[4 + i] - y1[2 * i + 1] * s[4 + i]);
@@ -225,25 +252,25 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeAr
       }
     }
     if (out != nullptr) {
-      x0[r].store(out + r * oh + e0);
-      x1[r].store(out + r * oh + e1);
+      if (live) x0[r].store(out + r * oh + e0);
+      if (live1) x1[r].store(out + r * oh + e1);
     }
     if (pool != nullptr) {
-      x0[r].store(pool + r * a.kp_sh + e0);
-      x1[r].store(pool + r * a.kp_sh + e1);
+      if (live) x0[r].store(pool + r * a.kp_sh + e0);
+      if (live1) x1[r].store(pool + r * a.kp_sh + e1);
     }
   }
 }
 
 template <typename T, int LANES, bool NEOX>
 int launch_rope(RopeArgs& a, cudaStream_t stream) {
-  constexpr int ROWS = sizeof(T) == 4 ? 2 : 4;
+  constexpr int ROWS = sizeof(T) == 4 ? 1 : 2;
   a.q_units = (a.hq + ROWS - 1) / ROWS;
   a.k_units = (a.hkv + ROWS - 1) / ROWS;
   a.units = a.q_units + a.k_units * (a.v != nullptr ? 2 : 1);
-  const long long threads = a.tokens * a.units * LANES;
-  const long long blocks = (threads + kRopeThreads - 1) / kRopeThreads;
-  if (blocks > INT32_MAX) return AKV_ERR_INVALID;
+  const long long groups = a.tokens * a.units, per = kRopeThreads / LANES;
+  const long long blocks = (groups + per - 1) / per;
+  if (groups + per > UINT32_MAX) return AKV_ERR_INVALID;  // 32-bit group numbers
   qk_norm_rope_kernel<T, LANES, NEOX, ROWS><<<(unsigned)blocks, kRopeThreads, 0, stream>>>(a);
   return launch_status();
 }
