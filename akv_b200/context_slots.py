@@ -101,7 +101,9 @@ class SlotMapper:
         the Drop's ``next_position`` (default ``raw_lens``).  ``parents``:
         int32, one per new token, the parent's number in the request or -1
         (at most 64 new tokens per request); positions then follow the
-        depth.  ``block_table``: int32 [>= batch, columns], filled with the
+        depth.  A row whose last page a Drop has freed (all of its tokens
+        dropped) is passed with ``raw_lens`` rounded up to whole pages, or the
+        new tokens would go on in that page.  ``block_table``: int32 [>= batch, columns], filled with the
         page ids of whole rows.  Two requests of one call must not share a
         row, unless at most one of them has new tokens.  Failures that only
         the device sees are bits of ``status`` (``SlotMap.check``)."""

@@ -676,7 +676,9 @@ int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chun
  * columns], row stride row_stride); its raw_lens[b] tokens fill the row's
  * first columns and it receives new_lens[b] more.  page_size (1, or a power
  * of two from 4 to 128): token t sits at offset t % page_size of its page.
- * New tokens continue the row's last page, then take pages from the free ring
+ * New tokens continue the row's last page (which must not have been freed: a
+ * row whose last page a Drop freed has its length rounded up to whole pages),
+ * then take pages from the free ring
  * (akv_drop_compact's: ring[ring_capacity], ring_state = {head, tail}) in
  * request order.  With `commit` the ring's head moves past them; without it
  * they are lent: the next call gives out the same pages.

@@ -43,7 +43,7 @@ def compacted(page, seed):
     req_to_token = torch.from_numpy(table).cuda()
     ring = FreeSlotRing(torch.from_numpy(ids[at:]), capacity=len(ids) + 200, device="cuda")
     comp = DropCompactor(int(counts.sum()), 3, len(ranges) // 2, torch.device("cuda", 0))
-    res = comp.run(counts, range_offsets, ranges, row_ids, req_to_token, ring, page_size=page)
+    res = comp.run(counts, range_offsets, ranges, req_to_token, row_ids, ring, page_size=page)
     torch.cuda.synchronize()
     assert int(res.status[0]) == 0
     slots = (int(ids.max()) + 1) * page
