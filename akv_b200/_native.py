@@ -81,9 +81,10 @@ QK_NORM_ROPE = PackedArgs(
     "v_pool_stride_head num_slots slots slots_is64 error_flag")
 TREE_ATTENTION = PackedArgs(
     "q q_stride_token q_stride_head k_pool v_pool k_stride_slot k_stride_head v_stride_slot "
-    "v_stride_head num_slots dtype kv_indices draft_slots tree_mask q_positions kv_positions "
-    "window sinks sm_scale/d num_q_heads num_kv_heads head_dim items cta_items n_ctas merges "
-    "n_merges partial_acc partial_ml out out_stride_token out_stride_head lse error_flag")
+    "v_stride_head num_slots dtype tokens keys kv_indices draft_slots tree_mask q_positions "
+    "kv_positions window sinks sm_scale/d num_q_heads num_kv_heads head_dim items cta_items "
+    "n_ctas merges n_merges partial_acc partial_ml out out_stride_token out_stride_head lse "
+    "error_flag")
 
 # name -> argument types, in the order of include/akv_b200.h
 SIGNATURES = {

@@ -125,8 +125,10 @@ def _vector(name, t, dtype, index, n):
 
 class TreeAttention:
     """Plans and partial results live in the instance: runs of one instance,
-    replays of its graphs among them, must not overlap on the device, and a
-    captured run reads the plan that the device holds when it replays."""
+    replays of its graphs among them, must not overlap on the device.  A
+    captured run keeps its launch sizes but reads the plan that the device
+    holds when it replays, so a new plan needs a new capture; one with as many
+    CTAs, merges, tokens and keys (the same lengths in another order) does not."""
 
     def __init__(self, num_q_heads, num_kv_heads, head_dim, max_batch, device, *,
                  dtype=torch.bfloat16, sm_scale=None, ctas=None):
@@ -136,8 +138,8 @@ class TreeAttention:
             raise ValueError("tree attention supports head_dim 64 and 128")
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("tree attention runs on bf16 or fp16")
-        if max_batch <= 0:
-            raise ValueError("max_batch must be positive")
+        if max_batch <= 0 or (ctas is not None and ctas <= 0):
+            raise ValueError("max_batch and ctas must be positive")
         if sm_scale is not None and not sm_scale > 0:
             raise ValueError("sm_scale must be positive")
         device = torch.device(device)
@@ -165,8 +167,8 @@ class TreeAttention:
         self._dev = torch.zeros(size, dtype=torch.int32, device=device)
         self._acc = torch.empty((partials, TILE_ROWS, head_dim), dtype=torch.float32, device=device)
         self._ml = torch.empty((partials, TILE_ROWS, 2), dtype=torch.float32, device=device)
-        # [0]: error bits kept until check(); [1]: the abort word of the current launch.
-        self.error_flag = torch.zeros(2, dtype=torch.int32, device=device)
+        # Error bits, kept until check().
+        self.error_flag = torch.zeros(1, dtype=torch.int32, device=device)
         self._plan_ptr, self._flag_ptr = self._dev.data_ptr(), self.error_flag.data_ptr()
         self._partial_ptrs = self._acc.data_ptr(), self._ml.data_ptr()
         self._code = _native.DTYPE_CODE[dtype]
@@ -240,7 +242,8 @@ class TreeAttention:
             lse_ptr = lse.data_ptr()
         status = _native.launch(index, _native.lib.akv_tree_attention, _native.TREE_ATTENTION.pack(
             q.data_ptr(), q_token, q_head, k_pool.data_ptr(), v_pool.data_ptr(), k_slot, k_head,
-            v_slot, v_head, min(k_pool.shape[0], v_pool.shape[0]), self._code, kv_ptr or dev,
+            v_slot, v_head, min(k_pool.shape[0], v_pool.shape[0]), self._code, tokens, self.keys,
+            kv_ptr or dev,
             draft_ptr, mask_ptr, q_pos, kv_pos, window, sinks_ptr, self.sm_scale, self.hq,
             self.hkv, self.d, dev, dev + 4 * self._at[1], self.n_ctas, dev + 4 * self._at[0],
             self.n_merges, *self._partial_ptrs, out.data_ptr(), o_token, o_head, lse_ptr,
@@ -249,7 +252,8 @@ class TreeAttention:
         return (out, lse) if return_lse else out
 
     ERRORS = {1: "a key slot outside the KV pools was read as slot 0",
-              2: "a wait inside the kernel ran out; the output of that launch is invalid"}
+              2: "a wait inside the kernel ran out; the output of that launch is invalid",
+              4: "a captured run was replayed on a plan of more tokens or keys"}
 
     def check(self):
         """Raise RuntimeError if a launch since the last check reported an

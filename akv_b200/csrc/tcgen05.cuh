@@ -152,6 +152,19 @@ __device__ __forceinline__ void tmem_st16_sync(uint32_t ta, const uint32_t* a) {
       "r"(a[15])
       : "memory");
 }
+// A store of 16 columns; tmem_st_wait() then ends all of the thread's stores.
+__device__ __forceinline__ void tmem_st16_async(uint32_t ta, const uint32_t (&a)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,"
+      "%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(ta),
+      "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(a[4]), "r"(a[5]), "r"(a[6]), "r"(a[7]),
+      "r"(a[8]), "r"(a[9]), "r"(a[10]), "r"(a[11]), "r"(a[12]), "r"(a[13]), "r"(a[14]),
+      "r"(a[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 // Two stores of 16 columns (P's hi and lo words) and their wait.
 __device__ __forceinline__ void tmem_st16x2_sync(uint32_t ta, const uint32_t* a, uint32_t tb,
                                                  const uint32_t* b) {

@@ -45,6 +45,7 @@ struct TreeParams {
   const void* v;
   long long k_ss, k_sh, v_ss, v_sh;
   long long num_slots;
+  long long tokens, keys;  // entries of the token and key vectors
   const int* kv_indices;
   const int* draft_slots;
   const unsigned long long* tree_mask;
@@ -75,6 +76,16 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Key tiles of an item: none if it reaches past the call's vectors, as one of
+// a plan made after the call was captured may.
+__device__ __forceinline__ int item_tiles(const TreeParams& p, const TreeItem& w) {
+  if ((long long)w.q0 + w.n > p.tokens || (long long)w.kv0 + w.prefix > p.keys) {
+    if (p.error_flag) atomicOr(p.error_flag, 4);
+    return 0;
+  }
+  return (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
 }
 
 // Slot of key j of an item; -1: a padding token, read as zeros.
@@ -363,13 +374,12 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
       uint32_t cnt = 0, n_q = 0;
       bool ok = true;
       for (int it = it0; it < it1 && ok; ++it) {
-        const int4 w1 = reinterpret_cast<const int4*>(p.items + it)[1];  // lo, hi, head0, tile0
-        const int4 w2 = reinterpret_cast<const int4*>(p.items + it)[2];  // steps, units, partial
-        const int n_tiles = (w1.y - w1.x + kTreeKeys - 1) / kTreeKeys;
-        const bool pair = w2.z == 2;
+        const TreeItem w = p.items[it];
+        const int n_tiles = item_tiles(p, w);
+        const bool pair = w.units == 2;
         const int step = pair ? 1 : 2;
         const int n = pair ? n_tiles : (n_tiles - u + 1) / 2;  // this unit's tiles
-        const uint32_t ring = base + C::kRingOff + (w2.x ? u * C::kHeadBytes : 0);
+        const uint32_t ring = base + C::kRingOff + (w.head_step ? u * C::kHeadBytes : 0);
         auto release = [&](uint32_t slot) {
           umma_commit(bar_empty(slot));
           if (!pair) umma_commit(bar_empty(slot));
@@ -439,7 +449,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     bool ok = true;
     for (int it = it0; it < it1 && ok; ++it) {
       const TreeItem w = p.items[it];
-      const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
+      const int n_tiles = item_tiles(p, w);
       const int heads = w.head_step ? 2 : 1;
       auto fetch = [&](int t) {
         const int j = w.lo + t * kTreeKeys + kKpw * pw + lane % kKpw;
@@ -527,7 +537,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         const TreeItem w = p.items[it];
         const int row = (w.tile0 + u * w.tile_step) * kTreeRows + r;
         const int i = row / p.group, h = (w.head0 + u * w.head_step) * p.group + row - i * p.group;
-        if (i < w.n) {
+        if (i < w.n && item_tiles(p, w) > 0) {
           const T* src = static_cast<const T*>(p.q) + (long long)(w.q0 + i) * p.q_st +
                          (long long)h * p.q_sh;
 #pragma unroll
@@ -540,14 +550,14 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     load_q(it0);
     for (int it = it0; it < it1; ++it) {
       const TreeItem w = p.items[it];
-      const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
+      const int n_tiles = item_tiles(p, w);
       const bool pair = w.units == 2;
       const int n = pair ? n_tiles : (n_tiles - u + 1) / 2;
       const int head = w.head0 + u * w.head_step;
       const int row0 = (w.tile0 + u * w.tile_step) * kTreeRows;
       const int i = (row0 + r) / p.group, h = head * p.group + (row0 + r) - i * p.group;
-      const bool live = i < w.n;
-      const bool warp_live = row0 + (warp & 3) * 32 < w.n * p.group;
+      const bool live = i < w.n && n_tiles > 0;
+      const bool warp_live = n_tiles > 0 && row0 + (warp & 3) * 32 < w.n * p.group;
       const unsigned long long mask = live ? row_mask(p, w, i) : 0;
       const int pos = live && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
       cp_async_wait<0>();
@@ -641,8 +651,9 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
             // P's columns, and O's, are free once the product before is done
             // (with P over the scores S(c) came after it).
             if (b == kTreeKeys - 32 && kFree && c > 0) ok = warp_wait(bar_o(u), c - 1 & 1, abort);
-            tmem_st16_sync(tu + C::kColP + b / 2, pk);
+            tmem_st16_async(tu + C::kColP + b / 2, pk);
           }
+          tmem_st_wait();
           float l0, l1;
           f2_unpack(f2_add(sum[0], sum[1]), l0, l1);
           l = l * alpha + (l0 + l1);
@@ -778,7 +789,7 @@ tree_merge_kernel(const TreeParams p, const TreeMerge* merges) {
   const int head = g.head0 + u * (g.steps & 1);
   const int row = (g.tile0 + u * (g.steps >> 1 & 1)) * kTreeRows + r;
   const int i = row / p.group, h = head * p.group + row % p.group;
-  if (i >= g.n) return;
+  if (i >= g.n || g.q0 + g.n > p.tokens) return;
   pdl_wait();
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) +
                      ((long long)g.first + u) * kTreeRows + r;
@@ -836,7 +847,7 @@ extern "C" int akv_tree_attention(const akv_tree_attention_args* args, void* str
   const akv_tree_attention_args& x = *args;
   if (x.num_kv_heads <= 0 || x.num_q_heads <= 0 || x.num_q_heads > INT32_MAX / 64 ||
       x.num_q_heads % x.num_kv_heads || x.n_ctas < 0 || x.n_ctas > INT32_MAX || x.n_merges < 0 ||
-      x.n_merges > INT32_MAX || !(x.sm_scale > 0.) || x.num_slots <= 0 ||
+      x.n_merges > INT32_MAX || x.tokens < 0 || x.keys < 0 || !(x.sm_scale > 0.) || x.num_slots <= 0 ||
       x.num_slots > INT32_MAX || (x.dtype != AKV_F16 && x.dtype != AKV_BF16))
     return AKV_ERR_INVALID;
   if (x.head_dim != 64 && x.head_dim != 128) return AKV_ERR_UNSUPPORTED;
@@ -858,7 +869,8 @@ extern "C" int akv_tree_attention(const akv_tree_attention_args* args, void* str
   for (int64_t s : strides)
     if (s % 8) return AKV_ERR_INVALID;  // 16-byte rows
   TreeParams p{x.q, x.q_stride_token, x.q_stride_head, x.k_pool, x.v_pool, x.k_stride_slot,
-               x.k_stride_head, x.v_stride_slot, x.v_stride_head, x.num_slots, x.kv_indices,
+               x.k_stride_head, x.v_stride_slot, x.v_stride_head, x.num_slots, x.tokens, x.keys,
+               x.kv_indices,
                x.draft_slots, reinterpret_cast<const unsigned long long*>(x.tree_mask),
                x.q_positions, x.kv_positions, x.window, x.sinks, (float)x.sm_scale * kLog2e,
                (int)(x.num_q_heads / x.num_kv_heads), (int)x.num_q_heads,

@@ -698,7 +698,8 @@ int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chun
  * status (int32): AKV_SLOTS_* bits of this call.  RING_UNDERFLOW and CAPACITY
  * refuse the whole call (slots -1; rows, block table and ring untouched);
  * BAD_REQUEST treats that request as one without new tokens; BAD_PAGE leaves
- * that request's slots -1 and its row and block table untouched; BAD_PARENT
+ * that request's slots -1 and its row and block table untouched (its pages
+ * count as taken); BAD_PARENT
  * makes the token a root.  Two requests of a call must not share a row, unless
  * at most one of them has new tokens.  workspace: DEVICE uint32 [2], zero before the first call and
  * left zero by every call; calls that share it must not overlap.
@@ -838,9 +839,11 @@ int akv_qk_norm_rope(const akv_qk_norm_rope_args* args, void* stream);
  * 4][128][4], partial_ml fp32 [partials][128][2].  tree_work_list of
  * akv_b200/context_tree.py builds all of them.
  *
- * error_flag: DEVICE int32 [2] or NULL: [0] collects 1 (a slot outside the
- * pools, read as slot 0) and 2 (a wait ran out: the launch's output is
- * invalid); [1] is the launch's abort word, cleared by every launch.
+ * tokens and keys are the lengths of the token vectors (q, out, draft_slots,
+ * tree_mask, q_positions) and key vectors (kv_indices, kv_positions); an item
+ * that reaches past them is left out.  error_flag: DEVICE int32 or NULL,
+ * collects 1 (a slot outside the pools, read as slot 0), 2 (a wait ran out: the
+ * launch's output is invalid) and 4 (an item past tokens or keys).
  */
 int32_t akv_tree_attention_units(void);
 typedef struct akv_tree_attention_args {
@@ -855,6 +858,8 @@ typedef struct akv_tree_attention_args {
   int64_t v_stride_head;
   int64_t num_slots;
   int64_t dtype;
+  int64_t tokens;
+  int64_t keys;
   const int32_t* kv_indices;
   const int32_t* draft_slots;
   const int64_t* tree_mask;

@@ -121,7 +121,7 @@ def test_wrappers_refuse_cpu_tensors():
 
 def tree_args(**change):
     a = dict(q=BUF, q_st=512, q_sh=64, k=BUF, v=BUF, k_ss=128, k_sh=64, v_ss=128, v_sh=64, slots=8,
-             dtype=1, indices=BUF, draft=BUF, mask=BUF, qpos=None, kpos=None, window=-1, sinks=None,
+             dtype=1, tokens=8, keys=8, indices=BUF, draft=BUF, mask=BUF, qpos=None, kpos=None, window=-1, sinks=None,
              scale=1.0, hq=8, hkv=2, dim=64, items=BUF, cta_items=BUF, n_ctas=1, merges=None, n_merges=0,
              acc=None, ml=None, out=BUF, o_st=512, o_sh=64, lse=None, flag=None)
     assert set(change) <= set(a)
@@ -129,7 +129,8 @@ def tree_args(**change):
 
 
 @pytest.mark.parametrize("change", [
-    dict(hkv=0), dict(hq=0), dict(hq=9), dict(n_ctas=-1), dict(n_merges=-1), dict(slots=0), dict(dtype=2),
+    dict(hkv=0), dict(hq=0), dict(hq=9), dict(n_ctas=-1), dict(tokens=-1), dict(keys=-1),
+    dict(scale=0.0), dict(scale=float("nan")), dict(k_ss=-8), dict(v_ss=1 << 31), dict(slots=1 << 31), dict(n_merges=-1), dict(slots=0), dict(dtype=2),
     dict(q=None), dict(k=None), dict(v=None), dict(indices=None), dict(draft=None), dict(mask=None),
     dict(items=None), dict(cta_items=None), dict(out=None), dict(n_merges=1), dict(window=3),
     dict(window=3, qpos=BUF), dict(q=ODD), dict(k=ODD), dict(v=ODD), dict(out=ODD), dict(q_st=516),

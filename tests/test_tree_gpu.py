@@ -124,7 +124,7 @@ def check(c, ctas=None):
     attn = attention(c, ctas)
     out, lse = launch(c, attn, return_lse=True)
     torch.cuda.synchronize()
-    assert attn.error_flag.tolist()[0] == 0
+    assert int(attn.error_flag) == 0
     compare(c, out, lse)
     return out, lse
 
@@ -240,7 +240,7 @@ def test_padding_tokens_read_as_zeros_and_bad_slots_are_reported():
     attn.check()
     c["indices"][3] = -1
     launch(c, attn)
-    assert int(attn.error_flag[0]) == 1
+    assert int(attn.error_flag) == 1
 
 
 def test_strided_pools_and_outputs():
@@ -288,6 +288,37 @@ def test_replayed_graphs_follow_masks_slots_and_plans():
     out.zero_()
     graph.replay()
     assert torch.equal(out, launch(other, attention(other)))
+
+
+def test_a_replay_on_a_larger_plan_stays_in_its_tensors():
+    """The captured call's vectors bound it, whatever plan the device holds."""
+    c = make([100, 200], [8, 8], 2, 8, 64, torch.bfloat16, seed=10)
+    attn = attention(c)
+    wide = torch.full((200, 16, 64), 3.0, dtype=c["dtype"], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    launch(c, attn, out=wide)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        launch(c, attn, out=wide)
+    attn.plan([0, 100, 400], [0, 64, 128])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((wide[16:] == 3).all())
+    with pytest.raises(RuntimeError, match="replayed"):
+        attn.check()
+    attn.plan(c["kv"], c["dr"])
+    graph.replay()
+    assert torch.equal(wide[:16], launch(c, attention(c)))
+
+
+def test_visible_nan_keys_make_their_rows_nan():
+    c = make([700, 5], [16, 3], 2, 8, 64, torch.bfloat16, seed=16)
+    for at in (3, 40, 333, 699):        # columns of every kind of a tile
+        k = c["k"].clone()
+        k[int(c["indices"][at]), 1, 9] = float("nan")
+        out, lse = launch({**c, "k": k}, attention(c), return_lse=True)
+        assert bool(out[:16, 8:].isnan().all()) and bool(lse[:16, 8:].isnan().all())
+        assert bool(out[:16, :8].isfinite().all()) and bool(out[16:].isfinite().all())
 
 
 def test_results_do_not_change_from_run_to_run():
