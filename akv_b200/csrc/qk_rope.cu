@@ -18,18 +18,23 @@
 // j + D/16, which rotate within themselves.  So the rotation needs no exchange,
 // the lanes of an access are neighbours, and the norm's sum is log2(D/16)
 // shuffles.  A lane keeps its 8 cos, 8 sin and 16 weights in registers for the
-// two rows (one in fp32) that it requests before it uses the first.  Measured on
-// 16,411 tokens of 64 + 8 + 8 heads of 128, bf16 (681 MB): 142 us, 4.8 TB/s,
-// 0.73 of the copy rate, at 8 blocks of 128 threads per SM; four rows per lane
-// (102 registers, 5 blocks) 156-179 us, one row 177 us, two rows at a time
-// in a loop that keeps the table row 160 us (spills): residency counts most.
+// four rows (two in fp32) that it requests before it uses the first; the
+// arithmetic is packed (f32x2), two elements an instruction, since with scalar
+// instructions their issue was the limit (142 us at best on the first case
+// below).  Measured, bf16: 16,411 tokens of 64 + 8 + 8 heads of 128 (681 MB)
+// 127 us, 5.4 TB/s, 0.82 of the copy rate, at 12 blocks of 64 threads per SM
+// (80 registers); two rows per lane 132 us, eight 138 us, four at 16 warps per SM
+// 141 us and at 28 146 us (spills).  2,048 tokens of head_dim 64 (42.5 MB) 12.5
+// us; one token 4.4 us, the launch.
 
-#include "common.cuh"
+#include <type_traits>
+
+#include "attention_common.cuh"
 
 namespace akv {
 namespace {
 
-constexpr int kRopeThreads = 128;
+constexpr int kRopeThreads = 64;
 
 struct RopeArgs {
   const void* q;
@@ -49,7 +54,7 @@ struct RopeArgs {
   const void* q_weight;
   const void* k_weight;
   int weight_f32;
-  float eps;
+  float eps, inv_dim;
   const void* positions;
   int positions_is64;
   const void* slots;
@@ -78,10 +83,37 @@ struct Eight {
   __device__ __forceinline__ float get(int i) const {
     return Elem<T>::to_f32(v[i / Vec16<T>::N].e[i % Vec16<T>::N]);
   }
-  __device__ __forceinline__ void set(int i, float x) {
-    v[i / Vec16<T>::N].e[i % Vec16<T>::N] = Elem<T>::from_f32(x);
+  __device__ __forceinline__ void set2(int i, float x, float y) {  // elements i, i + 1
+    T* e = &v[i / Vec16<T>::N].e[i % Vec16<T>::N];
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      *reinterpret_cast<__nv_bfloat162*>(e) = __floats2bfloat162_rn(x, y);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      *reinterpret_cast<__half2*>(e) = __floats2half2_rn(x, y);
+    } else {
+      e[0] = x;
+      e[1] = y;
+    }
   }
 };
+
+// The two elements of each of a lane's eight turning pairs, in packed fp32
+// pairs of neighbours: x turns into x c - y s, y into y c + x s.
+struct Turn {
+  f32x2 x[4], y[4];
+};
+// From values (or weights) of the lane's two runs.
+template <bool NEOX>
+__device__ __forceinline__ Turn turn_of(const float (&a)[8], const float (&b)[8]) {
+  Turn t;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float* e = k < 2 ? a : b;  // adjacent pairs: 0-3 in the first run, 4-7 in the second
+    const int i = 4 * (k & 1);
+    t.x[k] = NEOX ? f2_pack(a[2 * k], a[2 * k + 1]) : f2_pack(e[i], e[i + 2]);
+    t.y[k] = NEOX ? f2_pack(b[2 * k], b[2 * k + 1]) : f2_pack(e[i + 1], e[i + 3]);
+  }
+  return t;
+}
 
 template <typename T>
 __device__ __forceinline__ void load8(const void* base, long long at, float (&out)[8]) {
@@ -114,9 +146,10 @@ __device__ __forceinline__ void load_turn(const void* base, long long a, long lo
 }
 
 // T: element type; LANES: lanes per row (D / 16 rounded up to a power of
-// two); NEOX: halves or adjacent pairs; ROWS: rows per lane group.
-template <typename T, int LANES, bool NEOX, int ROWS>
-__global__ void __launch_bounds__(kRopeThreads, 8) qk_norm_rope_kernel(const RopeArgs a) {
+// two); NEOX: halves or adjacent pairs; FULL: D is 16 LANES, so that every lane
+// has two runs; ROWS: rows per lane group.
+template <typename T, int LANES, bool NEOX, bool FULL, int ROWS>
+__global__ void __launch_bounds__(kRopeThreads, 12) qk_norm_rope_kernel(const RopeArgs a) {
   const uint32_t group = blockIdx.x * (kRopeThreads / LANES) + threadIdx.x / LANES;
   const int j = threadIdx.x % LANES;
   const uint32_t token32 = group / (uint32_t)a.units;
@@ -139,7 +172,8 @@ __global__ void __launch_bounds__(kRopeThreads, 8) qk_norm_rope_kernel(const Rop
   const bool turned1 = NEOX ? turned : 8 * (j + LANES) < a.rotary;
   const int e0 = NEOX && t >= 0 ? a.rotary + 8 * t : 8 * j;
   const int e1 = !NEOX ? 8 * (j + LANES) : t >= 0 ? (a.rotary + a.dim) / 2 + 8 * t : half + 8 * j;
-  const bool live = NEOX ? 16 * j < a.dim : 8 * j < a.dim, live1 = NEOX ? live : e1 < a.dim;
+  const bool live = FULL || (NEOX ? 16 * j < a.dim : 8 * j < a.dim);
+  const bool live1 = FULL || (NEOX ? live : e1 < a.dim);
 
   const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v);
   const long long st = kind == 0 ? a.q_st : kind == 1 ? a.k_st : a.v_st;
@@ -199,8 +233,16 @@ __global__ void __launch_bounds__(kRopeThreads, 8) qk_norm_rope_kernel(const Rop
     }
   }
   const void* weight = kind == 0 ? a.q_weight : a.k_weight;
-  float w0[8], w1[8];
+  f32x2 c2[4], s2[4], n2[4];  // cos, sin, -sin
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    c2[k] = f2_pack(c[2 * k], c[2 * k + 1]);
+    s2[k] = f2_pack(s[2 * k], s[2 * k + 1]);
+    n2[k] = f2_pack(-s[2 * k], -s[2 * k + 1]);
+  }
+  Turn w;
   if (weight != nullptr) {
+    float w0[8] = {}, w1[8] = {};
     if (a.weight_f32) {
       if (live) load8<float>(weight, e0, w0);
       if (live1) load8<float>(weight, e1, w1);
@@ -208,6 +250,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) qk_norm_rope_kernel(const Rop
       if (live) load8<T>(weight, e0, w0);
       if (live1) load8<T>(weight, e1, w1);
     }
+    w = turn_of<NEOX>(w0, w1);
   }
 
   T* out = static_cast<T*>(kind == 0 ? a.q_out : a.k_out);
@@ -226,29 +269,39 @@ __global__ void __launch_bounds__(kRopeThreads, 8) qk_norm_rope_kernel(const Rop
       y0[i] = live ? x0[r].get(i) : 0.f;
       y1[i] = live1 ? x1[r].get(i) : 0.f;
     }
+    Turn v = turn_of<NEOX>(y0, y1);
     if (weight != nullptr) {
-      float ss = 0.f;
+      f32x2 sx = f2_pack(0.f, 0.f), sy = sx;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += y0[i] * y0[i] + y1[i] * y1[i];
+      for (int k = 0; k < 4; ++k) {
+        sx = f2_fma(v.x[k], v.x[k], sx);
+        sy = f2_fma(v.y[k], v.y[k], sy);
+      }
+      float a0, a1;
+      f2_unpack(f2_add(sx, sy), a0, a1);
+      float ss = a0 + a1;
 #pragma unroll
       for (int d = LANES / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(lanes, ss, d);
-      const float inv = rsqrtf(ss / (float)a.dim + a.eps);
+      const float inv = rsqrtf(ss * a.inv_dim + a.eps);
+      const f32x2 inv2 = f2_pack(inv, inv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (live) y0[i] *= inv * w0[i];
-        if (live1) y1[i] *= inv * w1[i];
+      for (int k = 0; k < 4; ++k) {
+        v.x[k] = f2_mul(v.x[k], f2_mul(w.x[k], inv2));
+        v.y[k] = f2_mul(v.y[k], f2_mul(w.y[k], inv2));
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int k = 0; k < 4; ++k) {
+      float p0, p1, q0, q1;
+      f2_unpack(f2_fma(v.x[k], c2[k], f2_mul(v.y[k], n2[k])), p0, p1);
+      f2_unpack(f2_fma(v.y[k], c2[k], f2_mul(v.x[k], s2[k])), q0, q1);
       if (NEOX) {
-        x0[r].set(i, y0[i] * c[i] - y1[i] * s[i]);
-        x1[r].set(i, y1[i] * c[i] + y0[i] * s[i]);
-      } else if (i < 4) {
-        x0[r].set(2 * i, y0[2 * i] * c[i] - y0[2 * i + 1] * s[i]);
-        x0[r].set(2 * i + 1, y0[2 * i + 1] * c[i] + y0[2 * i] * s[i]);
-        x1[r].set(2 * i, y1[2 * i] * c[4 + i] - y1[2 * i + 1] * s[4 + i]);
-        x1[r].set(2 * i + 1, y1[2 * i + 1] * c[4 + i] + y1[2 * i] * s[4 + i]);
+        x0[r].set2(2 * k, p0, p1);
+        x1[r].set2(2 * k, q0, q1);
+      } else {
+        Eight<T>& run = k < 2 ? x0[r] : x1[r];
+        run.set2(4 * (k & 1), p0, q0);
+        run.set2(4 * (k & 1) + 2, p1, q1);
       }
     }
     if (out != nullptr) {
@@ -262,22 +315,28 @@ __global__ void __launch_bounds__(kRopeThreads, 8) qk_norm_rope_kernel(const Rop
   }
 }
 
-template <typename T, int LANES, bool NEOX>
+template <typename T, int LANES, bool NEOX, bool FULL>
 int launch_rope(RopeArgs& a, cudaStream_t stream) {
-  constexpr int ROWS = sizeof(T) == 4 ? 1 : 2;
+  constexpr int ROWS = sizeof(T) == 4 ? 2 : 4;
   a.q_units = (a.hq + ROWS - 1) / ROWS;
   a.k_units = (a.hkv + ROWS - 1) / ROWS;
   a.units = a.q_units + a.k_units * (a.v != nullptr ? 2 : 1);
   const long long groups = a.tokens * a.units, per = kRopeThreads / LANES;
   const long long blocks = (groups + per - 1) / per;
   if (groups + per > UINT32_MAX) return AKV_ERR_INVALID;  // 32-bit group numbers
-  qk_norm_rope_kernel<T, LANES, NEOX, ROWS><<<(unsigned)blocks, kRopeThreads, 0, stream>>>(a);
+  qk_norm_rope_kernel<T, LANES, NEOX, FULL, ROWS>
+      <<<(unsigned)blocks, kRopeThreads, 0, stream>>>(a);
   return launch_status();
 }
 
 template <typename T, int LANES>
 int launch_rope_style(RopeArgs& a, int neox, cudaStream_t stream) {
-  return neox ? launch_rope<T, LANES, true>(a, stream) : launch_rope<T, LANES, false>(a, stream);
+  const bool full = a.dim == 16 * LANES;
+  if (neox)
+    return full ? launch_rope<T, LANES, true, true>(a, stream)
+                : launch_rope<T, LANES, true, false>(a, stream);
+  return full ? launch_rope<T, LANES, false, true>(a, stream)
+              : launch_rope<T, LANES, false, false>(a, stream);
 }
 
 template <typename T>
@@ -331,7 +390,7 @@ extern "C" int akv_qk_norm_rope(const akv_qk_norm_rope_args* args, void* stream)
              x.q_out_stride_head, x.k_out, x.k_out_stride_token, x.k_out_stride_head, x.k_pool,
              x.k_pool_stride_slot, x.k_pool_stride_head, x.v_pool, x.v_pool_stride_slot,
              x.v_pool_stride_head, x.q_weight, x.k_weight, x.weight_dtype == AKV_F32,
-             (float)x.eps, x.positions, x.positions_is64 != 0, x.slots, x.slots_is64 != 0,
+             (float)x.eps, 1.f / (float)x.head_dim, x.positions, x.positions_is64 != 0, x.slots, x.slots_is64 != 0,
              x.cos_sin_cache, (int)x.cache_dtype, x.cache_stride, x.max_position, x.num_slots,
              x.tokens, (int)x.num_q_heads, (int)x.num_kv_heads, (int)x.head_dim,
              (int)x.rotary_dim, 0, 0, 0, x.error_flag};
