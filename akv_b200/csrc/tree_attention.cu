@@ -78,16 +78,6 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Key tiles of an item: none if it reaches past the call's vectors, as one of
-// a plan made after the call was captured may.
-__device__ __forceinline__ int item_tiles(const TreeParams& p, const TreeItem& w) {
-  if ((long long)w.q0 + w.n > p.tokens || (long long)w.kv0 + w.prefix > p.keys) {
-    if (p.error_flag) atomicOr(p.error_flag, 4);
-    return 0;
-  }
-  return (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
-}
-
 // Slot of key j of an item; -1: a padding token, read as zeros.
 __device__ __forceinline__ long long key_slot(const TreeParams& p, const TreeItem& w, int j) {
   const bool cached = j < w.prefix;
@@ -358,11 +348,20 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     *abort = base & 1023 ? 1 : 0;  // the swizzled tiles need a 1024-byte aligned base
     *scrubbed = 0;
   }
+  // A CTA with an item that reaches past the call's vectors, as one of a plan
+  // made after the call was captured may, does nothing.
+  const int it0 = p.cta_items[blockIdx.x], items_end = p.cta_items[blockIdx.x + 1];
+  bool past = false;
+  for (int it = it0 + tid; it < items_end; it += C::kThreads) {
+    const TreeItem w = p.items[it];
+    past |= (long long)w.q0 + w.n > p.tokens || (long long)w.kv0 + w.prefix > p.keys;
+  }
   tc_fence_before();
-  __syncthreads();
+  past = __syncthreads_or(past);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int it0 = p.cta_items[blockIdx.x], it1 = p.cta_items[blockIdx.x + 1];
+  const int it1 = past ? it0 : items_end;
+  if (past && tid == 0 && p.error_flag) atomicOr(p.error_flag, 4);
 
   if (warp >= C::kSoftmax + C::kProducers) {
     // ---- MMA issuers: one thread per unit ----
@@ -375,7 +374,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
       bool ok = true;
       for (int it = it0; it < it1 && ok; ++it) {
         const TreeItem w = p.items[it];
-        const int n_tiles = item_tiles(p, w);
+        const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
         const bool pair = w.units == 2;
         const int step = pair ? 1 : 2;
         const int n = pair ? n_tiles : (n_tiles - u + 1) / 2;  // this unit's tiles
@@ -449,7 +448,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     bool ok = true;
     for (int it = it0; it < it1 && ok; ++it) {
       const TreeItem w = p.items[it];
-      const int n_tiles = item_tiles(p, w);
+      const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
       const int heads = w.head_step ? 2 : 1;
       auto fetch = [&](int t) {
         const int j = w.lo + t * kTreeKeys + kKpw * pw + lane % kKpw;
@@ -537,7 +536,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         const TreeItem w = p.items[it];
         const int row = (w.tile0 + u * w.tile_step) * kTreeRows + r;
         const int i = row / p.group, h = (w.head0 + u * w.head_step) * p.group + row - i * p.group;
-        if (i < w.n && item_tiles(p, w) > 0) {
+        if (i < w.n) {
           const T* src = static_cast<const T*>(p.q) + (long long)(w.q0 + i) * p.q_st +
                          (long long)h * p.q_sh;
 #pragma unroll
@@ -550,14 +549,14 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     load_q(it0);
     for (int it = it0; it < it1; ++it) {
       const TreeItem w = p.items[it];
-      const int n_tiles = item_tiles(p, w);
+      const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
       const bool pair = w.units == 2;
       const int n = pair ? n_tiles : (n_tiles - u + 1) / 2;
       const int head = w.head0 + u * w.head_step;
       const int row0 = (w.tile0 + u * w.tile_step) * kTreeRows;
       const int i = (row0 + r) / p.group, h = head * p.group + (row0 + r) - i * p.group;
-      const bool live = i < w.n && n_tiles > 0;
-      const bool warp_live = n_tiles > 0 && row0 + (warp & 3) * 32 < w.n * p.group;
+      const bool live = i < w.n;
+      const bool warp_live = row0 + (warp & 3) * 32 < w.n * p.group;
       const unsigned long long mask = live ? row_mask(p, w, i) : 0;
       const int pos = live && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
       cp_async_wait<0>();

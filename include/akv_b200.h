@@ -840,8 +840,8 @@ int akv_qk_norm_rope(const akv_qk_norm_rope_args* args, void* stream);
  * akv_b200/context_tree.py builds all of them.
  *
  * tokens and keys are the lengths of the token vectors (q, out, draft_slots,
- * tree_mask, q_positions) and key vectors (kv_indices, kv_positions); an item
- * that reaches past them is left out.  error_flag: DEVICE int32 or NULL,
+ * tree_mask, q_positions) and key vectors (kv_indices, kv_positions); a CTA
+ * with an item that reaches past them does nothing.  error_flag: DEVICE int32 or NULL,
  * collects 1 (a slot outside the pools, read as slot 0), 2 (a wait ran out: the
  * launch's output is invalid) and 4 (an item past tokens or keys).
  */
