@@ -548,138 +548,146 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     };
     load_q(it0);
     for (int it = it0; it < it1; ++it) {
-      const TreeItem w = p.items[it];
-      const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
-      const bool pair = w.units == 2;
-      const int n = pair ? n_tiles : (n_tiles - u + 1) / 2;
-      const int head = w.head0 + u * w.head_step;
-      const int row0 = (w.tile0 + u * w.tile_step) * kTreeRows;
-      const int i = (row0 + r) / p.group, h = head * p.group + (row0 + r) - i * p.group;
-      const bool live = i < w.n;
-      const bool warp_live = row0 + (warp & 3) * 32 < w.n * p.group;
-      const unsigned long long mask = live ? row_mask(p, w, i) : 0;
-      const int pos = live && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
-      cp_async_wait<0>();
-      if (n > 0) {
-        fence_async_smem();
-        mbar_arrive(bar_q(u));
-      } else {
-        load_q(it + 1);
-      }
       float m = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int v = 0; v < n && ok; ++v) {
-        const uint32_t c = cnt + v;
-        const int j0 = w.lo + (pair ? v : 2 * v + u) * kTreeKeys;
-        ok = warp_wait(bar_s(u), c & 1, abort);
-        if (!ok) break;
-        if (v == n - 1) load_q(it + 1);
-        if (warp_live) {
-          tc_fence_after();
-          if (p.window >= 0 || j0 + kTreeKeys > w.prefix) {
-            // Hidden keys get a score of -inf in tensor memory, so that the
-            // ordinary path below has no mask (and no registers for one).
-#pragma unroll 1
-            for (int b = 0; b < kTreeKeys; b += 64) {
-              const unsigned long long seen = seen64(p, w, mask, i, pos, j0 + b, lane);
-              if (__all_sync(0xffffffffu, seen == ~0ull)) continue;
-#pragma unroll 1
-              for (int q = 0; q < 64; q += 32) {
-                const uint32_t bits = (uint32_t)(seen >> q);
-                float x[32];
-                tmem_ld32_sync(tu + b + q, x);
-                uint32_t y[32];
-#pragma unroll
-                for (int k = 0; k < 32; ++k)
-                  y[k] = __float_as_uint(bits >> k & 1 ? x[k] : -INFINITY);
-                tmem_st32_sync(tu + b + q, y);
-              }
-            }
-          }
-          // The scores are read twice, for the maximum and for P: more than
-          // 64 of them in registers cost spills.
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int b = 0; b < kTreeKeys; b += 64) {
-            float s[64];
-            tmem_ld64_sync(tu + b, s);
-#pragma unroll
-            for (int k = 0; k < 64; k += 2)
-              m4[k >> 1 & 3] = max3_nan(m4[k >> 1 & 3], s[k], s[k + 1]);
-          }
-          const float bm =
-              max3_nan(max3_nan(m4[0], m4[1], m4[2]), m4[3], -INFINITY) * p.scale_log2;
-          // The base only moves when the tile exceeds it by 2^8; then l and
-          // O are rescaled.
-          float alpha = 1.f;
-          bool rescale = false;
-          if (bm > m + kStaleMax || (m == -INFINITY && bm != -INFINITY)) {
-            rescale = m != -INFINITY;
-            alpha = rescale ? fast_exp2(m - bm) : 0.f;
-            m = bm;
-          }
-          const float nb = m == -INFINITY ? 0.f : -m;
-          const f32x2 scale2 = f2_pack(p.scale_log2, p.scale_log2), nb2 = f2_pack(nb, nb);
-          f32x2 sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-          // The last columns come first: P overwrites the second half of its
-          // scores at head_dim 128, each piece of it columns that are read.
-#pragma unroll
-          for (int b = kTreeKeys - 32; b >= 0; b -= 32) {
-            float s[32];
-            tmem_ld32_sync(tu + b, s);
-            if (kFree && b == 0) {  // every score of the tile is read
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar_f(u));
-            }
-            uint32_t pk[16];
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              float x0, x1;
-              const f32x2 x = f2_fma(f2_pack(s[k], s[k + 1]), scale2, nb2);
-              if (kPoly >> (k / 2) & 1) {
-                exp2_pair(x, x0, x1);
-              } else {
-                f2_unpack(x, x0, x1);
-                x0 = fast_exp2(x0);
-                x1 = fast_exp2(x1);
-              }
-              sum[k >> 1 & 1] = f2_add(sum[k >> 1 & 1], f2_pack(x0, x1));
-              pk[k / 2] = pack2<T>(x0, x1);
-            }
-            // P's columns, and O's, are free once the product before is done
-            // (with P over the scores S(c) came after it).
-            if (b == kTreeKeys - 32 && kFree && c > 0) ok = warp_wait(bar_o(u), c - 1 & 1, abort);
-            tmem_st16_async(tu + C::kColP + b / 2, pk);
-          }
-          tmem_st_wait();
-          float l0, l1;
-          f2_unpack(f2_add(sum[0], sum[1]), l0, l1);
-          l = l * alpha + (l0 + l1);
-          if (!(bm < INFINITY)) l = NAN;  // an infinite or NaN score: the row is NaN
-          if (__any_sync(0xffffffffu, rescale)) {
-            tc_fence_after();
-#pragma unroll
-            for (int d = 0; d < D; d += 32) {
-              float o[32];
-              tmem_ld32_sync(tu + C::kColO + d, o);
-              uint32_t z[32];
-#pragma unroll
-              for (int k = 0; k < 32; ++k) z[k] = __float_as_uint(o[k] * alpha);
-              tmem_st32_sync(tu + C::kColO + d, z);
-            }
-          }
-          tc_fence_before();
-        } else if (kFree) {
-          // A warp without rows keeps the others' pace: with S(c + 1) made
-          // early it would otherwise arrive on p twice before they do once.
-          if (lane == 0) mbar_arrive(bar_f(u));
-          if (c > 0) ok = warp_wait(bar_o(u), c - 1 & 1, abort);
+      bool ok = true, warp_live;
+      int n;  // this unit's tiles
+      {
+        const TreeItem w = p.items[it];
+        const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
+        const bool pair = w.units == 2;
+        n = pair ? n_tiles : (n_tiles - u + 1) / 2;
+        const int row0 = (w.tile0 + u * w.tile_step) * kTreeRows, i = (row0 + r) / p.group;
+        warp_live = row0 + (warp & 3) * 32 < w.n * p.group;
+        const unsigned long long mask = i < w.n ? row_mask(p, w, i) : 0;
+        const int pos = i < w.n && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
+        cp_async_wait<0>();
+        if (n > 0) {
+          fence_async_smem();
+          mbar_arrive(bar_q(u));
+        } else {
+          load_q(it + 1);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p(u));
+        for (int v = 0; v < n && ok; ++v) {
+          const uint32_t c = cnt + v;
+          const int j0 = w.lo + (pair ? v : 2 * v + u) * kTreeKeys;
+          ok = warp_wait(bar_s(u), c & 1, abort);
+          if (!ok) break;
+          if (v == n - 1) load_q(it + 1);
+          if (warp_live) {
+            tc_fence_after();
+            if (p.window >= 0 || j0 + kTreeKeys > w.prefix) {
+              // Hidden keys get a score of -inf in tensor memory, so that the
+              // ordinary path below has no mask (and no registers for one).
+#pragma unroll 1
+              for (int b = 0; b < kTreeKeys; b += 64) {
+                const unsigned long long seen = seen64(p, w, mask, i, pos, j0 + b, lane);
+                if (__all_sync(0xffffffffu, seen == ~0ull)) continue;
+#pragma unroll 1
+                for (int q = 0; q < 64; q += 32) {
+                  const uint32_t bits = (uint32_t)(seen >> q);
+                  float x[32];
+                  tmem_ld32_sync(tu + b + q, x);
+                  uint32_t y[32];
+#pragma unroll
+                  for (int k = 0; k < 32; ++k)
+                    y[k] = __float_as_uint(bits >> k & 1 ? x[k] : -INFINITY);
+                  tmem_st32_sync(tu + b + q, y);
+                }
+              }
+            }
+            // The scores are read twice, for the maximum and for P: more than
+            // 64 of them in registers cost spills.
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int b = 0; b < kTreeKeys; b += 64) {
+              float s[64];
+              tmem_ld64_sync(tu + b, s);
+#pragma unroll
+              for (int k = 0; k < 64; k += 2)
+                m4[k >> 1 & 3] = max3_nan(m4[k >> 1 & 3], s[k], s[k + 1]);
+            }
+            const float bm =
+                max3_nan(max3_nan(m4[0], m4[1], m4[2]), m4[3], -INFINITY) * p.scale_log2;
+            // The base only moves when the tile exceeds it by 2^8; then l and
+            // O are rescaled.
+            float alpha = 1.f;
+            bool rescale = false;
+            if (bm > m + kStaleMax || (m == -INFINITY && bm != -INFINITY)) {
+              rescale = m != -INFINITY;
+              alpha = rescale ? fast_exp2(m - bm) : 0.f;
+              m = bm;
+            }
+            const float nb = m == -INFINITY ? 0.f : -m;
+            const f32x2 scale2 = f2_pack(p.scale_log2, p.scale_log2), nb2 = f2_pack(nb, nb);
+            f32x2 sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+            // The last columns come first: P overwrites the second half of its
+            // scores at head_dim 128, each piece of it columns that are read.
+#pragma unroll
+            for (int b = kTreeKeys - 32; b >= 0; b -= 32) {
+              float s[32];
+              tmem_ld32_sync(tu + b, s);
+              if (kFree && b == 0) {  // every score of the tile is read
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_f(u));
+              }
+              uint32_t pk[16];
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                float x0, x1;
+                const f32x2 x = f2_fma(f2_pack(s[k], s[k + 1]), scale2, nb2);
+                if (kPoly >> (k / 2) & 1) {
+                  exp2_pair(x, x0, x1);
+                } else {
+                  f2_unpack(x, x0, x1);
+                  x0 = fast_exp2(x0);
+                  x1 = fast_exp2(x1);
+                }
+                sum[k >> 1 & 1] = f2_add(sum[k >> 1 & 1], f2_pack(x0, x1));
+                pk[k / 2] = pack2<T>(x0, x1);
+              }
+              // P's columns, and O's, are free once the product before is done
+              // (with P over the scores S(c) came after it).
+              if (b == kTreeKeys - 32 && kFree && c > 0) ok = warp_wait(bar_o(u), c - 1 & 1, abort);
+              tmem_st16_async(tu + C::kColP + b / 2, pk);
+            }
+            tmem_st_wait();
+            float l0, l1;
+            f2_unpack(f2_add(sum[0], sum[1]), l0, l1);
+            l = l * alpha + (l0 + l1);
+            if (!(bm < INFINITY)) l = NAN;  // an infinite or NaN score: the row is NaN
+            if (__any_sync(0xffffffffu, rescale)) {
+              tc_fence_after();
+#pragma unroll
+              for (int d = 0; d < D; d += 32) {
+                float o[32];
+                tmem_ld32_sync(tu + C::kColO + d, o);
+                uint32_t z[32];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) z[k] = __float_as_uint(o[k] * alpha);
+                tmem_st32_sync(tu + C::kColO + d, z);
+              }
+            }
+            tc_fence_before();
+          } else if (kFree) {
+            // A warp without rows keeps the others' pace: with S(c + 1) made
+            // early it would otherwise arrive on p twice before they do once.
+            if (lane == 0) mbar_arrive(bar_f(u));
+            if (c > 0) ok = warp_wait(bar_o(u), c - 1 & 1, abort);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_p(u));
+        }
       }
       if (!ok) break;
+      // The item is read, and the row worked out, again: over the tiles they
+      // would only hold registers.
+      const TreeItem w = p.items[it];
+      const bool pair = w.units == 2;
+      const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
+      const int row = (w.tile0 + u * w.tile_step) * kTreeRows + r, i = row / p.group;
+      const int head = w.head0 + u * w.head_step, h = head * p.group + row - i * p.group;
+      const bool live = i < w.n;
       cnt += n;
       if (n > 0 && !warp_wait(bar_o(u), cnt - 1 & 1, abort)) break;
       tc_fence_after();
@@ -736,8 +744,8 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
           }
         }
         if (live && *scrubbed)
-          restore<T>(p, w, mask, pos, head, direct ? dst : nullptr,
-                     direct ? nullptr : acc, d0, d1);
+          restore<T>(p, w, row_mask(p, w, i), p.window >= 0 ? p.q_positions[w.q0 + i] : 0, head,
+                     direct ? dst : nullptr, direct ? nullptr : acc, d0, d1);
         if (live && (pair || u == 0)) {
           if (!direct) {
             reinterpret_cast<float2*>(p.part_ml)[part * kTreeRows + r] = make_float2(m, l);
