@@ -187,6 +187,15 @@ def _load():
 
 
 lib = _load()
+try:
+    from . import _tensor_fields
+    from ._tensor_fields import fields  # noqa: F401  (address, device, type, sizes, strides)
+except ImportError as e:
+    raise ImportError(f"akv_b200._tensor_fields is not built; run `python -m akv_b200.build` ({e})")
+INT32, INT64 = _tensor_fields.INT32, _tensor_fields.INT64
+# fields()' type codes -> AKV_* element types
+FIELD_CODE = {_tensor_fields.F16: AKV_F16, _tensor_fields.BF16: AKV_BF16,
+              _tensor_fields.F32: AKV_F32}
 
 
 def ptr(t):

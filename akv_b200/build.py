@@ -4,7 +4,8 @@
 
 Compiles every ``csrc/*.cu`` with nvcc for ``sm_100a`` only and links them
 into ``akv_b200/libakv_b200.so`` in the source tree, so the built library
-travels with the tree.  ``-Xptxas -v`` output (registers, spills, shared
+travels with the tree; ``csrc/tensor_fields.cpp`` becomes the CPython module
+``_tensor_fields`` beside it (g++, torch's headers).  ``-Xptxas -v`` output (registers, spills, shared
 memory) is written to ``akv_b200/_build/ptxas.txt``.
 """
 
@@ -13,6 +14,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -20,6 +22,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libakv_b200.so")
+FIELDS = os.path.join(PKG, "_tensor_fields.so")  # CPython module: a tensor's fields in one call
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -36,6 +39,23 @@ def _stale(target, deps):
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def build_fields(force: bool = False) -> str:
+    import torch
+
+    src = os.path.join(CSRC, "tensor_fields.cpp")
+    if force or _stale(FIELDS, [src]):
+        t = os.path.dirname(torch.__file__)
+        lib = os.path.join(t, "lib")
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               "-I", os.path.join(t, "include"),
+               "-I", os.path.join(t, "include", "torch", "csrc", "api", "include"),
+               "-I", sysconfig.get_paths()["include"], src, "-o", FIELDS,
+               "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10"]
+        subprocess.run(cmd, check=True)
+    return FIELDS
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -61,6 +81,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force or _stale(LIB, objects):
         cmd = [NVCC, *ARCH, "-shared", "-o", LIB, *objects, "-lcudart"]
         subprocess.run(cmd, check=True)
+    build_fields(force)
     return LIB
 
 

@@ -18,17 +18,18 @@ import torch
 
 from . import _native
 
-_NONE = (0, 0, 0)
+_fields, _INT32, _INT64, _CODE = _native.fields, _native.INT32, _native.INT64, _native.FIELD_CODE
+_WHAT = ("must be [tokens, heads, head_dim] of the type and device of q, with unit last stride "
+         "(k, v and the outputs with its tokens and head_dim)")
 
 
-def _heads(name, t, dtype, index, shape):
-    """(address, stride of the first dimension, of the second)."""
-    s = t.stride()
-    if t.dtype != dtype or t.get_device() != index or len(s) != 3 or s[2] != 1 or \
-            (shape is not None and t.shape != shape):
-        raise ValueError(f"{name} must be [tokens, heads, head_dim] of the type and device of q, "
-                         "with unit last stride")
-    return t.data_ptr(), s[0], s[1]
+def _vector(name, t, n, index):
+    """(address, 1 if int64) of a contiguous index vector of n entries."""
+    ptr, dev, dt, size, step = _fields(1, t)
+    if size != n or dev != index or (step != 1 and n > 1) or (dt != _INT32 and dt != _INT64):
+        raise ValueError(f"{name} must be a contiguous int32 or int64 vector of one entry per "
+                         "token on the device of q")
+    return ptr, 1 if dt == _INT64 else 0
 
 
 def qk_norm_rope(q, k, positions, cos_sin_cache, *, q_weight=None, k_weight=None, eps=1e-6,
@@ -56,78 +57,74 @@ def qk_norm_rope(q, k, positions, cos_sin_cache, *, q_weight=None, k_weight=None
     A slot past the pools, or a position outside the table (rotated as
     position 0), is not stored and sets ``error_flag`` (int32 [1]) if given.
     """
-    index = q.get_device()
+    (q_ptr, index, dt, tokens, hq, d, q0, q1, unit, k_ptr, dev, k_dt, n, hkv, k_dim, k0, k1,
+     k_unit) = _fields(3, q, k)
     if index < 0:
         raise ValueError("qk_norm_rope runs on CUDA tensors")
-    dtype = q.dtype
-    code = _native.DTYPE_CODE.get(dtype)
+    code = _CODE.get(dt)
     if code is None:
         raise ValueError("qk_norm_rope runs on fp16, bf16 or fp32")
-    qa = _heads("q", q, dtype, index, None)
-    tokens, hq, d = q.shape
-    ka = _heads("k", k, dtype, index, None)
-    k_tokens, hkv, k_dim = k.shape
-    if k_tokens != tokens or k_dim != d:
-        raise ValueError("k must have q's tokens and head_dim")
-    if cos_sin_cache.ndim != 2 or cos_sin_cache.get_device() != index:
-        raise ValueError("cos_sin_cache must be [max_position, rotary_dim] on the device of q")
-    max_position, width = cos_sin_cache.shape
-    cache_stride, unit = cos_sin_cache.stride()
+    if unit != 1 or k_unit != 1 or dev != index or k_dt != dt or n != tokens or k_dim != d:
+        raise ValueError("q and k " + _WHAT)
+    table, dev, table_dt, max_position, width, cache_stride, unit = _fields(2, cos_sin_cache)
     rotary = width if rotary_dim is None else rotary_dim
-    cache_code = _native.DTYPE_CODE.get(cos_sin_cache.dtype)
-    if cache_code is None or rotary != width or unit != 1:
-        raise ValueError("cos_sin_cache must be floating point and rotary_dim wide")
+    cache_code = _CODE.get(table_dt)
+    if cache_code is None or rotary != width or unit != 1 or dev != index:
+        raise ValueError("cos_sin_cache must be floating point [max_position, rotary_dim] on the "
+                         "device of q")
     if d % 16 or d > 512 or rotary % 16 or not 0 < rotary <= d:
         raise ValueError("head_dim and rotary_dim must be multiples of 16, at most 512")
-    if positions.shape != (tokens,) or positions.get_device() != index or \
-            not positions.is_contiguous():
-        raise ValueError("positions must be a contiguous vector of one entry per token")
-    weight_code = code
-    for w in (q_weight, k_weight):
+    pos_ptr, pos64 = _vector("positions", positions, tokens, index)
+    weight_dt, weights = -1, [0, 0]
+    for side, w in enumerate((q_weight, k_weight)):
         if w is None:
             continue
-        if w.shape != (d,) or w.stride(0) != 1 or w.get_device() != index or \
-                w.dtype not in (dtype, torch.float32):
+        weights[side], dev, w_dt, n, unit = _fields(1, w)
+        if n != d or unit != 1 or dev != index or (w_dt != dt and _CODE.get(w_dt) != _native.AKV_F32):
             raise ValueError("norm weights must be [head_dim] of q's type or fp32")
-        weight_code = _native.DTYPE_CODE[w.dtype]
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError("norm weights must have one type")
+        if weight_dt not in (-1, w_dt):
+            raise ValueError("norm weights must have one type")
+        weight_dt = w_dt
     if q_out is None:
         q_out = torch.empty_like(q)
-    qo = _heads("q_out", q_out, dtype, index, q.shape)
-    va = kp = vp = _NONE
-    num_slots = slots_ptr = slots64 = 0
+    num_slots = slots_ptr = slots64 = v_ptr = v0 = v1 = 0
+    kp_ptr = kp0 = kp1 = vp_ptr = vp0 = vp1 = ko_ptr = ko0 = ko1 = 0
     if k_pool is not None:
         if v is None or v_pool is None or slots is None:
             raise ValueError("a store needs v, k_pool, v_pool and slots")
-        va = _heads("v", v, dtype, index, k.shape)
-        kp = _heads("k_pool", k_pool, dtype, index, None)
-        vp = _heads("v_pool", v_pool, dtype, index, None)
-        k_shape, v_shape = k_pool.shape, v_pool.shape
-        if k_shape[1:] != (hkv, d) or v_shape[1:] != (hkv, d):
-            raise ValueError("KV pools must be [slots, num_kv_heads, head_dim]")
-        num_slots = min(k_shape[0], v_shape[0])
-        if slots.shape != (tokens,) or slots.get_device() != index or not slots.is_contiguous():
-            raise ValueError("slots must be a contiguous vector of one entry per token")
-        slots_ptr, slots64 = slots.data_ptr(), _native.is64(slots)
+        (v_ptr, dev, v_dt, n, heads, dim, v0, v1, unit, kp_ptr, kp_dev, kp_dt, k_slots, kp_heads,
+         kp_dim, kp0, kp1, kp_unit, vp_ptr, vp_dev, vp_dt, v_slots, vp_heads, vp_dim, vp0, vp1,
+         vp_unit) = _fields(3, v, k_pool, v_pool)
+        if n != tokens or heads != hkv or dim != d or unit != 1 or dev != index or v_dt != dt:
+            raise ValueError("v " + _WHAT)
+        if kp_heads != hkv or vp_heads != hkv or kp_dim != d or vp_dim != d or kp_unit != 1 or \
+                vp_unit != 1 or kp_dev != index or vp_dev != index or kp_dt != dt or vp_dt != dt:
+            raise ValueError("KV pools must be [slots, num_kv_heads, head_dim] of the type and "
+                             "device of q, with unit last stride")
+        num_slots = k_slots if k_slots < v_slots else v_slots
+        slots_ptr, slots64 = _vector("slots", slots, tokens, index)
     elif v is not None or v_pool is not None or slots is not None:
         raise ValueError("a store needs v, k_pool, v_pool and slots")
     elif k_out is None:
         k_out = torch.empty_like(k)
-    ko = _NONE if k_out is None else _heads("k_out", k_out, dtype, index, k.shape)
+    qo_ptr, dev, out_dt, n, heads, dim, qo0, qo1, unit = _fields(3, q_out)
+    if n != tokens or heads != hq or dim != d or unit != 1 or dev != index or out_dt != dt:
+        raise ValueError("q_out " + _WHAT)
+    if k_out is not None:
+        ko_ptr, dev, out_dt, n, heads, dim, ko0, ko1, unit = _fields(3, k_out)
+        if n != tokens or heads != hkv or dim != d or unit != 1 or dev != index or out_dt != dt:
+            raise ValueError("k_out " + _WHAT)
     flag = 0
     if error_flag is not None:
         if error_flag.get_device() != index or error_flag.dtype != torch.int32:
             raise ValueError("error_flag must be an int32 tensor on the device of q")
         flag = error_flag.data_ptr()
-    positions64 = _native.is64(positions)
     if tokens == 0:
         return q_out, k_out
     status = _native.launch(index, _native.lib.akv_qk_norm_rope, _native.QK_NORM_ROPE.pack(
-        *qa, *ka, *va, code, tokens, hq, hkv, d, rotary, 1 if is_neox_style else 0,
-        0 if q_weight is None else q_weight.data_ptr(),
-        0 if k_weight is None else k_weight.data_ptr(), weight_code, eps, positions.data_ptr(),
-        positions64, cos_sin_cache.data_ptr(), cache_code, cache_stride, max_position, *qo, *ko,
-        *kp, *vp, num_slots, slots_ptr, slots64, flag))
+        q_ptr, q0, q1, k_ptr, k0, k1, v_ptr, v0, v1, code, tokens, hq, hkv, d, rotary,
+        1 if is_neox_style else 0, weights[0], weights[1], _CODE.get(weight_dt, code), eps, pos_ptr,
+        pos64, table, cache_code, cache_stride, max_position, qo_ptr, qo0, qo1, ko_ptr, ko0, ko1,
+        kp_ptr, kp0, kp1, vp_ptr, vp0, vp1, num_slots, slots_ptr, slots64, flag))
     _native.check(status, "qk_norm_rope")
     return q_out, k_out

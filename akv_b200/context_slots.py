@@ -55,12 +55,7 @@ class SlotMap:
             raise RuntimeError(f"slot map: {why}")
 
 
-def _vector(name, t, n, index):
-    """1 for an int64 vector of n entries on the device, 0 for int32."""
-    if t.shape != (n,) or not t.is_contiguous() or t.get_device() != index:
-        raise ValueError(f"{name} must be a contiguous vector of one entry per request, on the "
-                         "mapper's device")
-    return _native.is64(t)
+_fields, _INT32, _INT64 = _native.fields, _native.INT32, _native.INT64
 
 
 class SlotMapper:
@@ -107,38 +102,45 @@ class SlotMapper:
         page ids of whole rows.  Two requests of one call must not share a
         row, unless at most one of them has new tokens.  Failures that only
         the device sees are bits of ``status`` (``SlotMap.check``)."""
-        batch, index = row_ids.shape[0], self._index
+        index = self._index
+        (rows_ptr, rows_dev, rows_dt, batch, rows_step, raw_ptr, raw_dev, raw_dt, n_raw, raw_step,
+         new_ptr, new_dev, new_dt, n_new, new_step, free_ptr, free_dev, _, free_n, free_step,
+         state_ptr, state_dev, state_dt, state_n, _) = _fields(1, row_ids, raw_lens, new_lens,
+                                                               ring.ring, ring.state)
         if batch > self.max_batch:
             raise ValueError("batch exceeds max_batch")
-        rows, columns = req_to_token.shape
-        row_stride, unit = req_to_token.stride()
-        if req_to_token.dtype != torch.int32 or unit != 1 or req_to_token.get_device() != index:
+        if n_raw != batch or n_new != batch or not rows_dev == raw_dev == new_dev == index or \
+                (batch > 1 and not rows_step == raw_step == new_step == 1):
+            raise ValueError("row_ids, raw_lens and new_lens must be contiguous vectors of one "
+                             "entry per request, on the mapper's device")
+        for dt in (rows_dt, raw_dt, new_dt):
+            if dt != _INT32 and dt != _INT64:
+                raise ValueError("row_ids, raw_lens and new_lens must be int32 or int64")
+        if free_dev != index or state_dev != index or free_n < ring.capacity or state_n < 2 or \
+                state_dt != _INT64:
+            raise ValueError("the free ring must be on the mapper's device")
+        table, dev, dt, rows, columns, row_stride, unit = _fields(2, req_to_token)
+        if dt != _INT32 or unit != 1 or dev != index:
             raise ValueError("req_to_token must be int32 [rows, columns] with unit last stride, "
                              "on the mapper's device")
-        is64 = [_vector(name, t, batch, index) for name, t in
-                (("row_ids", row_ids), ("raw_lens", raw_lens), ("new_lens", new_lens))]
         next_ptr = next64 = parents_ptr = table_ptr = table_stride = table_columns = 0
         if next_positions is not None:
-            next64 = _vector("next_positions", next_positions, batch, index)
-            next_ptr = next_positions.data_ptr()
+            next_ptr, dev, dt, n, step = _fields(1, next_positions)
+            if n != batch or dev != index or (step != 1 and n > 1) or \
+                    (dt != _INT32 and dt != _INT64):
+                raise ValueError("next_positions must be a contiguous int32 or int64 vector of "
+                                 "one entry per request, on the mapper's device")
+            next64 = 1 if dt == _INT64 else 0
         if parents is not None:
-            if parents.dtype != torch.int32 or parents.ndim != 1 or \
-                    not parents.is_contiguous() or parents.get_device() != index or \
-                    parents.shape[0] < self.max_new_tokens:
+            parents_ptr, dev, dt, n, step = _fields(1, parents)
+            if dt != _INT32 or dev != index or n < self.max_new_tokens or (step != 1 and n > 1):
                 raise ValueError("parents must be a contiguous int32 vector of max_new_tokens "
                                  "entries on the mapper's device")
-            parents_ptr = parents.data_ptr()
         if block_table is not None:
-            table_rows, table_columns = block_table.shape
-            table_stride, unit = block_table.stride()
-            if block_table.dtype != torch.int32 or unit != 1 or table_rows < batch or \
-                    block_table.get_device() != index:
+            table_ptr, dev, dt, n, table_columns, table_stride, unit = _fields(2, block_table)
+            if dt != _INT32 or unit != 1 or n < batch or dev != index:
                 raise ValueError("block_table must be int32 [>= batch, columns] with unit last "
                                  "stride, on the mapper's device")
-            table_ptr = block_table.data_ptr()
-        free, state = ring.ring, ring.state
-        if free.get_device() != index or state.get_device() != index:
-            raise ValueError("the free ring must be on the mapper's device")
         offsets = self._offsets if batch == self.max_batch else self._offsets[: batch + 1]
         result = SlotMap(offsets, self._slots, self._positions,
                          self._mask if parents is not None else None, block_table, self._totals,
@@ -148,9 +150,9 @@ class SlotMapper:
                 t.zero_()
             return result
         status = _native.launch(index, _native.lib.akv_map_slots, _native.MAP_SLOTS.pack(
-            req_to_token.data_ptr(), row_stride, rows, columns, row_ids.data_ptr(), is64[0],
-            raw_lens.data_ptr(), is64[1], new_lens.data_ptr(), is64[2], batch, self.page_size,
-            free.data_ptr(), state.data_ptr(), ring.capacity, next_ptr, next64, parents_ptr,
+            table, row_stride, rows, columns, rows_ptr, 1 if rows_dt == _INT64 else 0, raw_ptr,
+            1 if raw_dt == _INT64 else 0, new_ptr, 1 if new_dt == _INT64 else 0, batch,
+            self.page_size, free_ptr, state_ptr, ring.capacity, next_ptr, next64, parents_ptr,
             self.max_new_tokens, *self._outputs, table_ptr, table_stride, table_columns,
             *self._words, 1 if commit else 0))
         _native.check(status, "map_slots")

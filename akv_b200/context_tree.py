@@ -102,25 +102,7 @@ def tree_work_list(kv_indptr, draft_indptr, group, num_kv_heads, pair_heads, cta
     return items.astype(np.int32), cta_items, merges.astype(np.int32), int(cut.sum()) * UNITS
 
 
-def _rows(name, t, dtype, index, tokens, shape):
-    """The first two strides of a [>= tokens, heads, head_dim] tensor."""
-    n, *rest = t.shape
-    s = t.stride()
-    if tuple(rest) != shape or n < tokens or t.dtype != dtype or s[2] != 1 or \
-            t.get_device() != index:
-        raise ValueError(f"{name} must be [tokens or slots, heads, head_dim] = [>= {tokens}, "
-                         f"{shape[0]}, {shape[1]}] {dtype} with unit last stride, on the plan's "
-                         "device")
-    return s[0], s[1]
-
-
-def _vector(name, t, dtype, index, n):
-    """The address of a contiguous vector of at least n entries."""
-    if t.dtype != dtype or t.ndim != 1 or t.shape[0] < n or not t.is_contiguous() or \
-            t.get_device() != index:
-        raise ValueError(f"{name} must be a contiguous {dtype} vector of the plan's length, on "
-                         "the plan's device")
-    return t.data_ptr()
+_fields, _INT32, _INT64 = _native.fields, _native.INT32, _native.INT64
 
 
 class TreeAttention:
@@ -213,41 +195,63 @@ class TreeAttention:
 
         The head's maximum, sum and accumulator are fp32; P is rounded to the
         pools' type for P.V.  Returns out, or (out, lse fp32 [tokens, Hq])."""
-        index, tokens, dtype = self._index, self.tokens, self.dtype
-        q_token, q_head = _rows("q", q, dtype, index, tokens, (self.hq, self.d))
-        k_slot, k_head = _rows("k_pool", k_pool, dtype, index, 1, (self.hkv, self.d))
-        v_slot, v_head = _rows("v_pool", v_pool, dtype, index, 1, (self.hkv, self.d))
+        index, tokens, keys, hq, hkv, d = (self._index, self.tokens, self.keys, self.hq, self.hkv,
+                                           self.d)
+        (q_ptr, q_dev, q_dt, n, heads, dim, q_token, q_head, q_unit, k_ptr, k_dev, k_dt, k_slots,
+         k_heads, k_dim, k_slot, k_head, k_unit, v_ptr, v_dev, v_dt, v_slots, v_heads, v_dim,
+         v_slot, v_head, v_unit) = _fields(3, q, k_pool, v_pool)
+        code = _native.FIELD_CODE.get(q_dt)
+        if code != self._code or n < tokens or heads != hq or dim != d or q_unit != 1 or \
+                q_dev != index:
+            raise ValueError("q must be [>= tokens, num_q_heads, head_dim] of the planned type "
+                             "with unit last stride, on the plan's device")
+        if k_dt != q_dt or v_dt != q_dt or k_heads != hkv or v_heads != hkv or k_dim != d or \
+                v_dim != d or k_unit != 1 or v_unit != 1 or k_dev != index or v_dev != index:
+            raise ValueError("KV pools must be [slots, num_kv_heads, head_dim] of the planned type "
+                             "with unit last stride, on the plan's device")
+        (kv_ptr, kv_dev, kv_dt, kv_n, kv_step, draft_ptr, draft_dev, draft_dt, draft_n, draft_step,
+         mask_ptr, mask_dev, mask_dt, mask_n, mask_step) = _fields(1, kv_indices, draft_slots,
+                                                                   tree_mask)
+        if kv_n < keys or draft_n < tokens or mask_n < tokens or kv_dt != _INT32 or \
+                draft_dt != _INT32 or mask_dt != _INT64 or \
+                not kv_dev == draft_dev == mask_dev == index or (kv_step != 1 and kv_n > 1) or \
+                (draft_step != 1 and draft_n > 1) or (mask_step != 1 and mask_n > 1):
+            raise ValueError("kv_indices (int32), draft_slots (int32) and tree_mask (int64) must "
+                             "be contiguous vectors of the plan's lengths, on its device")
         window = -1 if window is None or window < 0 else int(window)
-        ints = torch.int32
-        kv_ptr = _vector("kv_indices", kv_indices, ints, index, self.keys)
-        draft_ptr = _vector("draft_slots", draft_slots, ints, index, tokens)
-        mask_ptr = _vector("tree_mask", tree_mask, torch.int64, index, tokens)
         dev = self._plan_ptr
         q_pos = kv_pos = sinks_ptr = lse_ptr = 0
         if window >= 0:
             if q_positions is None or kv_positions is None:
                 raise ValueError("a window needs q_positions and kv_positions")
-            q_pos = _vector("q_positions", q_positions, ints, index, tokens)
-            kv_pos = _vector("kv_positions", kv_positions, ints, index, self.keys) or dev
+            (q_pos, dev0, dt0, n0, step0, kv_pos, dev1, dt1, n1,
+             step1) = _fields(1, q_positions, kv_positions)
+            if n0 < tokens or n1 < keys or not dt0 == dt1 == _INT32 or \
+                    not dev0 == dev1 == index or (step0 != 1 and n0 > 1) or (step1 != 1 and n1 > 1):
+                raise ValueError("q_positions and kv_positions must be contiguous int32 vectors "
+                                 "of the plan's lengths, on its device")
+            kv_pos = kv_pos or dev
         if sinks is not None:
-            if sinks.shape != (self.hq,):
-                raise ValueError("sinks must be fp32 [num_q_heads]")
-            sinks_ptr = _vector("sinks", sinks, torch.float32, index, self.hq)
+            sinks_ptr, dev0, dt0, n0, step0 = _fields(1, sinks)
+            if n0 != hq or _native.FIELD_CODE.get(dt0) != _native.AKV_F32 or dev0 != index or \
+                    (step0 != 1 and n0 > 1):
+                raise ValueError("sinks must be fp32 [num_q_heads] on the plan's device")
         if out is None:
-            out = torch.empty((tokens, self.hq, self.d), dtype=dtype, device=self.device)
-        o_token, o_head = _rows("out", out, dtype, index, tokens, (self.hq, self.d))
+            out = torch.empty((tokens, hq, d), dtype=self.dtype, device=self.device)
+        o_ptr, o_dev, o_dt, n, heads, dim, o_token, o_head, unit = _fields(3, out)
+        if n < tokens or heads != hq or dim != d or unit != 1 or o_dev != index or o_dt != q_dt:
+            raise ValueError("out must be [>= tokens, num_q_heads, head_dim] of the planned type "
+                             "with unit last stride, on the plan's device")
         lse = None
         if return_lse:
             lse = torch.empty((tokens, self.hq), dtype=torch.float32, device=self.device)
             lse_ptr = lse.data_ptr()
         status = _native.launch(index, _native.lib.akv_tree_attention, _native.TREE_ATTENTION.pack(
-            q.data_ptr(), q_token, q_head, k_pool.data_ptr(), v_pool.data_ptr(), k_slot, k_head,
-            v_slot, v_head, min(k_pool.shape[0], v_pool.shape[0]), self._code, tokens, self.keys,
-            kv_ptr or dev,
-            draft_ptr, mask_ptr, q_pos, kv_pos, window, sinks_ptr, self.sm_scale, self.hq,
-            self.hkv, self.d, dev, dev + 4 * self._at[1], self.n_ctas, dev + 4 * self._at[0],
-            self.n_merges, *self._partial_ptrs, out.data_ptr(), o_token, o_head, lse_ptr,
-            self._flag_ptr))
+            q_ptr, q_token, q_head, k_ptr, v_ptr, k_slot, k_head, v_slot, v_head,
+            k_slots if k_slots < v_slots else v_slots, code, tokens, keys, kv_ptr or dev,
+            draft_ptr, mask_ptr, q_pos, kv_pos, window, sinks_ptr, self.sm_scale, hq, hkv, d, dev,
+            dev + 4 * self._at[1], self.n_ctas, dev + 4 * self._at[0], self.n_merges,
+            *self._partial_ptrs, o_ptr, o_token, o_head, lse_ptr, self._flag_ptr))
         _native.check(status, "tree_attention")
         return (out, lse) if return_lse else out
 

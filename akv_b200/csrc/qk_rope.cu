@@ -390,8 +390,8 @@ extern "C" int akv_qk_norm_rope(const akv_qk_norm_rope_args* args, void* stream)
              x.q_out_stride_head, x.k_out, x.k_out_stride_token, x.k_out_stride_head, x.k_pool,
              x.k_pool_stride_slot, x.k_pool_stride_head, x.v_pool, x.v_pool_stride_slot,
              x.v_pool_stride_head, x.q_weight, x.k_weight, x.weight_dtype == AKV_F32,
-             (float)x.eps, 1.f / (float)x.head_dim, x.positions, x.positions_is64 != 0, x.slots, x.slots_is64 != 0,
-             x.cos_sin_cache, (int)x.cache_dtype, x.cache_stride, x.max_position, x.num_slots,
+             (float)x.eps, 1.f / (float)x.head_dim, x.positions, x.positions_is64 != 0, x.slots,
+             x.slots_is64 != 0, x.cos_sin_cache, (int)x.cache_dtype, x.cache_stride, x.max_position, x.num_slots,
              x.tokens, (int)x.num_q_heads, (int)x.num_kv_heads, (int)x.head_dim,
              (int)x.rotary_dim, 0, 0, 0, x.error_flag};
   const int neox = x.is_neox_style != 0;

@@ -15,6 +15,27 @@
 // 128-key tiles of one request for one or two (head, row tile) units; the
 // host cuts the flat list of all key tiles into equal runs, one per CTA, and
 // a second kernel joins the pieces of units that were cut.
+//
+// Bound.  A key costs Hkv D 4 bytes and 4 Hq D flops per drafted token: HBM up to
+// about 16 tokens per request at a group of 8, the softmax and the tensor
+// cores above.  Measured (device time): 64 requests of 16 tokens over 4K-12K
+// keys at random slots, 64 / 8 heads of 64 (1.11 GB): 265 us, 4.2 TB/s, 0.64 of
+// the copy rate, 527 TFLOP/s; with its softmax taken out 208 us (the gather), with its
+// loads taken out 253 us (scores -> P -> P.V per tile; a unit's 128 keys take
+// about 3,900 cycles, of which 2,200 are exponentials at two warps per
+// scheduler).  Trees of 33-64 tokens over 16K-32K keys of head_dim 128: 515 us,
+// 662 TFLOP/s, 0.40 of cuBLAS bf16; a head's K/V are gathered once per two row tiles, 430 us
+// alone.  What a step changed, and what was tried and left, is in the comments below.
+//
+// The pieces that decide the time: 128-key tiles with one CTA per SM (64-key
+// tiles with two CTAs 342 us on the first case, 80 registers a thread spill);
+// producers that issue a copy in four instructions (29 with a 64-bit
+// product and a swizzle each: 299 us); masks applied to the scores in tensor
+// memory, so that the ordinary path has none; a quarter of the exponentials as
+// polynomials on the FMA pipes (none 287 us, three eighths 279); registers (the
+// same loop at 96 instead of 128 a thread, by spills, 10 % slower).  No gain: units
+// half a tile apart, scores loaded behind the work on the last ones, one pass
+// over the scores with a running base, 16 softmax warps.
 
 #include <type_traits>
 
@@ -761,6 +782,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         if (!warp_wait(bar_x, n_x++ & 1, abort)) break;
       }
     }
+    cp_async_wait<0>();  // a next item's Q, if a failed wait ended the loop
   }
   tc_fence_before();
   __syncthreads();
@@ -854,8 +876,8 @@ extern "C" int akv_tree_attention(const akv_tree_attention_args* args, void* str
   const akv_tree_attention_args& x = *args;
   if (x.num_kv_heads <= 0 || x.num_q_heads <= 0 || x.num_q_heads > INT32_MAX / 64 ||
       x.num_q_heads % x.num_kv_heads || x.n_ctas < 0 || x.n_ctas > INT32_MAX || x.n_merges < 0 ||
-      x.n_merges > INT32_MAX || x.tokens < 0 || x.keys < 0 || !(x.sm_scale > 0.) || x.num_slots <= 0 ||
-      x.num_slots > INT32_MAX || (x.dtype != AKV_F16 && x.dtype != AKV_BF16))
+      x.n_merges > INT32_MAX || x.tokens < 0 || x.keys < 0 || !(x.sm_scale > 0.) ||
+      x.num_slots <= 0 || x.num_slots > INT32_MAX || (x.dtype != AKV_F16 && x.dtype != AKV_BF16))
     return AKV_ERR_INVALID;
   if (x.head_dim != 64 && x.head_dim != 128) return AKV_ERR_UNSUPPORTED;
   if (x.n_ctas == 0) return AKV_OK;
