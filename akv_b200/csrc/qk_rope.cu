@@ -21,11 +21,14 @@
 // four rows (two in fp32) that it requests before it uses the first; the
 // arithmetic is packed (f32x2), two elements an instruction, since with scalar
 // instructions their issue was the limit (142 us at best on the first case
-// below).  Measured, bf16: 16,411 tokens of 64 + 8 + 8 heads of 128 (681 MB)
-// 127 us, 5.4 TB/s, 0.82 of the copy rate, at 12 blocks of 64 threads per SM
-// (80 registers); two rows per lane 132 us, eight 138 us, four at 16 warps per SM
-// 141 us and at 28 146 us (spills).  2,048 tokens of head_dim 64 (42.5 MB) 12.5
-// us; one token 4.4 us, the launch.
+// below).  Measured, bf16 (calls one after another in a graph, other inputs each):
+// 16,411 tokens of 64 + 8 + 8 heads of 128 (681 MB) 124 us, 5.5 TB/s, 0.84 of the
+// copy rate, at 12 blocks of 64 threads per SM (80 registers); two rows per lane 132
+// us, eight 138 us, four at 16 warps per SM 141 us and at 28 146 us (spills).  2,048
+// tokens of head_dim 64 (42.5 MB) 11.8 us; one token 3.5 us.  With only a part of
+// D turning (fp16, pairs, 64 of 128, 76.6 MB) 17.5 us, 4.4 TB/s: 2.6 waves of
+// blocks, and the masks of what does not turn (16.5 without; two rows per lane
+// 18.8).
 
 #include <type_traits>
 
@@ -147,8 +150,8 @@ __device__ __forceinline__ void load_turn(const void* base, long long a, long lo
 
 // T: element type; LANES: lanes per row (D / 16 rounded up to a power of
 // two); NEOX: halves or adjacent pairs; FULL: D is 16 LANES, so that every lane
-// has two runs; ROWS: rows per lane group.
-template <typename T, int LANES, bool NEOX, bool FULL, int ROWS>
+// has two runs; TURN: all of D turns; ROWS: rows per lane group.
+template <typename T, int LANES, bool NEOX, bool FULL, bool TURN, int ROWS>
 __global__ void __launch_bounds__(kRopeThreads, 12) qk_norm_rope_kernel(const RopeArgs a) {
   const uint32_t group = blockIdx.x * (kRopeThreads / LANES) + threadIdx.x / LANES;
   const int j = threadIdx.x % LANES;
@@ -240,6 +243,7 @@ __global__ void __launch_bounds__(kRopeThreads, 12) qk_norm_rope_kernel(const Ro
     s2[k] = f2_pack(s[2 * k], s[2 * k + 1]);
     n2[k] = f2_pack(-s[2 * k], -s[2 * k + 1]);
   }
+  const f32x2 keep = turned ? ~0ull : 0, keep1 = turned1 ? ~0ull : 0;
   Turn w;
   if (weight != nullptr) {
     float w0[8] = {}, w1[8] = {};
@@ -292,9 +296,20 @@ __global__ void __launch_bounds__(kRopeThreads, 12) qk_norm_rope_kernel(const Ro
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      f32x2 xs = f2_mul(v.x[k], s2[k]), ys;
+      if (TURN) {
+        ys = f2_mul(v.y[k], n2[k]);
+      } else {
+        // Past the rotation the turn is by cos 1 and sin 0, and the products
+        // are masked to 0: an infinity times sin 0 would be NaN.  The sign is
+        // set here too, since n2's registers would spill.
+        const f32x2 on = NEOX || k < 2 ? keep : keep1;
+        xs &= on;
+        ys = (f2_mul(v.y[k], s2[k]) & on) ^ 0x8000000080000000ull;
+      }
       float p0, p1, q0, q1;
-      f2_unpack(f2_fma(v.x[k], c2[k], f2_mul(v.y[k], n2[k])), p0, p1);
-      f2_unpack(f2_fma(v.y[k], c2[k], f2_mul(v.x[k], s2[k])), q0, q1);
+      f2_unpack(f2_fma(v.x[k], c2[k], ys), p0, p1);
+      f2_unpack(f2_fma(v.y[k], c2[k], xs), q0, q1);
       if (NEOX) {
         x0[r].set2(2 * k, p0, p1);
         x1[r].set2(2 * k, q0, q1);
@@ -315,7 +330,7 @@ __global__ void __launch_bounds__(kRopeThreads, 12) qk_norm_rope_kernel(const Ro
   }
 }
 
-template <typename T, int LANES, bool NEOX, bool FULL>
+template <typename T, int LANES, bool NEOX, bool FULL, bool TURN>
 int launch_rope(RopeArgs& a, cudaStream_t stream) {
   constexpr int ROWS = sizeof(T) == 4 ? 2 : 4;
   a.q_units = (a.hq + ROWS - 1) / ROWS;
@@ -324,19 +339,22 @@ int launch_rope(RopeArgs& a, cudaStream_t stream) {
   const long long groups = a.tokens * a.units, per = kRopeThreads / LANES;
   const long long blocks = (groups + per - 1) / per;
   if (groups + per > UINT32_MAX) return AKV_ERR_INVALID;  // 32-bit group numbers
-  qk_norm_rope_kernel<T, LANES, NEOX, FULL, ROWS>
+  qk_norm_rope_kernel<T, LANES, NEOX, FULL, TURN, ROWS>
       <<<(unsigned)blocks, kRopeThreads, 0, stream>>>(a);
   return launch_status();
 }
 
+template <typename T, int LANES, bool NEOX>
+int launch_rope_turn(RopeArgs& a, cudaStream_t stream) {
+  if (a.dim != 16 * LANES) return launch_rope<T, LANES, NEOX, false, false>(a, stream);
+  return a.rotary == a.dim ? launch_rope<T, LANES, NEOX, true, true>(a, stream)
+                           : launch_rope<T, LANES, NEOX, true, false>(a, stream);
+}
+
 template <typename T, int LANES>
 int launch_rope_style(RopeArgs& a, int neox, cudaStream_t stream) {
-  const bool full = a.dim == 16 * LANES;
-  if (neox)
-    return full ? launch_rope<T, LANES, true, true>(a, stream)
-                : launch_rope<T, LANES, true, false>(a, stream);
-  return full ? launch_rope<T, LANES, false, true>(a, stream)
-              : launch_rope<T, LANES, false, false>(a, stream);
+  return neox ? launch_rope_turn<T, LANES, true>(a, stream)
+              : launch_rope_turn<T, LANES, false>(a, stream);
 }
 
 template <typename T>
@@ -391,8 +409,8 @@ extern "C" int akv_qk_norm_rope(const akv_qk_norm_rope_args* args, void* stream)
              x.k_pool_stride_slot, x.k_pool_stride_head, x.v_pool, x.v_pool_stride_slot,
              x.v_pool_stride_head, x.q_weight, x.k_weight, x.weight_dtype == AKV_F32,
              (float)x.eps, 1.f / (float)x.head_dim, x.positions, x.positions_is64 != 0, x.slots,
-             x.slots_is64 != 0, x.cos_sin_cache, (int)x.cache_dtype, x.cache_stride, x.max_position, x.num_slots,
-             x.tokens, (int)x.num_q_heads, (int)x.num_kv_heads, (int)x.head_dim,
+             x.slots_is64 != 0, x.cos_sin_cache, (int)x.cache_dtype, x.cache_stride, x.max_position,
+             x.num_slots, x.tokens, (int)x.num_q_heads, (int)x.num_kv_heads, (int)x.head_dim,
              (int)x.rotary_dim, 0, 0, 0, x.error_flag};
   const int neox = x.is_neox_style != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -147,6 +147,28 @@ def test_infinities_and_zero_rows():
     assert bool(out[clean].isfinite().all())
 
 
+@pytest.mark.parametrize("neox", [True, False])
+@pytest.mark.parametrize("d,rotary", [(128, 64), (80, 48), (256, 16)])
+@pytest.mark.parametrize("normed", [False, True])
+def test_dimensions_past_the_rotation_do_not_reach_one_another(neox, d, rotary, normed):
+    """An infinity there changes its own element (and the norm), no other."""
+    from akv_b200.context_rope import qk_norm_rope
+
+    x = inputs(d - rotary, 3, 2, d, rotary, torch.float16, seed=2)
+    row = torch.arange(d - rotary, device="cuda")
+    for t in (x["q"], x["k"]):  # token i: the i-th of these dimensions
+        t[row, 1, rotary + row] = float("inf") if normed else float("nan")
+        t[row, 0, rotary + row] = -float("inf")
+    w = dict(q_weight=x["wq"], k_weight=x["wk"]) if normed else {}
+    q, k = qk_norm_rope(x["q"], x["k"], x["pos"], x["table"], is_neox_style=neox, **w)
+    for got, t, wt in ((q, x["q"], x["wq"]), (k, x["k"], x["wk"])):
+        want, size = formula(t, wt if normed else None, x["table"], x["pos"], neox, 1e-6)
+        odd = ~torch.isfinite(want)
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.isinf(got), torch.isinf(want))
+        near(got.masked_fill(odd, 0), want.masked_fill(odd, 0), size.masked_fill(odd, 0), d)
+
+
 def test_a_row_past_32_bits_of_elements():
     """Pool rows whose element offset passes 2^31."""
     from akv_b200.context_rope import qk_norm_rope
