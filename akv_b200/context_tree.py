@@ -122,8 +122,8 @@ class TreeAttention:
             raise ValueError("tree attention runs on bf16 or fp16")
         if max_batch <= 0 or (ctas is not None and ctas <= 0):
             raise ValueError("max_batch and ctas must be positive")
-        if sm_scale is not None and not sm_scale > 0:
-            raise ValueError("sm_scale must be positive")
+        if sm_scale is not None and not 1e-30 < sm_scale < 1e30:
+            raise ValueError("sm_scale must be positive and an ordinary fp32 number")
         device = torch.device(device)
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
@@ -191,7 +191,7 @@ class TreeAttention:
         sink).  ``window`` (None or negative: none) hides keys with
         q_position - kv_position > window and needs both position vectors
         (int32; those of the drafted keys are ``q_positions``).  Rows of
-        ``out`` past the planned tokens are left as they were.
+        ``out`` past the planned tokens are left as they were; ``out`` may be ``q``.
 
         The head's maximum, sum and accumulator are fp32; P is rounded to the
         pools' type for P.V.  Returns out, or (out, lse fp32 [tokens, Hq])."""

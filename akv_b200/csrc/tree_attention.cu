@@ -24,7 +24,7 @@
 // loads taken out 253 us (scores -> P -> P.V per tile; a unit's 128 keys take
 // about 3,900 cycles, of which 2,200 are exponentials at two warps per
 // scheduler).  Trees of 33-64 tokens over 16K-32K keys of head_dim 128: 515 us,
-// 662 TFLOP/s, 0.40 of cuBLAS bf16; a head's K/V are gathered once per two row tiles, 430 us
+// 663 TFLOP/s, 0.40 of cuBLAS bf16; a head's K/V are gathered once per two row tiles, 437 us
 // alone.  What a step changed, and what was tried and left, is in the comments below.
 //
 // The pieces that decide the time: 128-key tiles with one CTA per SM (64-key
@@ -307,9 +307,8 @@ __device__ __forceinline__ void restore(const TreeParams& p, const TreeItem& w,
 }
 
 // Warps 0-3 and 4-7 are the softmax of units 0 and 1 (warp w: rows 32 (w % 4)
-// .., one row per thread), 8-15 the producers,
-// 16 and 17 the MMA issuers, one per unit so that units never wait for one
-// another.  A pair item gives the units different heads or row tiles over
+// .., one row per thread), 8-11 the producers, 12 and 13 the MMA issuers, one
+// per unit so that units never wait for one another.  A pair item gives the units different heads or row tiles over
 // the same keys; a single one gives both the same rows and alternate key
 // tiles, and its accumulators are joined out of tensor memory at the end.
 // Barriers.  Per slot: full (every producer thread's copies have landed),
@@ -317,7 +316,7 @@ __device__ __forceinline__ void restore(const TreeParams& p, const TreeItem& w,
 // reads a single item's slot signals twice).  Per unit: q (its Q tile is
 // stored), s (scores done), f (head_dim 64: the scores are read, so the
 // next product may overwrite them while P is made), p (P stored), o (P.V
-// done).  x: the units meet around the join.  A waiter is never two phases
+// done), d (all of it done, at the end).  x: the units meet around the join.  A waiter is never two phases
 // behind: S(c + 1) needs f(c) or o(c), P(c + 1) is stored after o(c).  Waits are
 // bounded; once one runs out the CTA's abort flag ends every role's loop and
 // *error_flag gets bit 2.
@@ -340,7 +339,8 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
   auto bar_p = [&](int u) { return unit_bar(u, 3); };
   auto bar_o = [&](int u) { return unit_bar(u, 4); };
   const uint32_t bar_x = unit_bar(2, 0);
-  static_assert(8 * (2 * C::kSlots + 11) <= 240, "barriers and flags");
+  auto bar_d = [&](int u) { return bars + 8u * (2 * C::kSlots + 11 + u); };
+  static_assert(8 * (2 * C::kSlots + 13) <= 240, "barriers and flags");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOff + 240);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + C::kBarOff + 244);
   volatile int* scrubbed = reinterpret_cast<volatile int*>(smem + C::kBarOff + 248);
@@ -363,6 +363,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
       mbar_init(bar_f(u), 4);
       mbar_init(bar_p(u), 4);
       mbar_init(bar_o(u), 1);
+      mbar_init(bar_d(u), 1);
     }
     mbar_init(bar_x, C::kSoftmax);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -459,10 +460,18 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         at.phase ^= end / C::kSlots & 1;
         at.slot = end % C::kSlots;
       }
+      if (n_q > 0) {
+        // Every product and every commit has arrived before the CTA gives its
+        // memories back: the last slot's release outlives the roles' waits, and
+        // after a failed wait so may products.
+        volatile int late = 0;
+        umma_commit(bar_d(u));
+        if (!ws_wait(bar_d(u), 0, &late)) *abort = 1;
+      }
     }
     __syncwarp();
   } else if (warp >= C::kSoftmax) {
-    // ---- producers: warp pw gathers keys 16 pw .. of every tile ----
+    // ---- producers: warp pw gathers keys 32 pw .. of every tile ----
     constexpr int kKpw = kTreeKeys / C::kProducers;
     const int pw = warp - C::kSoftmax;
     Pos at;
@@ -876,7 +885,8 @@ extern "C" int akv_tree_attention(const akv_tree_attention_args* args, void* str
   const akv_tree_attention_args& x = *args;
   if (x.num_kv_heads <= 0 || x.num_q_heads <= 0 || x.num_q_heads > INT32_MAX / 64 ||
       x.num_q_heads % x.num_kv_heads || x.n_ctas < 0 || x.n_ctas > INT32_MAX || x.n_merges < 0 ||
-      x.n_merges > INT32_MAX || x.tokens < 0 || x.keys < 0 || !(x.sm_scale > 0.) ||
+      x.n_merges > INT32_MAX || x.tokens < 0 || x.keys < 0 || !((float)x.sm_scale > 0.f) ||
+      !((float)x.sm_scale * kLog2e < INFINITY) ||  // a hidden score of -inf stays -inf
       x.num_slots <= 0 || x.num_slots > INT32_MAX || (x.dtype != AKV_F16 && x.dtype != AKV_BF16))
     return AKV_ERR_INVALID;
   if (x.head_dim != 64 && x.head_dim != 128) return AKV_ERR_UNSUPPORTED;

@@ -142,6 +142,13 @@ def test_tree_attention_refuses(change):
     assert _native.lib.akv_tree_attention(*tree_args(**change)) == _native.AKV_ERR_INVALID
 
 
+@pytest.mark.parametrize("scale", [1e-50, 1e39, float("inf"), float("nan")])
+def test_tree_attention_refuses_scales_that_fp32_does_not_hold(scale):
+    from akv_b200 import _native
+
+    assert _native.lib.akv_tree_attention(*tree_args(scale=scale)) == _native.AKV_ERR_INVALID
+
+
 def test_tree_attention_of_nothing_is_ok_and_other_head_dims_are_unsupported():
     from akv_b200 import _native
 

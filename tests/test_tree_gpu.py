@@ -329,6 +329,15 @@ def test_results_do_not_change_from_run_to_run():
         assert torch.equal(launch(c, attn), first)
 
 
+@pytest.mark.parametrize("ctas", [None, 2, 1])
+def test_the_output_may_be_the_queries(ctas):
+    c = make([700, 30, 0, 1500], [16, 64, 3, 5], 3, 5, 64, torch.bfloat16, sinks=True)
+    want = launch(c, attention(c, ctas))
+    mine = {**c, "q": c["q"].clone()}
+    got = launch(mine, attention(c, ctas), out=mine["q"])
+    assert got is mine["q"] and torch.equal(got, want)
+
+
 def test_two_instances_on_two_streams():
     cases = [make([1500, 40], [16, 20], 4, 8, 64, torch.bfloat16, seed=s) for s in (13, 14)]
     attns = [attention(c) for c in cases]
