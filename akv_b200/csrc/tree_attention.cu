@@ -19,13 +19,15 @@
 // Bound.  A key costs Hkv D 4 bytes and 4 Hq D flops per drafted token: HBM up to
 // about 16 tokens per request at a group of 8, the softmax and the tensor
 // cores above.  Measured (device time): 64 requests of 16 tokens over 4K-12K
-// keys at random slots, 64 / 8 heads of 64 (1.11 GB): 265 us, 4.2 TB/s, 0.64 of
-// the copy rate, 527 TFLOP/s; with its softmax taken out 208 us (the gather), with its
-// loads taken out 253 us (scores -> P -> P.V per tile; a unit's 128 keys take
+// keys at random slots, 64 / 8 heads of 64 (1.11 GB): 262 us, 4.2 TB/s, 0.65 of
+// the copy rate, 533 TFLOP/s; with its softmax taken out 208 us (the gather), with
+// its loads taken out 253 us (scores -> P -> P.V per tile; a unit's 128 keys take
 // about 3,900 cycles, of which 2,200 are exponentials at two warps per
-// scheduler).  Trees of 33-64 tokens over 16K-32K keys of head_dim 128: 515 us,
-// 663 TFLOP/s, 0.40 of cuBLAS bf16; a head's K/V are gathered once per two row tiles, 437 us
-// alone.  What a step changed, and what was tried and left, is in the comments below.
+// scheduler).  Trees of 33-64 tokens over 16K-32K keys of head_dim 128: 511 us,
+// 668 TFLOP/s, 0.40 of cuBLAS bf16; a head's K/V are gathered once per two row
+// tiles, 437 us alone.  Short items are a chain of latencies, about 10,000 cycles
+// for one of one tile: 128 requests of 8 tokens and 100-140 keys in a window 45 us
+// (48 before an item's Q was handed on ahead of the epilogue before it).
 //
 // The pieces that decide the time: 128-key tiles with one CTA per SM (64-key
 // tiles with two CTAs 342 us on the first case, 80 registers a thread spill);
@@ -37,6 +39,7 @@
 // half a tile apart, scores loaded behind the work on the last ones, one pass
 // over the scores with a running base, 16 softmax warps.
 
+#include <climits>
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -111,13 +114,12 @@ __device__ __forceinline__ long long key_slot(const TreeParams& p, const TreeIte
   return slot < 0 ? -1 : slot;
 }
 
-// Visible drafted tokens of token i: its mask, without those the window hides.
+// Visible drafted tokens of a token at `pos`: its mask m, without those the
+// window hides.
 __device__ __forceinline__ unsigned long long row_mask(const TreeParams& p, const TreeItem& w,
-                                                       int i) {
-  unsigned long long m = p.tree_mask[w.q0 + i];
+                                                       unsigned long long m, long long pos) {
   if (w.n < 64) m &= (1ull << w.n) - 1;
   if (p.window >= 0) {
-    const long long pos = p.q_positions[w.q0 + i];
     for (unsigned long long left = m; left; left &= left - 1) {
       const int j = __ffsll((long long)left) - 1;
       if (pos - p.q_positions[w.q0 + j] > p.window) m &= ~(1ull << j);
@@ -126,15 +128,15 @@ __device__ __forceinline__ unsigned long long row_mask(const TreeParams& p, cons
   return m;
 }
 
-// Joins the sink to a row's maximum m (base 2) and sum l: `scale` is the
+// Joins the sink (-inf: none) to a row's maximum m (base 2) and sum l: `scale` is the
 // factor of the accumulator in the output, lse the natural logarithm.  The
 // maximum takes the sink in, so neither a sink far above every score nor one
 // of a row without keys overflows.
 struct RowEnd {
   float scale, lse;
 };
-__device__ __forceinline__ RowEnd row_end(const float* sinks, int h, float m, float l) {
-  const float sink = sinks ? sinks[h] * kLog2e : -INFINITY;
+__device__ __forceinline__ RowEnd row_end(float sink, float m, float l) {
+  sink *= kLog2e;
   const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
   const float f = fast_exp2(m - base);
   const float den = l * f + fast_exp2(sink - base);
@@ -320,7 +322,7 @@ __device__ __forceinline__ void restore(const TreeParams& p, const TreeItem& w,
 // behind: S(c + 1) needs f(c) or o(c), P(c + 1) is stored after o(c).  Waits are
 // bounded; once one runs out the CTA's abort flag ends every role's loop and
 // *error_flag gets bit 2.
-template <typename T, int D>
+template <typename T, int D, bool WIN>
 __global__ void __launch_bounds__(TreeCfg<D>::kThreads, 1)
 tree_attention_kernel(const __grid_constant__ TreeParams p) {
   using C = TreeCfg<D>;
@@ -480,9 +482,18 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
       const TreeItem w = p.items[it];
       const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
       const int heads = w.head_step ? 2 : 1;
+      int last = INT_MIN;  // the request's last position
+      if (WIN) {
+        for (int i = lane; i < w.n; i += 32) last = max(last, p.q_positions[w.q0 + i]);
+        last = __reduce_max_sync(0xffffffffu, last);
+      }
+      bool hidden = false;  // this lane's next key, by the window, from some token
       auto fetch = [&](int t) {
         const int j = w.lo + t * kTreeKeys + kKpw * pw + lane % kKpw;
-        return t < n_tiles && j < w.hi ? (int)key_slot(p, w, j) : -1;
+        if (t >= n_tiles || j >= w.hi) return -1;
+        hidden = WIN && j < w.prefix &&
+                 (long long)last - p.kv_positions[w.kv0 + j] > p.window;
+        return (int)key_slot(p, w, j);
       };
       int next = fetch(0);
       // chunks: 16-byte pieces per key, consecutive lanes on one key.
@@ -490,12 +501,14 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         constexpr int kCpk = decltype(chunks)::value, kPer = 32 / kCpk, kRounds = kKpw / kPer;
         const int c = lane % kCpk, hh = c / (D / 8), cc = c % (D / 8), sub = lane / kCpk;
         const int slot = next;
+        // An infinity or NaN of a V row that only some rows see would reach
+        // the others as 0 * V: the warp's keys of this tile are searched for them
+        // before they are handed on if one may be hidden (by the tree, if the
+        // tile has drafted tokens, or the window).
+        const bool guarded =
+            w.lo + (t + 1) * kTreeKeys > w.prefix || (WIN && __any_sync(0xffffffffu, hidden));
         next = fetch(t + 1);
         const bool whole = __all_sync(0xffffffffu, slot >= 0);
-        // An infinity or NaN of a V row that only some rows see would reach
-        // the others as 0 * V: tiles with drafted tokens or a window are
-        // searched for them before they are handed on.
-        const bool guarded = p.window >= 0 || w.lo + (t + 1) * kTreeKeys > w.prefix;
         // The slots of the keys that this lane copies a piece of, all before
         // the first copy: between the copies each would wait for its shuffle.
         int sl[kRounds];
@@ -576,7 +589,20 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
       }
       cp_async_commit();
     };
+    // Hands it on: before the epilogue of the item before, which the first
+    // scores then run beside.
+    auto send_q = [&](int it) {
+      if (it >= it1) return;
+      const TreeItem w = p.items[it];
+      const int n_tiles = (w.hi - w.lo + kTreeKeys - 1) / kTreeKeys;
+      cp_async_wait<0>();
+      if (w.units == 2 || n_tiles > u) {
+        fence_async_smem();
+        mbar_arrive(bar_q(u));
+      }
+    };
     load_q(it0);
+    send_q(it0);
     for (int it = it0; it < it1; ++it) {
       float m = -INFINITY, l = 0.f;
       bool ok = true, warp_live;
@@ -588,43 +614,51 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         n = pair ? n_tiles : (n_tiles - u + 1) / 2;
         const int row0 = (w.tile0 + u * w.tile_step) * kTreeRows, i = (row0 + r) / p.group;
         warp_live = row0 + (warp & 3) * 32 < w.n * p.group;
-        const unsigned long long mask = i < w.n ? row_mask(p, w, i) : 0;
         const int pos = i < w.n && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
-        cp_async_wait<0>();
-        if (n > 0) {
-          fence_async_smem();
-          mbar_arrive(bar_q(u));
-        } else {
-          load_q(it + 1);
-        }
+        const unsigned long long word = i < w.n ? row_mask(p, w, p.tree_mask[w.q0 + i], pos) : 0;
+        if (n == 0) load_q(it + 1);
+        const int last = WIN ? __reduce_max_sync(0xffffffffu, pos) : 0;
         for (int v = 0; v < n && ok; ++v) {
           const uint32_t c = cnt + v;
           const int j0 = w.lo + (pair ? v : 2 * v + u) * kTreeKeys;
+          bool old = false;  // the window hides a key of the tile from a row of the warp
+          if (WIN && j0 + kTreeKeys <= w.prefix) {
+            const int* kp = p.kv_positions + w.kv0 + j0 + lane;
+            const int oldest = min(min(kp[0], kp[32]), min(kp[64], kp[96]));
+            old = __any_sync(0xffffffffu, (long long)last - oldest > p.window);
+          }
           ok = warp_wait(bar_s(u), c & 1, abort);
           if (!ok) break;
           if (v == n - 1) load_q(it + 1);
           if (warp_live) {
             tc_fence_after();
-            if (p.window >= 0 || j0 + kTreeKeys > w.prefix) {
+            // (The kernel without windows keeps the run-time tests of one, here and
+            // in the helpers: compiled without them its loop is 2 to 4 % slower.)
+            const bool tail = j0 + kTreeKeys > w.prefix;
+            if (WIN ? tail || old : tail || p.window >= 0) {
               // Hidden keys get a score of -inf in tensor memory, so that the
               // ordinary path below has no mask (and no registers for one).
 #pragma unroll 1
               for (int b = 0; b < kTreeKeys; b += 64) {
-                const unsigned long long seen = seen64(p, w, mask, i, pos, j0 + b, lane);
+                const unsigned long long seen = seen64(p, w, word, i, pos, j0 + b, lane);
                 if (__all_sync(0xffffffffu, seen == ~0ull)) continue;
 #pragma unroll 1
                 for (int q = 0; q < 64; q += 32) {
                   const uint32_t bits = (uint32_t)(seen >> q);
                   float x[32];
                   tmem_ld32_sync(tu + b + q, x);
-                  uint32_t y[32];
+                  uint32_t y[2][16];
 #pragma unroll
                   for (int k = 0; k < 32; ++k)
-                    y[k] = __float_as_uint(bits >> k & 1 ? x[k] : -INFINITY);
-                  tmem_st32_sync(tu + b + q, y);
+                    y[k / 16][k % 16] = __float_as_uint(bits >> k & 1 ? x[k] : -INFINITY);
+                  tmem_st16_async(tu + b + q, y[0]);
+                  tmem_st16_async(tu + b + q + 16, y[1]);
                 }
               }
+              tmem_st_wait();
             }
+          }
+          if (warp_live) {
             // The scores are read twice, for the maximum and for P: more than
             // 64 of them in registers cost spills.
             float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -718,8 +752,10 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
       const int row = (w.tile0 + u * w.tile_step) * kTreeRows + r, i = row / p.group;
       const int head = w.head0 + u * w.head_step, h = head * p.group + row - i * p.group;
       const bool live = i < w.n;
+      const float sink = live && p.sinks ? p.sinks[h] : -INFINITY;  // on its way over the wait
       cnt += n;
       if (n > 0 && !warp_wait(bar_o(u), cnt - 1 & 1, abort)) break;
+      send_q(it + 1);
       tc_fence_after();
       float f[2] = {1.f, 0.f};
       if (!pair) {  // the two units' rows meet
@@ -741,7 +777,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         const long long part = (long long)w.partial + (pair ? u : 0);
         float* acc = p.part_acc + part * D * kTreeRows + 4 * r;
         RowEnd e = {0.f, 0.f};
-        if (direct) e = row_end(p.sinks, live ? h : 0, m, l);
+        if (direct) e = row_end(sink, m, l);
         T* dst = static_cast<T*>(p.out) + (long long)(w.q0 + i) * p.o_st + (long long)h * p.o_sh;
         // A pair's units write all their columns, a single item's half each.
         const int d0 = pair ? 0 : u * (D / 2), d1 = pair ? D : d0 + D / 2;
@@ -773,9 +809,11 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
                   make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
           }
         }
-        if (live && *scrubbed)
-          restore<T>(p, w, row_mask(p, w, i), p.window >= 0 ? p.q_positions[w.q0 + i] : 0, head,
+        if (live && *scrubbed) {
+          const long long at = p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
+          restore<T>(p, w, row_mask(p, w, p.tree_mask[w.q0 + i], at), at, head,
                      direct ? dst : nullptr, direct ? nullptr : acc, d0, d1);
+        }
         if (live && (pair || u == 0)) {
           if (!direct) {
             reinterpret_cast<float2*>(p.part_ml)[part * kTreeRows + r] = make_float2(m, l);
@@ -849,21 +887,32 @@ tree_merge_kernel(const TreeParams p, const TreeMerge* merges) {
     num[2] += a.z * f;
     num[3] += a.w * f;
   }
-  const RowEnd e = row_end(p.sinks, h, m, den);
+  const RowEnd e = row_end(p.sinks ? p.sinks[h] : -INFINITY, m, den);
   T* o = static_cast<T*>(p.out) + (long long)(g.q0 + i) * p.o_st + (long long)h * p.o_sh + d;
   *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(num[0] * e.scale, num[1] * e.scale),
                                             pack2<T>(num[2] * e.scale, num[3] * e.scale));
   if (p.lse && d == 0) p.lse[(long long)(g.q0 + i) * p.num_q_heads + h] = e.lse;
 }
 
+template <typename T, int D, bool WIN>
+int launch_items(const TreeParams& p, int n_ctas, cudaStream_t s) {
+  using C = TreeCfg<D>;
+  if (cudaFuncSetAttribute(tree_attention_kernel<T, D, WIN>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+    return AKV_ERR_CUDA;
+  tree_attention_kernel<T, D, WIN><<<n_ctas, C::kThreads, C::kSmem, s>>>(p);
+  return AKV_OK;
+}
+
 template <typename T, int D>
 int launch_tree(const TreeParams& p, int n_ctas, const TreeMerge* merges, int n_merges,
                 cudaStream_t s) {
-  using C = TreeCfg<D>;
-  if (cudaFuncSetAttribute(tree_attention_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           C::kSmem) != cudaSuccess)
-    return AKV_ERR_CUDA;
-  tree_attention_kernel<T, D><<<n_ctas, C::kThreads, C::kSmem, s>>>(p);
+  // With a window, tiles that no row loses a key of take the ordinary way: 128
+  // requests of 2,040 keys and 8 tokens 160 us (all tiles searched and masked: 255,
+  // without a window 144).  In one kernel that costs the others 4 to 9 %.
+  const int status = p.window >= 0 ? launch_items<T, D, true>(p, n_ctas, s)
+                                   : launch_items<T, D, false>(p, n_ctas, s);
+  if (status != AKV_OK) return status;
   if (n_merges > 0 &&
       launch_pdl(tree_merge_kernel<T, D>, dim3(n_merges, kTreeUnits * kTreeRows / merge_rows<D>()),
                  dim3(kMergeThreads), 0, s, p, merges) != cudaSuccess)

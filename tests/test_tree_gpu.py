@@ -216,6 +216,47 @@ def test_masked_keys_may_hold_anything(d, bad, window):
             assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("group", [8, 5])
+@pytest.mark.parametrize("shuffled", [False, True])
+def test_windows_over_many_tiles(d, group, shuffled):
+    """Tiles wholly inside, wholly outside and across the windows, also with
+    positions that do not rise along the row, and tokens far apart."""
+    c = make([1500, 900, 128, 2000], [16, 33, 4, 64], 3, group, d, torch.float16, seed=9, window=1300,
+             sinks=True)
+    if shuffled:
+        g = torch.Generator(device="cuda").manual_seed(3)
+        c["kpos"] = c["kpos"][torch.randperm(len(c["kpos"]), generator=g, device="cuda")].contiguous()
+        c["qpos"] = c["qpos"] + 150 * (torch.arange(len(c["qpos"]), device="cuda") % 3).int()
+    check(c)
+    check(c, ctas=5)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_bad_values_inside_and_outside_long_windows(d, bad):
+    """One bad V element at a key that every row sees, that some rows see and
+    that none sees, each in a tile of its own: it changes that element of the
+    rows that see it and nothing else."""
+    c = make([1000, 300], [16, 5], 2, 8, d, torch.bfloat16, seed=10, window=700)
+    c["qpos"][:16] = int(c["kpos"][999]) + 1 + 40 * torch.arange(16, device="cuda").int()
+    attn = attention(c)
+    clean, clean_lse = launch(c, attn, return_lse=True)
+    seen_by = lambda j: c["qpos"][:16] - c["kpos"][j] <= 700  # noqa: E731
+    counts = torch.stack([seen_by(j).sum() for j in range(1000)])
+    for keys in ((counts == 16), (counts > 0) & (counts < 16), (counts == 0)):
+        j = int(torch.nonzero(keys).flatten()[int(keys.sum()) // 2])
+        v = c["v"].clone()
+        v[int(c["indices"][j]), 1, 7] = bad
+        out, lse = launch({**c, "v": v}, attn, return_lse=True)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        hit[:16][seen_by(j), 8:, 7] = True
+        assert torch.equal(lse, clean_lse) and torch.equal(out[~hit], clean[~hit])
+        want = torch.full_like(out, bad)
+        assert torch.equal(out[hit].isnan(), want[hit].isnan())
+        assert torch.equal(out[hit].nan_to_num(0.5), want[hit].nan_to_num(0.5))
+
+
 def test_one_infinite_element_of_a_visible_key():
     c = make([70], [3], 2, 8, 64, torch.bfloat16, seed=6)
     c["mask"].copy_(torch.tensor([1, 3, 5]))
