@@ -23,11 +23,13 @@
 // table entry, so one launch with two dependent load rounds is the floor.
 // Every block therefore sums the whole batch's lengths itself (a batch is a
 // few hundred loads from L2) instead of waiting for a scan kernel.  Measured
-// (device time, replayed from a graph): one request 6.4 us; 64 requests over
-// 16-slot pages with block tables 8.2 us; 512 requests of 0-64 drafted tokens
-// with block tables of 4.2M entries (33.8 MB) 15.5 us, of which the tables 7;
-// more blocks per request cost more sums than they save (19.9 us at two, 28
-// at four).
+// (device time, calls one after another in a graph): one request 4.2 us; 64
+// requests over 16-slot pages with block tables 5.4 us; 512 requests of 0-64
+// drafted tokens with block tables of 4.2M entries (33.8 MB) 14.9 us, of which the
+// tables about 8 (20.8 us with 4-byte copies; eight 16-byte loads in flight
+// instead of four, or blocks of 512 threads, 20 us: then not all blocks are
+// resident).  More blocks per request cost more sums than they save (4-byte
+// copies: 15.5 us at one block, 19.9 at two, 28 at four).
 
 #include <algorithm>
 
@@ -247,8 +249,25 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
   if (a.block_table != nullptr && give && !me.bad) {
     int32_t* out = a.block_table + (long long)b * a.table_stride;
     const int old = (int)old_pages, pages = (int)(old_pages + me.need);
-    // Four entries at a time, their loads all before the first store.
     int g = start;
+    // Pages of one slot are a copy: 16 bytes a load where both rows allow it.
+    if (a.shift == 0 &&
+        ((reinterpret_cast<uintptr_t>(row) | reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
+      const int4* from = reinterpret_cast<const int4*>(row);
+      int4* to = reinterpret_cast<int4*>(out);
+      const int quads = old >> 2;
+      int i = start;
+      for (; i + 3 * step < quads; i += 4 * step) {
+        int4 id[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) id[k] = from[i + k * step];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to[i + k * step] = id[k];
+      }
+      for (; i < quads; i += step) to[i] = from[i];
+      g += 4 * quads;
+    }
+    // Four entries at a time, their loads all before the first store.
     for (; g + 3 * step < old; g += 4 * step) {
       int id[4];
 #pragma unroll

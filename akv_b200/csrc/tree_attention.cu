@@ -310,17 +310,19 @@ __device__ __forceinline__ void restore(const TreeParams& p, const TreeItem& w,
 
 // Warps 0-3 and 4-7 are the softmax of units 0 and 1 (warp w: rows 32 (w % 4)
 // .., one row per thread), 8-11 the producers, 12 and 13 the MMA issuers, one
-// per unit so that units never wait for one another.  A pair item gives the units different heads or row tiles over
-// the same keys; a single one gives both the same rows and alternate key
-// tiles, and its accumulators are joined out of tensor memory at the end.
+// per unit so that units never wait for one another.  A pair item gives the
+// units different heads or row tiles over the same keys; a single one gives both
+// the same rows and alternate key tiles, and its accumulators are joined out of
+// tensor memory at the end.
 // Barriers.  Per slot: full (every producer thread's copies have landed),
 // empty (the products of both units that read it are done; the unit that
 // reads a single item's slot signals twice).  Per unit: q (its Q tile is
 // stored), s (scores done), f (head_dim 64: the scores are read, so the
 // next product may overwrite them while P is made), p (P stored), o (P.V
-// done), d (all of it done, at the end).  x: the units meet around the join.  A waiter is never two phases
-// behind: S(c + 1) needs f(c) or o(c), P(c + 1) is stored after o(c).  Waits are
-// bounded; once one runs out the CTA's abort flag ends every role's loop and
+// done), d (all of it done, at the end).  x: the units meet around the join.  A
+// waiter is never two phases behind: S(c + 1) needs f(c) or o(c), P(c + 1) is
+// stored after o(c), and Q of an item is sent after the last o before it.  Waits
+// are bounded; once one runs out the CTA's abort flag ends every role's loop and
 // *error_flag gets bit 2.
 template <typename T, int D, bool WIN>
 __global__ void __launch_bounds__(TreeCfg<D>::kThreads, 1)

@@ -71,7 +71,7 @@ def expected(c):
                 masks=np.array(masks, np.uint64).view(np.int64), pages=at - c["head"])
 
 
-def launch(c, *, commit=True, capacity=None, mapper=None, lens64=True, dev="cuda"):
+def launch(c, *, commit=True, capacity=None, mapper=None, lens64=True, dev="cuda", lay=lambda x: x):
     from akv_b200.context_drop import FreeSlotRing
     from akv_b200.context_slots import SlotMapper
 
@@ -82,7 +82,7 @@ def launch(c, *, commit=True, capacity=None, mapper=None, lens64=True, dev="cuda
     ring.ring.copy_(torch.from_numpy(c["ring"]))
     ring.state.copy_(torch.tensor([c["head"], c["tail"]]))
     index = torch.int64 if lens64 else torch.int32
-    t = dict(rows=torch.from_numpy(c["rows"]).to(dev),
+    t = dict(rows=lay(torch.from_numpy(c["rows"]).to(dev)),
              row_ids=torch.from_numpy(c["row_ids"]).to(dev, index),
              cached=torch.from_numpy(c["cached"]).to(dev, index),
              new=torch.from_numpy(c["new"]).to(dev, index),
@@ -91,7 +91,7 @@ def launch(c, *, commit=True, capacity=None, mapper=None, lens64=True, dev="cuda
     if parents is not None:
         parents = np.concatenate((parents, np.zeros(max(0, capacity - len(parents)), np.int32)))
         parents = torch.from_numpy(parents).to(dev)
-    t["table"] = None if c["table"] is None else torch.from_numpy(c["table"]).to(dev)
+    t["table"] = None if c["table"] is None else lay(torch.from_numpy(c["table"]).to(dev))
     view = mapper.run(t["rows"], t["row_ids"], t["cached"], t["new"], ring,
                       next_positions=t["next"], parents=parents, block_table=t["table"],
                       commit=commit)
@@ -134,6 +134,28 @@ def test_slot_map_batches(batch):
     rng = np.random.default_rng(batch)
     c = case(rng, rng.integers(0, 90, batch), rng.integers(0, 65, batch), 16, tree=True, table=True)
     check(c, *launch(c), True)
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 4])
+@pytest.mark.parametrize("pad", [0, 1, 3, 4])
+def test_long_block_tables_at_any_alignment(offset, pad):
+    """Pages of one slot: rows that may be copied 16 bytes at a time and rows
+    that may not, some of each in one call."""
+    rng = np.random.default_rng(8 * offset + pad)
+    c = case(rng, [4096, 4099, 0, 3, 5000, 1022, 12288], [1, 9, 5, 2, 64, 0, 33], 1, tree=True, table=True)
+
+    def lay(x):
+        n, m = x.shape
+        wide = torch.full((n, m + offset + pad), -7, dtype=x.dtype, device=x.device)
+        wide[:, offset: offset + m] = x
+        return wide[:, offset: offset + m]
+
+    view, t = launch(c, lay=lay)
+    check(c, view, t, True)
+    for x in (t["rows"], t["table"]):
+        edge = torch.as_strided(x, (x.shape[0], offset), (x.stride(0), 1),
+                                x.storage_offset() - offset)
+        assert bool((edge == -7).all())
 
 
 def test_slot_map_prompt_chunks():
