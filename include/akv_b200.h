@@ -844,6 +844,7 @@ int akv_qk_norm_rope(const akv_qk_norm_rope_args* args, void* stream);
  * with an item that reaches past them does nothing.  error_flag: DEVICE int32 or NULL,
  * collects 1 (a slot outside the pools, read as slot 0), 2 (a wait ran out: the
  * launch's output is invalid) and 4 (an item past tokens or keys).
+ * sm_scale is positive and, times log2(e), finite in fp32.  out may be q.
  */
 int32_t akv_tree_attention_units(void);
 typedef struct akv_tree_attention_args {

@@ -119,6 +119,29 @@ def test_wrappers_refuse_cpu_tensors():
         qk_norm_rope(x, x, torch.zeros(2, dtype=torch.int32), torch.zeros(4, 64))
 
 
+def test_fields_of_tensors_and_what_they_refuse():
+    import torch
+
+    from akv_b200 import _native
+
+    a = torch.zeros(5, 6, dtype=torch.int32)
+    b = torch.zeros(7, 8, dtype=torch.bfloat16)[::2, 1:]
+    got = _native.fields(2, a, b)
+    assert got == (a.data_ptr(), -1, _native.INT32, 5, 6, 6, 1,
+                   b.data_ptr(), -1, got[9], 4, 7, 16, 1)
+    assert _native.FIELD_CODE[got[9]] == _native.AKV_BF16 and _native.fields(2) == ()
+    codes = [_native.fields(1, torch.zeros(1, dtype=t))[2]
+             for t in (torch.int64, torch.float16, torch.float32)]
+    assert codes[0] == _native.INT64
+    assert [_native.FIELD_CODE[c] for c in codes[1:]] == [_native.AKV_F16, _native.AKV_F32]
+    sparse = torch.zeros(2, 2).to_sparse()
+    for bad in ((), (-1,), (9,), (2, [1]), (2, None), (1, a), (3, a), (2, a, 5), (2, sparse)):
+        with pytest.raises(ValueError):
+            _native.fields(*bad)
+    with pytest.raises(TypeError):
+        _native.fields("2", a)
+
+
 def tree_args(**change):
     a = dict(q=BUF, q_st=512, q_sh=64, k=BUF, v=BUF, k_ss=128, k_sh=64, v_ss=128, v_sh=64, slots=8,
              dtype=1, tokens=8, keys=8, indices=BUF, draft=BUF, mask=BUF, qpos=None, kpos=None, window=-1, sinks=None,
