@@ -32,9 +32,9 @@ class SlotMap:
     [new_offsets[b], new_offsets[b + 1])."""
 
     new_offsets: torch.Tensor   # int32 [batch + 1]
-    slots: torch.Tensor         # int32 [max_new_tokens]; -1: none given out
-    positions: torch.Tensor     # int32 [max_new_tokens]
-    tree_mask: torch.Tensor | None  # int64 [max_new_tokens], with parents
+    slots: torch.Tensor         # int32 [max_new_tokens]; -1: none given out, or behind the last token
+    positions: torch.Tensor     # int32 [max_new_tokens]; 0 behind the last token
+    tree_mask: torch.Tensor | None  # int64 [max_new_tokens], with parents; not written behind them
     block_table: torch.Tensor | None
     totals: torch.Tensor        # int32 [2]: new tokens, pages taken or lent
     status: torch.Tensor        # int32 [1]: AKV_SLOTS_* bits
@@ -81,6 +81,7 @@ class SlotMapper:
 
         self._offsets = vector(self.max_batch + 1)
         self._slots, self._positions = vector(self.max_new_tokens), vector(self.max_new_tokens)
+        self._slots.fill_(-1)
         self._mask = vector(self.max_new_tokens, torch.int64)
         self._totals, self._status, self._work = vector(2), vector(1), vector(2)
         self._outputs = tuple(t.data_ptr() for t in (self._offsets, self._slots, self._positions,
@@ -146,7 +147,8 @@ class SlotMapper:
                          self._mask if parents is not None else None, block_table, self._totals,
                          self._status)
         if batch == 0:
-            for t in (result.new_offsets, result.totals, result.status):
+            self._slots.fill_(-1)
+            for t in (self._positions, result.new_offsets, result.totals, result.status):
                 t.zero_()
             return result
         status = _native.launch(index, _native.lib.akv_map_slots, _native.MAP_SLOTS.pack(

@@ -244,6 +244,18 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
     }
   }
 
+  // Behind the last token no slot and no position of an earlier call stays: a
+  // caller may pass the whole vectors on with padded rows.  Entries that hold
+  // neither are left as they are.
+  {
+    const long long stride = (long long)gridDim.y * step;
+    for (long long i = (long long)s.all_fresh + (long long)b * step + start; i < a.capacity;
+         i += stride) {
+      if (a.slots[i] >= 0) a.slots[i] = -1;
+      if (a.positions[i] > 0) a.positions[i] = 0;
+    }
+  }
+
   // Block table: the pages of [0, L) from the row, the fresh ones from the
   // ring (the row's new columns are being written by this launch).
   if (a.block_table != nullptr && give && !me.bad) {

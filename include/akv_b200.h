@@ -689,7 +689,9 @@ int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chun
  * ancestors j (token numbers of the request).  parents: int32, -1 for a root,
  * otherwise an earlier token of the request; at most 64 new tokens per
  * request.  A position is next_positions[b] (NULL: raw_lens[b]) plus the
- * token's depth in the tree, or its number without one.  block_table (NULL:
+ * token's depth in the tree, or its number without one.  Behind the last new
+ * token no slot or position of an earlier call stays: slots >= 0 become -1,
+ * positions > 0 become 0 (tree_mask is not written there).  block_table (NULL:
  * none) int32 [batch, table_columns]: the page ids of the row's pages, the new
  * ones included; entries behind a request's last page are left as they
  * were.  It describes whole rows: tokens dropped from a row are not left out.

@@ -1,0 +1,110 @@
+"""Slot maps at the edges of the mapper's contract: entries behind the last
+token, rows that cannot go on, requests that are not in order."""
+
+import pytest
+import torch
+
+from test_slots_gpu import CODES
+
+pytestmark = pytest.mark.gpu
+
+
+def test_no_slot_of_another_call_is_left_behind_the_last_token():
+    """A mapper larger than its batch: what follows the last token holds no
+    slot and no position, on a first call, after a larger call that took its
+    pages, eager and replayed, in a refused call and in one of no request."""
+    from akv_b200.context_drop import FreeSlotRing
+    from akv_b200.context_slots import SlotMapper
+
+    ring = FreeSlotRing(torch.arange(10, 74), device="cuda")
+    rows = torch.zeros(2, 64, dtype=torch.int32, device="cuda")
+    ids, none = torch.tensor([0, 1], device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
+    lens = torch.zeros(2, dtype=torch.int64, device="cuda")
+    mapper = SlotMapper(2, 16, "cuda")
+
+    def run(new, commit=True):
+        view = mapper.run(rows, ids, lens, new, ring, commit=commit)
+        return view
+
+    def tail_is_free(view, n):
+        assert int((view.slots >= 0).sum()) == n and bool((view.slots[:n] >= 0).all())
+        assert view.slots[n:].tolist() == [-1] * (16 - n)
+        assert view.positions[n:].tolist() == [0] * (16 - n)
+
+    few, many = torch.tensor([1, 2], device="cuda"), torch.tensor([9, 7], device="cuda")
+    tail_is_free(run(few, commit=False), 3)
+    tail_is_free(run(many), 16)
+    lens += many
+    tail_is_free(run(few), 3)
+    lens += few
+    tail_is_free(run(many, commit=False), 16)
+    new = few.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        view = run(new, commit=False)
+    for n in ([9, 7], [1, 0], [0, 0], [3, 3]):
+        new.copy_(torch.tensor(n, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        tail_is_free(view, sum(n))
+    ring.state[0] = ring.state[1]       # no page is free
+    refused = run(few)
+    assert int(refused.status) == CODES["underflow"]
+    assert refused.slots.tolist() == [-1] * 16 and refused.positions[3:].tolist() == [0] * 13
+    ring.state[0] -= 32
+    tail_is_free(run(many, commit=False), 16)
+    tail_is_free(mapper.run(rows, none, none, none, ring), 0)
+
+
+def test_padded_rows_behind_the_last_token_are_not_stored():
+    """The whole of the mapper's vectors with padded projections, as a step of
+    a fixed size passes them: no row of the pools changes but the new tokens'."""
+    from akv_b200.context_drop import FreeSlotRing
+    from akv_b200.context_rope import qk_norm_rope
+    from akv_b200.context_slots import SlotMapper
+
+    ring = FreeSlotRing(torch.arange(5, 69), device="cuda")
+    rows = torch.zeros(2, 64, dtype=torch.int32, device="cuda")
+    ids, lens = torch.tensor([1, 0], device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    mapper = SlotMapper(2, 16, "cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pools = [torch.randn(80, 2, 64, generator=g, device="cuda").half() for _ in range(2)]
+    q, k, v = (torch.randn(16, h, 64, generator=g, device="cuda").half() for h in (4, 2, 2))
+    table = torch.randn(100, 64, generator=g, device="cuda")
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    new = torch.zeros(2, dtype=torch.int64, device="cuda")
+
+    def step():
+        view = mapper.run(rows, ids, lens, new, ring)
+        qk_norm_rope(q, k, view.positions, table, v=v, k_pool=pools[0], v_pool=pools[1],
+                     slots=view.slots, error_flag=flag)
+        return view
+
+    def check(n):
+        before = [p.clone() for p in pools]
+        new.copy_(torch.tensor(n, device="cuda"))
+        yield
+        at = view.slots[: sum(n)].long()
+        assert int(flag) == 0 and len(set(at.tolist())) == sum(n)
+        assert torch.equal(pools[1][at], v[: sum(n)])
+        rest = torch.ones(80, dtype=torch.bool, device="cuda")
+        rest[at] = False
+        for pool, old in zip(pools, before):
+            assert torch.equal(pool[rest], old[rest])
+        lens.add_(new)
+
+    for n in ([1, 2], [9, 7], [1, 0], [2, 2]):
+        run = check(n)
+        next(run)
+        view = step()
+        next(run, None)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        view = step()
+    for n in ([8, 7], [2, 1], [0, 0], [3, 1]):
+        run = check(n)
+        next(run)
+        graph.replay()
+        next(run, None)
