@@ -52,7 +52,7 @@ struct SlotArgs {
   int new_lens_is64;
   int batch;
   int shift;  // log2(page size)
-  const int32_t* ring;
+  int32_t* ring;
   long long* ring_state;
   int64_t ring_capacity;
   const void* next_positions;  // null: the row length
@@ -91,6 +91,51 @@ __device__ __forceinline__ Request load_request(const SlotArgs& a, int b) {
   const long long up = (1ll << a.shift) - 1;
   r.need = r.bad ? 0 : ((end + up) >> a.shift) - ((r.len + up) >> a.shift);
   return r;
+}
+
+// A row ends inside a page whose last slot is not at its offset: it cannot go on.
+__device__ __forceinline__ bool off_page(int last, long long len, int p_mask) {
+  return last < 0 || (last & p_mask) != ((len - 1) & p_mask);
+}
+
+// Pages counted for requests that off_page stopped, which no row holds: moves
+// them in the ring behind those that were given out, entries [head, head +
+// taken), where they are the first free ones once the head has passed the
+// others.  Returns their number.  One warp, after every block has read its
+// pages.  From the last to the first, so that an entry is read before one of a
+// later request, which never lies before it, takes its place.
+__device__ long long return_pages(const SlotArgs& a, long long head, long long taken, int lane) {
+  const int p_mask = (1 << a.shift) - 1;
+  auto entry = [&](long long at) { return a.ring + (head + at) % a.ring_capacity; };
+  long long end = taken, to = taken;  // pages before which request's; next free place
+  for (int i0 = (a.batch - 1) / 32 * 32; i0 >= 0; i0 -= 32) {
+    long long need = 0;
+    bool lost = false;
+    if (i0 + lane < a.batch) {
+      const Request r = load_request(a, i0 + lane);
+      need = r.need;
+      lost = need > 0 && (r.len & p_mask) != 0 &&
+             off_page(a.req_to_token[r.row * a.row_stride + r.len - 1], r.len, p_mask);
+    }
+    const long long upto = warp_inclusive_scan(need);
+    const long long all = __shfl_sync(0xffffffffu, upto, 31);
+    for (unsigned left = __ballot_sync(0xffffffffu, lost); left;) {
+      const int src = 31 - __clz(left);
+      left ^= 1u << src;
+      const long long n = __shfl_sync(0xffffffffu, need, src);
+      const long long from = end - all + __shfl_sync(0xffffffffu, upto, src) - n;
+      for (long long k = n; k > 0; k -= 32) {  // 32 entries, the last ones first
+        const long long at = k - 1 - lane;
+        const int page = at >= 0 ? *entry(from + at) : 0;
+        __syncwarp();
+        if (at >= 0) *entry(to - n + at) = page;
+        __syncwarp();
+      }
+      to -= n;
+    }
+    end -= all;
+  }
+  return taken - to;
 }
 
 // Sums of one block over the batch, valid in every thread afterwards.
@@ -155,7 +200,7 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
   const bool over = (long long)s.all_fresh > a.capacity;
   const bool refused = short_ring || over;  // of the whole call: no slot is given out
   // A row whose last slot does not sit at its offset of a page cannot go on.
-  const bool bad_page = partial && (last < 0 || (last & p_mask) != ((me.len - 1) & p_mask));
+  const bool bad_page = partial && off_page(last, me.len, p_mask);
   const bool give = !refused && !bad_page;
   int st = 0;
   if (me.bad) st |= AKV_SLOTS_BAD_REQUEST;
@@ -303,15 +348,28 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
   }
   // Status bits gather in arrivals[1] and the last block publishes them (so
   // a call leaves its own status, not a sum over calls) and, with commit,
-  // takes the pages: every block has read the ring's head by then.
+  // takes the pages: every block has read the ring by then.
   if (st) atomicOr(a.arrivals + 1, (unsigned)st);
   __syncthreads();
-  if (tid == 0) {
-    __threadfence();
-    const unsigned blocks = gridDim.x * gridDim.y;
-    if (atomicInc(a.arrivals, blocks - 1) == blocks - 1) {
-      *a.status = (int32_t)atomicExch(a.arrivals + 1, 0u);
-      if (a.commit && !refused) a.ring_state[0] = head + (long long)s.all_need;
+  if (warp == 0) {
+    int bits = -1;
+    if (lane == 0) {
+      __threadfence();
+      const unsigned blocks = gridDim.x * gridDim.y;
+      if (atomicInc(a.arrivals, blocks - 1) == blocks - 1)
+        bits = (int)atomicExch(a.arrivals + 1, 0u);
+    }
+    bits = __shfl_sync(0xffffffffu, bits, 0);
+    if (bits < 0) return;  // not the last block
+    long long taken = (long long)s.all_need;
+    if (a.commit && !refused && (bits & AKV_SLOTS_BAD_PAGE)) {
+      __threadfence();
+      taken -= return_pages(a, head, taken, lane);
+      if (lane == 0) a.totals[1] = (int32_t)taken;
+    }
+    if (lane == 0) {
+      *a.status = bits;
+      if (a.commit && !refused) a.ring_state[0] = head + taken;
     }
   }
 }

@@ -700,8 +700,9 @@ int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chun
  * status (int32): AKV_SLOTS_* bits of this call.  RING_UNDERFLOW and CAPACITY
  * refuse the whole call (slots -1; rows, block table and ring untouched);
  * BAD_REQUEST treats that request as one without new tokens; BAD_PAGE leaves
- * that request's slots -1 and its row and block table untouched (its pages
- * count as taken); BAD_PARENT
+ * that request's slots -1 and its row and block table untouched (its pages are
+ * skipped over by the requests behind it; with commit they stay in the ring,
+ * as the next ones to be given out, and totals do not count them); BAD_PARENT
  * makes the token a root.  Two requests of a call must not share a row, unless
  * at most one of them has new tokens.  workspace: DEVICE uint32 [2], zero before the first call and
  * left zero by every call; calls that share it must not overlap.
@@ -719,7 +720,7 @@ typedef struct akv_map_slots_args {
   int64_t new_lens_is64;
   int64_t batch;
   int64_t page_size;
-  const int32_t* ring;
+  int32_t* ring;
   int64_t* ring_state;
   int64_t ring_capacity;
   const void* next_positions;

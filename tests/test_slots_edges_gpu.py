@@ -1,10 +1,11 @@
 """Slot maps at the edges of the mapper's contract: entries behind the last
 token, rows that cannot go on, requests that are not in order."""
 
+import numpy as np
 import pytest
 import torch
 
-from test_slots_gpu import CODES
+from test_slots_gpu import CODES, case, launch
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +109,68 @@ def test_padded_rows_behind_the_last_token_are_not_stored():
         next(run)
         graph.replay()
         next(run, None)
+
+
+@pytest.mark.parametrize("bad_rows", [[0], [1], [2], [0, 2], [0, 1, 2, 3], [3]])
+@pytest.mark.parametrize("page", [4, 16])
+@pytest.mark.parametrize("full", [False, True])
+def test_pages_of_a_row_with_a_bad_end_are_not_lost(bad_rows, page, full):
+    """The ring's head moves by the pages that rows hold, and what is left in
+    the ring with what was given out is what it held before, each page once."""
+    rng = np.random.default_rng(page)
+    n_new = 3 * page + 1
+    c = case(rng, [page + 1, 2, 3 * page + 2, 1], [n_new] * 4, page, table=True)
+    if full:                                   # every entry of the ring is a free page
+        assert c["tail"] - c["head"] == len(c["ring"])
+    else:
+        c["ring"] = np.concatenate((c["ring"][c["head"] % len(c["ring"]):],
+                                    c["ring"][: c["head"] % len(c["ring"])], np.full(5, 1 << 20, np.int32)))
+        c["tail"] -= c["head"]
+        c["head"] = 0
+    for b in bad_rows:
+        r, end = c["row_ids"][b], c["cached"][b] - 1
+        c["rows"][r, end] += 1
+    size = len(c["ring"])
+    before = [int(c["ring"][i % size]) for i in range(c["head"], c["tail"])]
+    view, t = launch(c)
+    assert int(view.status.item()) == CODES["page"]
+    head, tail = t["ring"].state.tolist()
+    left = [int(t["ring"].ring[i % size]) for i in range(head, tail)]
+    slots, offsets = view.slots.tolist(), view.new_offsets.tolist()
+    given = []
+    for b in range(4):
+        mine = slots[offsets[b]: offsets[b + 1]]
+        assert len(mine) == n_new
+        if b in bad_rows:
+            assert mine == [-1] * n_new
+        else:
+            fresh = [s // page for i, s in enumerate(mine) if (c["cached"][b] + i) % page == 0]
+            given += fresh
+            assert t["rows"][c["row_ids"][b], c["cached"][b]: c["cached"][b] + n_new].tolist() == mine
+    assert tail == c["tail"] and head - c["head"] == len(given) == int(view.totals[1])
+    assert sorted(left + given) == sorted(before) and len(set(before)) == len(before)
+    view, t = launch(c, commit=False)          # lent: the ring is as it was
+    assert t["ring"].state.tolist() == [c["head"], c["tail"]]
+    np.testing.assert_array_equal(t["ring"].ring.cpu().numpy(), c["ring"])
+
+
+def test_pages_of_many_rows_with_bad_ends_are_not_lost():
+    rng = np.random.default_rng(12)
+    batch, page = 700, 4
+    c = case(rng, rng.integers(0, 30, batch), rng.integers(0, 30, batch), page)
+    ends = [b for b in range(batch) if c["cached"][b] % page and rng.random() < 0.4]
+    for b in ends:
+        c["rows"][c["row_ids"][b], c["cached"][b] - 1] += 1
+    size = len(c["ring"])
+    before = sorted(int(c["ring"][i % size]) for i in range(c["head"], c["tail"]))
+    view, t = launch(c)
+    assert int(view.status.item()) == CODES["page"]
+    head, tail = t["ring"].state.tolist()
+    ring = t["ring"].ring.cpu().numpy()
+    left = [int(ring[i % size]) for i in range(head, tail)]
+    rows, given = t["rows"].cpu().numpy(), []
+    for b in range(batch):
+        for i in range(c["cached"][b], c["cached"][b] + c["new"][b]):
+            if b not in ends and i % page == 0:
+                given.append(int(rows[c["row_ids"][b], i]) // page)
+    assert sorted(left + given) == before and int(view.totals[1]) == len(given)
