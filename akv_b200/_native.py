@@ -24,6 +24,7 @@ DROP_BAD_PAGE = 16
 REPOSITION_BULK_V = 1
 SLOTS_RING_UNDERFLOW, SLOTS_CAPACITY, SLOTS_BAD_REQUEST = 1, 2, 4
 SLOTS_BAD_PAGE, SLOTS_BAD_PARENT = 8, 16
+SLOTS_KEEP_OFFSETS = 1 << 32
 
 DTYPE_CODE = {torch.float16: AKV_F16, torch.bfloat16: AKV_BF16, torch.float32: AKV_F32}
 

@@ -89,7 +89,7 @@ class SlotMapper:
         self._words = tuple(t.data_ptr() for t in (self._totals, self._status, self._work))
 
     def run(self, req_to_token, row_ids, raw_lens, new_lens, ring, *, next_positions=None,
-            parents=None, block_table=None, commit=True) -> SlotMap:
+            parents=None, block_table=None, commit=True, keep_offsets=False) -> SlotMap:
         """``req_to_token`` int32 [rows, columns]; ``row_ids``, ``raw_lens`` (columns
         in use) and ``new_lens`` int32 or int64 [batch]; ``ring`` a
         ``FreeSlotRing`` of page ids (slots at page_size 1).
@@ -100,7 +100,11 @@ class SlotMapper:
         depth.  A row whose last page a Drop has freed (all of its tokens
         dropped) is passed with ``raw_lens`` rounded up to whole pages, or the
         new tokens would go on in that page.  ``block_table``: int32 [>= batch, columns], filled with the
-        page ids of whole rows.  Two requests of one call must not share a
+        page ids of whole rows.  A request whose row or lengths are out of range (one that no longer
+        fits its row, say) counts as one without new tokens, and the entries of those behind it
+        move up; with ``keep_offsets`` it keeps its entries, without slots, which is what tokens
+        need that are laid out by the caller's own lengths (a length that is itself out of range
+        then refuses the call).  Two requests of one call must not share a
         row, unless at most one of them has new tokens.  Failures that only
         the device sees are bits of ``status`` (``SlotMap.check``)."""
         index = self._index
@@ -156,6 +160,7 @@ class SlotMapper:
             1 if raw_dt == _INT64 else 0, new_ptr, 1 if new_dt == _INT64 else 0, batch,
             self.page_size, free_ptr, state_ptr, ring.capacity, next_ptr, next64, parents_ptr,
             self.max_new_tokens, *self._outputs, table_ptr, table_stride, table_columns,
-            *self._words, 1 if commit else 0))
+            *self._words,
+            (1 if commit else 0) + (_native.SLOTS_KEEP_OFFSETS if keep_offsets else 0)))
         _native.check(status, "map_slots")
         return result

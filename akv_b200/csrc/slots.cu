@@ -69,11 +69,12 @@ struct SlotArgs {
   int32_t* status;
   unsigned* arrivals;
   int commit;
+  int keep;  // a bad request keeps its entries of the outputs
 };
 
 struct Request {
   long long len, fresh, row, need;
-  bool bad;
+  bool bad, unsized;  // unsized: bad, and its length leaves no room to keep
 };
 
 __device__ __forceinline__ Request load_request(const SlotArgs& a, int b) {
@@ -82,12 +83,13 @@ __device__ __forceinline__ Request load_request(const SlotArgs& a, int b) {
   r.len = ld_index(a.raw_lens, b, a.raw_lens_is64);
   r.fresh = ld_index(a.new_lens, b, a.new_lens_is64);
   const long long end = r.len + r.fresh;
-  // A bad request takes part as one without new tokens.
-  r.bad = r.row < 0 || r.row >= a.rows || r.len < 0 || r.fresh < 0 || r.len > a.columns ||
-          r.fresh > a.columns || end > a.columns ||
-          (a.parents != nullptr && r.fresh > kTreeNodes) ||
+  r.unsized = r.fresh < 0 || r.fresh > a.columns || (a.parents != nullptr && r.fresh > kTreeNodes);
+  r.bad = r.unsized || r.row < 0 || r.row >= a.rows || r.len < 0 || r.len > a.columns ||
+          end > a.columns ||
           (a.block_table != nullptr && ((end - 1) >> a.shift) >= a.table_columns);
-  if (r.bad) r.fresh = 0;
+  // A bad request takes part as one without new tokens, or (keep) as one whose
+  // tokens take no page.
+  if (r.bad && (r.unsized || !a.keep)) r.fresh = 0;
   const long long up = (1ll << a.shift) - 1;
   r.need = r.bad ? 0 : ((end + up) >> a.shift) - ((r.len + up) >> a.shift);
   return r;
@@ -145,7 +147,6 @@ struct Sums {
 
 __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs a) {
   __shared__ unsigned long long s_sum[4][kSlotThreads / 32];
-  __shared__ int s_bad;
   __shared__ long long s_ring[3];
   const int b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -157,14 +158,12 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
   const bool partial = !me.bad && (me.len & p_mask) != 0;
   const int last = partial ? row[me.len - 1] : 0;
   if (tid == 0) {
-    s_bad = 0;
     s_ring[0] = a.ring_state[0];
     s_ring[1] = a.ring_state[1];
     s_ring[2] = s_ring[0] % a.ring_capacity;
   }
-  __syncthreads();
   Sums s = {0, 0, 0, 0};
-  bool bad = false;
+  bool unsized = false;
   for (int i = tid; i < a.batch; i += kSlotThreads) {
     const Request r = load_request(a, i);
     s.all_need += r.need;
@@ -173,9 +172,8 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
       s.need += r.need;
       s.fresh += r.fresh;
     }
-    bad |= r.bad;
+    unsized |= r.unsized;
   }
-  if (bad) s_bad = 1;
   s.need = warp_sum(s.need);
   s.fresh = warp_sum(s.fresh);
   s.all_need = warp_sum(s.all_need);
@@ -186,7 +184,7 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
     s_sum[2][warp] = s.all_need;
     s_sum[3][warp] = s.all_fresh;
   }
-  __syncthreads();
+  unsized = __syncthreads_or(unsized) && a.keep;
   s = Sums{0, 0, 0, 0};
 #pragma unroll
   for (int w = 0; w < kSlotThreads / 32; ++w) {
@@ -198,10 +196,11 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
   const long long head = s_ring[0];
   const bool short_ring = (long long)s.all_need > s_ring[1] - head;
   const bool over = (long long)s.all_fresh > a.capacity;
-  const bool refused = short_ring || over;  // of the whole call: no slot is given out
+  const bool none = over || unsized;            // the outputs list no token
+  const bool refused = short_ring || none;  // of the whole call: no slot is given out
   // A row whose last slot does not sit at its offset of a page cannot go on.
   const bool bad_page = partial && off_page(last, me.len, p_mask);
-  const bool give = !refused && !bad_page;
+  const bool give = !refused && !bad_page && !me.bad;
   int st = 0;
   if (me.bad) st |= AKV_SLOTS_BAD_REQUEST;
   if (bad_page) st |= AKV_SLOTS_BAD_PAGE;
@@ -214,7 +213,9 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
     return a.ring[at < a.ring_capacity ? at : at - a.ring_capacity];
   };
   const int start = blockIdx.x * kSlotThreads + tid, step = gridDim.x * kSlotThreads;
-  const long long next = a.next_positions ? ld_index(a.next_positions, b, a.next_is64) : me.len;
+  const long long next = me.bad ? 0  // no position to go on from
+                         : a.next_positions ? ld_index(a.next_positions, b, a.next_is64)
+                                            : me.len;
   const long long out0 = (long long)s.fresh;
 
   // New tokens.  With a tree they are one warp's work (64 nodes at most, two
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
 
   // Block table: the pages of [0, L) from the row, the fresh ones from the
   // ring (the row's new columns are being written by this launch).
-  if (a.block_table != nullptr && give && !me.bad) {
+  if (a.block_table != nullptr && give) {
     int32_t* out = a.block_table + (long long)b * a.table_stride;
     const int old = (int)old_pages, pages = (int)(old_pages + me.need);
     int g = start;
@@ -337,10 +338,10 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
   }
 
   if (blockIdx.x == 0 && tid == 0) {
-    a.new_offsets[b] = (int32_t)(over ? 0 : s.fresh);
+    a.new_offsets[b] = (int32_t)(none ? 0 : s.fresh);
     if (b == a.batch - 1) {
-      a.new_offsets[a.batch] = (int32_t)(over ? 0 : s.all_fresh);
-      a.totals[0] = (int32_t)(over ? 0 : s.all_fresh);
+      a.new_offsets[a.batch] = (int32_t)(none ? 0 : s.all_fresh);
+      a.totals[0] = (int32_t)(none ? 0 : s.all_fresh);
       a.totals[1] = (int32_t)(refused ? 0 : s.all_need);
       if (short_ring) st |= AKV_SLOTS_RING_UNDERFLOW;
       if (over) st |= AKV_SLOTS_CAPACITY;
@@ -400,12 +401,13 @@ extern "C" int akv_map_slots(const akv_map_slots_args* args, void* stream) {
   int shift = 0;
   while ((1 << shift) < page) ++shift;
   const int batch = (int)x.batch;
+  const bool keep = (x.commit & ~int64_t(1)) == AKV_SLOTS_KEEP_OFFSETS;
   SlotArgs a{x.req_to_token, x.row_stride, x.rows, x.columns, x.row_ids, x.row_ids_is64 != 0,
              x.raw_lens, x.raw_lens_is64 != 0, x.new_lens, x.new_lens_is64 != 0, batch, shift,
              x.ring, reinterpret_cast<long long*>(x.ring_state), x.ring_capacity,
              x.next_positions, x.next_is64 != 0, x.parents, x.capacity, x.new_offsets, x.slots,
              x.positions, x.tree_mask, x.block_table, x.table_stride, x.table_columns, x.totals,
-             x.status, x.workspace, x.commit != 0};
+             x.status, x.workspace, keep ? (int)(x.commit & 1) : x.commit != 0, keep};
   // Blocks per request: enough for about six per SM over the batch, no more
   // than the request's share of tokens or its table row can use.
   const long long longest =

@@ -45,6 +45,8 @@ extern "C" {
 #define AKV_SLOTS_BAD_REQUEST 4    /* a row or a length out of range          */
 #define AKV_SLOTS_BAD_PAGE 8       /* a row's last slot is not at its offset  */
 #define AKV_SLOTS_BAD_PARENT 16    /* a draft node's parent is not before it  */
+/* Added to akv_map_slots's `commit` (0 or 1): a bad request keeps its entries. */
+#define AKV_SLOTS_KEEP_OFFSETS (1ll << 32)
 
 /* Element types. */
 #define AKV_F16 0
@@ -699,7 +701,13 @@ int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chun
  *
  * status (int32): AKV_SLOTS_* bits of this call.  RING_UNDERFLOW and CAPACITY
  * refuse the whole call (slots -1; rows, block table and ring untouched);
- * BAD_REQUEST treats that request as one without new tokens; BAD_PAGE leaves
+ * BAD_REQUEST treats that request as one without new tokens: the entries of
+ * those behind it move up, and tokens that the caller has laid out by its own
+ * lengths no longer match them.  With commit + AKV_SLOTS_KEEP_OFFSETS it keeps
+ * its entries (slots -1, positions from 0, masks of its parents, no pages)
+ * and new_offsets are those of new_lens; a length that leaves no
+ * place for that (negative, past columns, past 64 with parents) refuses the
+ * whole call, with offsets and totals 0.  BAD_PAGE leaves
  * that request's slots -1 and its row and block table untouched (its pages are
  * skipped over by the requests behind it; with commit they stay in the ring,
  * as the next ones to be given out, and totals do not count them); BAD_PARENT

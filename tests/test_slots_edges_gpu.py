@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_slots_gpu import CODES, case, launch
+from test_slots_gpu import CODES, case, check, expected, launch
 
 pytestmark = pytest.mark.gpu
 
@@ -174,3 +174,70 @@ def test_pages_of_many_rows_with_bad_ends_are_not_lost():
             if b not in ends and i % page == 0:
                 given.append(int(rows[c["row_ids"][b], i]) // page)
     assert sorted(left + given) == before and int(view.totals[1]) == len(given)
+
+
+class Kept:
+    """A mapper whose calls keep the offsets of the lengths."""
+
+    def __init__(self, batch, tokens, page):
+        from akv_b200.context_slots import SlotMapper
+
+        self.mapper = SlotMapper(batch, tokens, "cuda", page_size=page)
+
+    def run(self, *args, **kw):
+        return self.mapper.run(*args, keep_offsets=True, **kw)
+
+
+@pytest.mark.parametrize("what", ["row", "negative", "columns", "table"])
+@pytest.mark.parametrize("tree", [False, True])
+def test_kept_offsets_are_those_of_the_lengths(what, tree):
+    """With keep_offsets a bad request keeps its entries, without slots, and the
+    others' slots, parents and masks stay where the caller's tokens are."""
+    rng = np.random.default_rng(13)
+    c = case(rng, [5, 6, 7, 2], [3, 4, 5, 2], 4, tree=tree, table=True)
+    bad = {**c, "row_ids": c["row_ids"].copy(), "cached": c["cached"].copy()}
+    if what == "row":
+        bad["row_ids"][1] = -1
+    elif what == "negative":
+        bad["cached"][1] = -4
+    elif what == "columns":
+        bad["cached"][1] = c["rows"].shape[1] - 1
+    else:
+        c["rows"] = bad["rows"] = np.pad(c["rows"], ((0, 0), (0, 90)), constant_values=-7)
+        bad["cached"][1] = 4 * c["table"].shape[1] - 2
+    view, t = launch(bad, mapper=Kept(4, 14, 4))
+    assert int(view.status.item()) == CODES["request"]
+    assert view.new_offsets.tolist() == [0, 3, 7, 12, 14]
+    # The rules without request 1, whose tokens take no page.
+    rest = {**c, "new": c["new"].copy()}
+    rest["new"][1] = 0
+    if tree:
+        rest["parents"] = np.delete(c["parents"], [3, 4, 5, 6])
+    want = expected(rest)
+    keep = [i for i in range(14) if not 3 <= i < 7]
+    assert view.slots[keep].tolist() == want["slots"]
+    assert view.slots[3:7].tolist() == [-1] * 4
+    assert view.positions[keep].tolist() == want["positions"]
+    assert bool((view.positions[3:7] >= 0).all()) and bool((view.positions[3:7] < 4).all())
+    if tree:
+        assert view.tree_mask[keep].tolist() == want["masks"].tolist()
+    np.testing.assert_array_equal(t["rows"].cpu().numpy(), want["rows"])
+    # Without bad requests both ways are the same.
+    check(c, *launch(c, mapper=Kept(4, 14, 4)), True)
+
+
+@pytest.mark.parametrize("new", [1 << 40, -1, 65])
+def test_kept_offsets_refuse_lengths_that_leave_none(new):
+    rng = np.random.default_rng(14)
+    c = case(rng, [5, 6, 7], [3, 3, 3], 1, tree=True, table=True)
+    c["rows"] = np.pad(c["rows"], ((0, 0), (0, 90)), constant_values=-7)
+    c["table"] = np.pad(c["table"], ((0, 0), (0, 90)), constant_values=-5)
+    bad = {**c, "new": c["new"].copy()}
+    bad["new"][1] = new
+    view, t = launch(bad, capacity=9, mapper=Kept(3, 9, 1))
+    assert int(view.status.item()) == CODES["request"]
+    assert view.new_offsets.tolist() == [0] * 4 and view.totals.tolist() == [0, 0]
+    assert view.slots.tolist() == [-1] * 9
+    np.testing.assert_array_equal(t["rows"].cpu().numpy(), c["rows"])
+    np.testing.assert_array_equal(t["table"].cpu().numpy(), c["table"])
+    assert t["ring"].state.tolist() == [c["head"], c["tail"]]
