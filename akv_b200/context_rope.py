@@ -24,10 +24,10 @@ _WHAT = ("must be [tokens, heads, head_dim] of the type and device of q, with un
 
 
 def _vector(name, t, n, index):
-    """(address, 1 if int64) of a contiguous index vector of n entries."""
+    """(address, 1 if int64) of a contiguous index vector of at least n entries."""
     ptr, dev, dt, size, step = _fields(1, t)
-    if size != n or dev != index or (step != 1 and n > 1) or (dt != _INT32 and dt != _INT64):
-        raise ValueError(f"{name} must be a contiguous int32 or int64 vector of one entry per "
+    if size < n or dev != index or (step != 1 and n > 1) or (dt != _INT32 and dt != _INT64):
+        raise ValueError(f"{name} must be a contiguous int32 or int64 vector of an entry for each "
                          "token on the device of q")
     return ptr, 1 if dt == _INT64 else 0
 
@@ -41,14 +41,15 @@ def qk_norm_rope(q, k, positions, cos_sin_cache, *, q_weight=None, k_weight=None
     last stride 1, the others multiples of 16 bytes (views of a fused
     projection).  D and ``rotary_dim`` (default: the table's width) are
     multiples of 16, D at most 512; dimensions from ``rotary_dim`` on are
-    normed and not rotated.  ``positions``: int32 or int64 [tokens];
-    ``cos_sin_cache`` [max_position, rotary_dim] as ``reposition_kv_layers``.
+    normed and not rotated.  ``positions``: int32 or int64 [>= tokens], as
+    ``slots`` below (a ``SlotMap``'s whole vectors fit); ``cos_sin_cache``
+    [max_position, rotary_dim] as ``reposition_kv_layers``.
 
     ``q_weight`` / ``k_weight``: [D], of q's type or both fp32; without one
     that side is rotated and not normed.  Arithmetic is fp32, rounded once.
 
     With ``k_pool`` / ``v_pool`` [slots, Hkv, D], ``v`` and ``slots`` (int32 or
-    int64 [tokens]), K and V are stored at the tokens' slots; a token with a
+    int64 [>= tokens]), K and V are stored at the tokens' slots; a token with a
     negative slot is padding and is not stored.  ``k_out`` then is written
     only if given; without pools it is allocated.  ``q_out`` may be ``q`` and
     ``k_out`` ``k``; other overlaps are not supported, and two tokens of one
