@@ -10,8 +10,13 @@ token, the row entries, and, where asked, block tables for a paged reader and
 the ancestor masks of drafted token trees for ``context_tree.TreeAttention``.
 
 A verification step lends its pages (``commit=False``): the ring keeps them,
-and the next call gives the same ones out again, so rejected tokens cost
-nothing.  A prompt chunk or a plain decode step takes them (``commit=True``).
+and the next call gives them out again, so rejected tokens cost nothing.  A
+prompt chunk or a plain decode step takes them (``commit=True``).  To take
+what a verification accepted, call again with the accepted counts and
+``commit=True`` and move the accepted tokens' K/V from the slots that were lent
+to the ones given now, all reads of a pool before its writes: they differ
+where a tree's path skips nodes, and for every request behind one that accepted
+fewer tokens than it drafted.
 """
 
 from __future__ import annotations
@@ -95,9 +100,9 @@ class SlotMapper:
         ``FreeSlotRing`` of page ids (slots at page_size 1).
         ``next_positions``: the position of each request's first new token,
         the Drop's ``next_position`` (default ``raw_lens``).  ``parents``:
-        int32, one per new token, the parent's number in the request or -1
-        (at most 64 new tokens per request); positions then follow the
-        depth.  A row whose last page a Drop has freed (all of its tokens
+        int32 [>= max_new_tokens], for each new token the parent's number in the
+        request or -1 (at most 64 new tokens per request); positions then follow
+        the depth.  A row whose last page a Drop has freed (all of its tokens
         dropped) is passed with ``raw_lens`` rounded up to whole pages, or the
         new tokens would go on in that page.  ``block_table``: int32 [>= batch, columns], filled with the
         page ids of whole rows.  A request whose row or lengths are out of range (one that no longer

@@ -683,7 +683,9 @@ int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chun
  * then take pages from the free ring
  * (akv_drop_compact's: ring[ring_capacity], ring_state = {head, tail}) in
  * request order.  With `commit` the ring's head moves past them; without it
- * they are lent: the next call gives out the same pages.
+ * they are lent: the next call gives them out again from its first request on,
+ * so tokens of a lent call that are kept must be moved to the slots that a
+ * call with commit and the kept counts gives.
  *
  * Outputs, new tokens in request order: new_offsets int32 [batch + 1]; slots
  * and positions int32 [capacity]; the row's new columns; with parents, tree_mask
