@@ -208,12 +208,8 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, ws_wait(bar, parity, abort));
 }
 
-// Key j visible to a row: its token's mask word and position.
-__device__ __forceinline__ bool key_seen(const TreeParams& p, const TreeItem& w,
-                                         unsigned long long mask, long long pos, int j) {
-  if (j >= w.prefix) return mask >> (j - w.prefix) & 1;
-  return p.window < 0 || pos - p.kv_positions[w.kv0 + j] <= p.window;
-}
+// Tiles per bit of an item's hit word.
+__device__ __forceinline__ int tiles_per_hit(int n_tiles) { return (n_tiles + 63) / 64; }
 
 // One CTA per SM with two units, each with 256 tensor-memory columns: scores
 // of 128 keys, the accumulator of D and, at head_dim 64, P beside them (at 128
@@ -234,7 +230,12 @@ struct TreeCfg {
   static constexpr int kRingOff = 2 * kQBytes;
   static constexpr int kRowOff = kRingOff + kSlots * kSlotBytes;  // [2][128] (maximum, sum)
   static constexpr int kBarOff = kRowOff + 2 * kTreeRows * 8;
-  static constexpr int kSmem = kBarOff + 256;
+  // Tiles of V that infinities or NaN were taken out of: a word per producer
+  // warp and item, for eight items.  The producers are at most four items
+  // ahead (an item has two slots at least), so a word is read before its place
+  // serves another item.
+  static constexpr int kHitOff = kBarOff + 256, kHitItems = 8;
+  static constexpr int kSmem = kHitOff + 8 * kProducers * kHitItems;
   static constexpr int kColP = D == 64 ? 128 : 64, kColO = 256 - D;
   static_assert(kSmem <= 232448, "shared memory of one CTA");
 };
@@ -286,26 +287,78 @@ __device__ __forceinline__ unsigned long long seen64(const TreeParams& p, const 
   return seen;
 }
 
-// Infinities and NaN were taken out of V tiles: adds those that a row sees to
-// columns [d0, d1) of its result (out, or the partial acc).
-template <typename T>
-__device__ __forceinline__ void restore(const TreeParams& p, const TreeItem& w,
-                                     unsigned long long mask, long long pos, int head, T* out,
-                                     float* acc, int d0, int d1) {
-#pragma unroll 1
-  for (int j = p.window >= 0 ? w.lo : max(w.lo, w.prefix / kTreeKeys * kTreeKeys); j < w.hi; ++j) {
-    if (!key_seen(p, w, mask, pos, j)) continue;
-    const long long slot = key_slot(p, w, j);
-    if (slot < 0) continue;
-    const T* v = static_cast<const T*>(p.v) + slot * p.v_ss + head * p.v_sh;
-#pragma unroll 1
-    for (int d = d0; d < d1; ++d) {
-      const float x = Elem<T>::to_f32(v[d]);
-      if (isfinite(x)) continue;
+// Infinities and NaN were taken out of tiles of V of an item (hits: bit b for
+// its tiles [b per, (b + 1) per)): adds those that a row sees to columns [d0,
+// d1) of its result (out, or the partial acc).  By a whole warp, rows `live` or
+// not: a lane searches a key's row and the warp then takes the keys that have
+// any, as bits of their columns, one after another.  The other roles wait for
+// it, 100 ms at most: measured, a tile of 128 keys of nothing but NaN takes 33 us
+// (head_dim 64) or 72 us (128), one with a single NaN under 1 us, so an item of
+// 170,000 such keys still ends in time.
+template <typename T, int D>
+__device__ __noinline__ void restore(const TreeParams& p, int item, unsigned long long hits,
+                                     int per, unsigned long long mask, long long pos, int head,
+                                     bool live, T* out, float* acc, int d0, int d1) {
+  constexpr int kWords = D / 32;
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  const TreeItem w = p.items[item];
+  const int lane = threadIdx.x & 31;
+  uint32_t up[kWords] = {}, down[kWords] = {};  // columns with +inf, with -inf; both: NaN
+  for (; hits; hits &= hits - 1) {
+    const int first = w.lo + (__ffsll((long long)hits) - 1) * per * kTreeKeys;
+    const int n = min(w.hi - first, per * kTreeKeys);
+    for (int k0 = 0; k0 < n; k0 += 32) {
+      uint32_t key_up[kWords] = {}, key_down[kWords] = {}, any = 0;
+      const int j = first + k0 + lane;
+      const long long slot = k0 + lane < n ? key_slot(p, w, j) : -1;
+      // The key's position; without a window one that is never hidden.
+      const long long at = p.window >= 0 && k0 + lane < n && j < w.prefix
+                               ? p.kv_positions[w.kv0 + j] : LLONG_MAX >> 1;
+      if (slot >= 0) {
+        const T* row = static_cast<const T*>(p.v) + slot * p.v_ss + head * p.v_sh;
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+          if (32 * k < d0 || 32 * k >= d1) continue;
+          uint4 v[4];  // 32 columns, requested together
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = *reinterpret_cast<const uint4*>(row + 32 * k + 8 * c);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const uint32_t x = (&v[e / 8].x)[e / 2 % 4] >> 16 * (e & 1) & 0xffffu;
+            if ((x & kExp) != kExp) continue;
+            const bool nan = (x & 0x7fffu) != kExp;
+            if (nan || !(x & 0x8000u)) key_up[k] |= 1u << e;
+            if (nan || (x & 0x8000u)) key_down[k] |= 1u << e;
+          }
+          any |= key_up[k] | key_down[k];
+        }
+      }
+      for (unsigned left = __ballot_sync(0xffffffffu, any); left; left &= left - 1) {
+        const int src = __ffs(left) - 1;
+        const int drafted = first + k0 + src - w.prefix;
+        const long long key_at = __shfl_sync(0xffffffffu, at, src);
+        const bool seen = live && (drafted >= 0 ? mask >> drafted & 1 : pos - key_at <= p.window);
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+          const uint32_t u = __shfl_sync(0xffffffffu, key_up[k], src);
+          const uint32_t d = __shfl_sync(0xffffffffu, key_down[k], src);
+          if (seen) {
+            up[k] |= u;
+            down[k] |= d;
+          }
+        }
+      }
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int k = 0; k < kWords; ++k)
+    for (uint32_t left = up[k] | down[k]; left; left &= left - 1) {
+      const int bit = __ffs(left) - 1, d = 32 * k + bit;
+      const float x = !(down[k] >> bit & 1) ? INFINITY : !(up[k] >> bit & 1) ? -INFINITY : NAN;
       if (out) out[d] = Elem<T>::from_f32(Elem<T>::to_f32(out[d]) + x);
       else acc[(d >> 2) * 4 * kTreeRows + (d & 3)] += x;
     }
-  }
 }
 
 // Warps 0-3 and 4-7 are the softmax of units 0 and 1 (warp w: rows 32 (w % 4)
@@ -348,6 +401,8 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOff + 240);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + C::kBarOff + 244);
   volatile int* scrubbed = reinterpret_cast<volatile int*>(smem + C::kBarOff + 248);
+  volatile unsigned long long* hits =
+      reinterpret_cast<volatile unsigned long long*>(smem + C::kHitOff);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == 0) {
@@ -371,8 +426,8 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
     }
     mbar_init(bar_x, C::kSoftmax);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *scrubbed = 0;  // 1: some tile of the CTA's items was a hit
     *abort = base & 1023 ? 1 : 0;  // the swizzled tiles need a 1024-byte aligned base
-    *scrubbed = 0;
   }
   // A CTA with an item that reaches past the call's vectors, as one of a plan
   // made after the call was captured may, does nothing.
@@ -489,6 +544,8 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         for (int i = lane; i < w.n; i += 32) last = max(last, p.q_positions[w.q0 + i]);
         last = __reduce_max_sync(0xffffffffu, last);
       }
+      volatile unsigned long long* hit_word = hits + pw * C::kHitItems + (it - it0) % C::kHitItems;
+      if (lane == 0) *hit_word = 0;
       bool hidden = false;  // this lane's next key, by the window, from some token
       auto fetch = [&](int t) {
         const int j = w.lo + t * kTreeKeys + kKpw * pw + lane % kKpw;
@@ -551,7 +608,10 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
                 hit = true;
               }
             }
-            if (hit) *scrubbed = 1;
+            if (__any_sync(0xffffffffu, hit) && lane == 0) {
+              *hit_word |= 1ull << t / tiles_per_hit(n_tiles);
+              *scrubbed = 1;
+            }
             fence_async_smem();
             mbar_arrive(bar_full(at.slot));
           } else {
@@ -811,10 +871,15 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
                   make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
           }
         }
-        if (live && *scrubbed) {
-          const long long at = p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
-          restore<T>(p, w, row_mask(p, w, p.tree_mask[w.q0 + i], at), at, head,
-                     direct ? dst : nullptr, direct ? nullptr : acc, d0, d1);
+        unsigned long long hit = 0;  // of all producers
+        if (*scrubbed)
+          for (int k = 0; k < C::kProducers; ++k)
+            hit |= hits[k * C::kHitItems + (it - it0) % C::kHitItems];
+        if (hit) {
+          const long long at = live && p.window >= 0 ? p.q_positions[w.q0 + i] : 0;
+          restore<T, D>(p, it, hit, tiles_per_hit(n_tiles),
+                        live ? row_mask(p, w, p.tree_mask[w.q0 + i], at) : 0, at, head, live,
+                        direct ? dst : nullptr, direct ? nullptr : acc, d0, d1);
         }
         if (live && (pair || u == 0)) {
           if (!direct) {

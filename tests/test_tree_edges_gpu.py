@@ -1,0 +1,116 @@
+"""Tree attention at its edges: infinities and NaN in long windows and in many
+items of one CTA, graphs replayed on other plans, small weights in fp16."""
+
+import numpy as np
+import pytest
+import torch
+
+from test_tree_gpu import attention, compare, exact, launch, make
+
+pytestmark = pytest.mark.gpu
+
+
+def seen_keys(c, b):
+    """[tokens, cached + drafted keys] of request b."""
+    lo, hi, x, y = (int(v) for v in (*c["kv"][b: b + 2], *c["dr"][b: b + 2]))
+    bits = (c["mask"][x:y, None] >> torch.arange(y - x, device="cuda")) & 1
+    seen = torch.cat((torch.ones(y - x, hi - lo, dtype=torch.bool, device="cuda"), bits.bool()), 1)
+    if c["window"] >= 0:
+        at = torch.cat((c["kpos"][lo:hi], c["qpos"][x:y]))
+        seen &= c["qpos"][x:y, None] - at <= c["window"]
+    return seen
+
+
+def check_bad_values(c, places, ctas=None):
+    """V elements ``places`` [(request, key, head, dim, value)] that are not
+    finite change those elements of the rows that see them, and nothing else:
+    all others are what zeros in their place give, bit for bit."""
+    attn = attention(c, ctas)
+    zero, bad = c["v"].clone(), c["v"].clone()
+    special = torch.zeros(len(c["q"]), c["hkv"], c["d"], dtype=torch.float64, device="cuda")
+    views = {b: seen_keys(c, b) for b in {p[0] for p in places}}
+    for b, key, head, dim, value in places:
+        lo, hi, x, y = (int(v) for v in (*c["kv"][b: b + 2], *c["dr"][b: b + 2]))
+        slot = int(c["indices"][lo + key] if key < hi - lo else c["draft"][x + key - (hi - lo)])
+        zero[slot, head, dim], bad[slot, head, dim] = 0, value
+        rows = views[b][:, key].nonzero().flatten() + x
+        special[rows, head, dim] += value
+    want, want_lse = launch({**c, "v": zero}, attn, return_lse=True)
+    out, lse = launch({**c, "v": bad}, attn, return_lse=True)
+    assert int(attn.error_flag) == 0
+    special = special.repeat_interleave(c["group"], 1)
+    hit = special != 0
+    assert bool(hit.any()) and torch.equal(lse, want_lse)
+    assert torch.equal(out[~hit], want[~hit])
+    got, sure = out[hit].double(), special[hit]
+    assert torch.equal(got.isnan(), sure.isnan())
+    assert torch.equal(got.nan_to_num(0.5), sure.nan_to_num(0.5))
+
+
+BAD = [float("nan"), float("inf"), -float("inf")]
+
+
+def draws(c, rng, n):
+    """n bad elements at keys that some row sees."""
+    out = []
+    while len(out) < n:
+        b = int(rng.integers(len(c["kv"]) - 1))
+        keys = seen_keys(c, b).any(0).nonzero().flatten()
+        if len(keys):
+            out.append((b, int(keys[int(rng.integers(len(keys)))]), int(rng.integers(c["hkv"])),
+                        int(rng.integers(c["d"])), BAD[int(rng.integers(3))]))
+    return out
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_one_bad_draft_element_behind_a_long_window_leaves_the_others(d, dtype):
+    """30,000 keys in a large window, all of it and a second request one CTA's work."""
+    c = make([30000, 700], [16, 9], 2, 8, d, dtype, seed=21, window=100000)
+    for value in BAD:
+        check_bad_values(c, [(0, 30000 + 3, 1, 5, value)], ctas=1)
+        check_bad_values(c, [(0, 30000 + 3, 1, 5, value)])
+
+
+@pytest.mark.parametrize("ctas", [1, 5])
+@pytest.mark.parametrize("d", [64, 128])
+def test_bad_elements_all_over_a_long_window(d, ctas):
+    """More tiles than an item's word has bits, hidden keys in every tile."""
+    c = make([20000, 300, 9000], [16, 64, 3], 2, 5, d, torch.bfloat16, seed=22, window=30000)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for b in range(3):  # positions in no order: every tile has hidden keys
+        part = slice(int(c["kv"][b]), int(c["kv"][b + 1]))
+        c["kpos"][part] = c["kpos"][part][torch.randperm(int(c["kv"][b + 1] - c["kv"][b]), generator=g,
+                                                         device="cuda")]
+    rng = np.random.default_rng(23)
+    check_bad_values(c, draws(c, rng, 40), ctas)
+
+
+@pytest.mark.parametrize("window", [-1, 60])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("group", [1, 8, 16])
+def test_bad_elements_in_many_short_items_of_one_cta(d, window, group):
+    rng = np.random.default_rng(24)
+    c = make(rng.integers(0, 200, 40), rng.integers(1, 20, 40), 3, group, d, torch.bfloat16, seed=25,
+             window=window)
+    # Without a window an infinity that all rows of a tile see takes the ordinary way, as its
+    # product with a weight above 0; the weights of this test are.
+    for ctas in (1, 3, None):
+        check_bad_values(c, draws(c, rng, 30), ctas)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_request_of_nothing_but_nan_leaves_the_others(d):
+    """Every V of a long request is NaN, with hidden keys in every tile."""
+    c = make([12000, 40, 300], [16, 8, 33], 2, 8, d, torch.bfloat16, seed=26, window=15000)
+    part = slice(0, 12000)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    c["kpos"][part] = c["kpos"][part][torch.randperm(12000, generator=g, device="cuda")]
+    v = c["v"].clone()
+    v[c["indices"][part].long()] = float("nan")
+    for ctas in (1, None):
+        attn = attention(c, ctas)
+        want, want_lse = launch(c, attn, return_lse=True)
+        out, lse = launch({**c, "v": v}, attn, return_lse=True)
+        assert int(attn.error_flag) == 0 and torch.equal(lse, want_lse)
+        assert bool(out[:16].isnan().all()) and torch.equal(out[16:], want[16:])
