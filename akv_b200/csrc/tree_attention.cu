@@ -292,8 +292,8 @@ __device__ __forceinline__ unsigned long long seen64(const TreeParams& p, const 
 // d1) of its result (out, or the partial acc).  By a whole warp, rows `live` or
 // not: a lane searches a key's row and the warp then takes the keys that have
 // any, as bits of their columns, one after another.  The other roles wait for
-// it, 100 ms at most: measured, a tile of 128 keys of nothing but NaN takes 33 us
-// (head_dim 64) or 72 us (128), one with a single NaN under 1 us, so an item of
+// it, 100 ms at most: measured, a tile of 128 keys with one NaN takes about 8 us,
+// one of nothing but NaN 33 us (head_dim 64) or 72 us (128), so an item of
 // 170,000 such keys still ends in time.
 template <typename T, int D>
 __device__ __noinline__ void restore(const TreeParams& p, int item, unsigned long long hits,
@@ -925,6 +925,9 @@ __global__ void __launch_bounds__(kMergeThreads)
 tree_merge_kernel(const TreeParams p, const TreeMerge* merges) {
   constexpr int kRows = merge_rows<D>();
   const TreeMerge g = merges[blockIdx.x];
+  // Before any return: once every block has left, the stream goes on, and the
+  // pieces' kernel has to be done by then.
+  pdl_wait();
   const int u = blockIdx.y / (kTreeRows / kRows);
   const int r = blockIdx.y % (kTreeRows / kRows) * kRows + threadIdx.x % kRows;
   const int d = threadIdx.x / kRows * 4;
@@ -933,7 +936,6 @@ tree_merge_kernel(const TreeParams p, const TreeMerge* merges) {
   const int row = (g.tile0 + u * (g.steps >> 1 & 1)) * kTreeRows + r;
   const int i = row / p.group, h = head * p.group + row % p.group;
   if (i >= g.n || g.q0 + g.n > p.tokens) return;
-  pdl_wait();
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) +
                      ((long long)g.first + u) * kTreeRows + r;
   const float* acc = p.part_acc + (((long long)g.first + u) * D + d) * kTreeRows + 4 * r;

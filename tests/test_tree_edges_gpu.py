@@ -114,3 +114,27 @@ def test_a_request_of_nothing_but_nan_leaves_the_others(d):
         out, lse = launch({**c, "v": v}, attn, return_lse=True)
         assert int(attn.error_flag) == 0 and torch.equal(lse, want_lse)
         assert bool(out[:16].isnan().all()) and torch.equal(out[16:], want[16:])
+
+
+def test_work_behind_a_merge_that_joins_nothing_waits_for_its_pieces():
+    """A replay on a plan whose every merge lies past the call's tokens: what
+    follows in the stream sees the error bits of the pieces' kernel."""
+    c = make([4000], [8], 2, 8, 64, torch.bfloat16, seed=27)
+    attn = attention(c, 8)
+    out = torch.empty_like(c["q"])
+    launch(c, attn, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        launch(c, attn, out=out)
+    attn.plan([0, 4000], [0, 64])       # 64 tokens where the call has 8
+    for _ in range(20):
+        attn.error_flag.zero_()
+        graph.replay()
+        seen = attn.error_flag.clone()
+        assert int(seen) == 4
+    attn.plan(c["kv"], c["dr"])
+    attn.error_flag.zero_()
+    graph.replay()
+    assert int(attn.error_flag) == 0
+    compare(c, out, launch(c, attn, return_lse=True)[1])
