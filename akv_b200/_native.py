@@ -219,6 +219,14 @@ def stream_of(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def capturing(index: int) -> bool:
+    """Whether the current torch stream of CUDA device ``index`` is being captured."""
+    if torch._C._cuda_getDevice() == index:
+        return torch._C._cuda_isCurrentStreamCapturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def launch(index: int, fn, args) -> int:
     """``fn(args, stream)`` on the current torch stream of CUDA device
     ``index``, which is made the current device for the call if it is not

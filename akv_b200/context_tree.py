@@ -11,7 +11,7 @@ same paged inputs as ``DecodeAttention`` plus the drafted tokens' slots and one
 Like ``DecodeAttention``, ``plan`` cuts the batch into a work list on the host
 (one pinned copy to the device) and ``run`` launches on the current stream
 without host synchronisation: one kernel, and a second one that joins the
-pieces of requests that were cut.
+pieces of requests that were cut.  A captured run follows later plans.
 """
 
 from __future__ import annotations
@@ -107,10 +107,13 @@ _fields, _INT32, _INT64 = _native.fields, _native.INT32, _native.INT64
 
 class TreeAttention:
     """Plans and partial results live in the instance: runs of one instance,
-    replays of its graphs among them, must not overlap on the device.  A
-    captured run keeps its launch sizes but reads the plan that the device
-    holds when it replays, so a new plan needs a new capture; one with as many
-    CTAs, merges, tokens and keys (the same lengths in another order) does not."""
+    replays of its graphs among them, must not overlap on the device.
+
+    A captured run launches the instance's largest grid and takes everything
+    else from the plan that the device holds when it replays, so a graph
+    serves any later ``plan`` (on the replaying stream) whose tokens and keys fit in the
+    tensors that were passed to it: pass vectors with room for a cache that
+    grows, and ``out``.  A plan that does not fit is reported by ``check``."""
 
     def __init__(self, num_q_heads, num_kv_heads, head_dim, max_batch, device, *,
                  dtype=torch.bfloat16, sm_scale=None, ctas=None):
@@ -143,9 +146,13 @@ class TreeAttention:
         self.max_items = self.max_batch * groups + self.ctas
         self.max_merges = min(self.max_batch * groups, self.ctas)
         partials = 2 * self.ctas * UNITS
-        self._at = (12 * self.max_items, 12 * self.max_items + 8 * self.max_merges)
-        size = self._at[1] + self.ctas + 1
-        self._host = torch.empty(size, dtype=torch.int32, pin_memory=True)
+        # The device's plan: cta_items, merges and items, so that one copy of a
+        # prefix brings it.  Entries past a plan's CTAs hold no item and those past its
+        # merges join nothing: what a run launches beyond them has no work.
+        self._at = (self.ctas + 1, self.ctas + 1 + 8 * self.max_merges)
+        size = self._at[1] + 12 * self.max_items
+        self._host = torch.zeros(size, dtype=torch.int32, pin_memory=True)
+        self._host_np = self._host.numpy()
         self._dev = torch.zeros(size, dtype=torch.int32, device=device)
         self._acc = torch.empty((partials, TILE_ROWS, head_dim), dtype=torch.float32, device=device)
         self._ml = torch.empty((partials, TILE_ROWS, 2), dtype=torch.float32, device=device)
@@ -168,14 +175,14 @@ class TreeAttention:
         assert len(items) <= self.max_items and len(merges) <= self.max_merges and \
             partials <= len(self._acc)
         self._copied.synchronize()
+        host, (m, i) = self._host_np, self._at
+        used = i + items.size
+        host[: len(cta_items)], host[len(cta_items): m] = cta_items, cta_items[-1]
+        host[m: m + merges.size], host[m + merges.size: i] = merges.reshape(-1), 0
+        host[i: used] = items.reshape(-1)
         stream = torch.cuda.current_stream(self.device)
         with torch.cuda.stream(stream):
-            for at, part in ((0, items), (self._at[0], merges), (self._at[1], cta_items)):
-                part = part.reshape(-1)
-                if len(part):
-                    self._host[at: at + len(part)].copy_(torch.from_numpy(part))
-                    self._dev[at: at + len(part)].copy_(self._host[at: at + len(part)],
-                                                        non_blocking=True)
+            self._dev[:used].copy_(self._host[:used], non_blocking=True)
             self._copied.record(stream)
         self.tokens, self.keys = int(draft_indptr_host[-1]), int(kv_indptr_host[-1])
         self.n_ctas, self.n_merges = len(cta_items) - 1, len(merges)
@@ -218,6 +225,10 @@ class TreeAttention:
                 (draft_step != 1 and draft_n > 1) or (mask_step != 1 and mask_n > 1):
             raise ValueError("kv_indices (int32), draft_slots (int32) and tree_mask (int64) must "
                              "be contiguous vectors of the plan's lengths, on its device")
+        if draft_n < n:
+            n = draft_n
+        if mask_n < n:
+            n = mask_n  # tokens that the vectors hold
         window = -1 if window is None or window < 0 else int(window)
         dev = self._plan_ptr
         q_pos = kv_pos = sinks_ptr = lse_ptr = 0
@@ -231,6 +242,10 @@ class TreeAttention:
                 raise ValueError("q_positions and kv_positions must be contiguous int32 vectors "
                                  "of the plan's lengths, on its device")
             kv_pos = kv_pos or dev
+            if n1 < kv_n:
+                kv_n = n1
+            if n0 < n:
+                n = n0
         if sinks is not None:
             sinks_ptr, dev0, dt0, n0, step0 = _fields(1, sinks)
             if n0 != hq or _native.FIELD_CODE.get(dt0) != _native.AKV_F32 or dev0 != index or \
@@ -238,26 +253,32 @@ class TreeAttention:
                 raise ValueError("sinks must be fp32 [num_q_heads] on the plan's device")
         if out is None:
             out = torch.empty((tokens, hq, d), dtype=self.dtype, device=self.device)
-        o_ptr, o_dev, o_dt, n, heads, dim, o_token, o_head, unit = _fields(3, out)
-        if n < tokens or heads != hq or dim != d or unit != 1 or o_dev != index or o_dt != q_dt:
+        o_ptr, o_dev, o_dt, o_n, heads, dim, o_token, o_head, unit = _fields(3, out)
+        if o_n < tokens or heads != hq or dim != d or unit != 1 or o_dev != index or o_dt != q_dt:
             raise ValueError("out must be [>= tokens, num_q_heads, head_dim] of the planned type "
                              "with unit last stride, on the plan's device")
         lse = None
         if return_lse:
             lse = torch.empty((tokens, self.hq), dtype=torch.float32, device=self.device)
-            lse_ptr = lse.data_ptr()
+            lse_ptr, n = lse.data_ptr(), tokens
+        if o_n < n:
+            n = o_n
+        n_ctas, n_merges = self.n_ctas, self.n_merges
+        if n and _native.capturing(index):
+            n_ctas, n_merges = self.ctas, self.max_merges
         status = _native.launch(index, _native.lib.akv_tree_attention, _native.TREE_ATTENTION.pack(
             q_ptr, q_token, q_head, k_ptr, v_ptr, k_slot, k_head, v_slot, v_head,
-            k_slots if k_slots < v_slots else v_slots, code, tokens, keys, kv_ptr or dev,
-            draft_ptr, mask_ptr, q_pos, kv_pos, window, sinks_ptr, self.sm_scale, hq, hkv, d, dev,
-            dev + 4 * self._at[1], self.n_ctas, dev + 4 * self._at[0], self.n_merges,
+            k_slots if k_slots < v_slots else v_slots, code, n, kv_n, kv_ptr or dev,
+            draft_ptr, mask_ptr, q_pos, kv_pos, window, sinks_ptr, self.sm_scale, hq, hkv, d,
+            dev + 4 * self._at[1], dev, n_ctas, dev + 4 * self._at[0], n_merges,
             *self._partial_ptrs, o_ptr, o_token, o_head, lse_ptr, self._flag_ptr))
         _native.check(status, "tree_attention")
         return (out, lse) if return_lse else out
 
     ERRORS = {1: "a key slot outside the KV pools was read as slot 0",
               2: "a wait inside the kernel ran out; the output of that launch is invalid",
-              4: "a captured run was replayed on a plan of more tokens or keys"}
+              4: "a captured run was replayed on a plan of more tokens or keys than its "
+                 "tensors hold"}
 
     def check(self):
         """Raise RuntimeError if a launch since the last check reported an

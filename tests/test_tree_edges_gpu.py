@@ -138,3 +138,96 @@ def test_work_behind_a_merge_that_joins_nothing_waits_for_its_pieces():
     graph.replay()
     assert int(attn.error_flag) == 0
     compare(c, out, launch(c, attn, return_lse=True)[1])
+
+
+def grown(c, cached, new, room_keys, room_tokens):
+    """The same pools under other lengths, vectors copied into ones of a fixed size."""
+    def wide(t, n):
+        out = t.new_zeros((n, *t.shape[1:]))
+        out[: len(t)] = t
+        return out
+
+    keys, total = int(sum(cached)), int(sum(new))
+    x = make(cached, new, c["hkv"], c["group"], c["d"], c["dtype"], seed=keys + total, sinks=True,
+             window=c["window"], extra_slots=len(c["k"]) - keys - total)
+    return x, {n: wide(x[n], room_tokens if n in ("q", "draft", "mask", "qpos") else room_keys)
+               for n in ("q", "draft", "mask", "qpos", "indices", "kpos")}
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [-1, 900])
+def test_one_graph_over_growing_caches_and_other_batches(d, window):
+    """Captured once and replayed on plans of other lengths, batches, CTA and
+    merge counts, an empty one among them: always what an eager run gives."""
+    rng = np.random.default_rng(31)
+    room_keys, room_tokens, batch = 12000, 120, 12
+    lens = rng.integers(0, 900, batch)
+    c = make(lens, [8] * batch, 2, 8, d, torch.bfloat16, seed=32, window=window, sinks=True,
+             extra_slots=16000)
+    from akv_b200.context_tree import TreeAttention
+
+    attn = TreeAttention(16, 2, d, batch, "cuda", ctas=23).plan(c["kv"], c["dr"])
+    fixed = grown(c, lens, [8] * batch, room_keys, room_tokens)[1]
+    buffers = {n: t.clone() for n, t in fixed.items()}
+    pools = dict(k=torch.zeros_like(c["k"]), v=torch.zeros_like(c["v"]))
+    sinks = torch.zeros(16, device="cuda")
+    out = torch.empty(room_tokens, 16, d, dtype=torch.bfloat16, device="cuda")
+
+    def run():
+        return attn.run(buffers["q"], pools["k"], pools["v"], buffers["indices"], buffers["draft"],
+                        buffers["mask"], sinks=sinks, window=window, q_positions=buffers["qpos"],
+                        kv_positions=buffers["kpos"], out=out)
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    steps, counts = [], set()
+    for _ in range(20):                                     # a cache that grows
+        lens = lens + rng.integers(0, 6, batch)
+        steps.append((lens.copy(), rng.integers(1, 10, batch)))
+    steps += [([5000], [64]), ([], []), ([0, 3], [1, 0]), ([40] * 12, [1] * 12), ([9000, 70], [3, 64]),
+              ([room_keys], [1]), ([1, 2], [64, 56])]
+    for cached, new in steps:
+        x, vectors = grown(c, cached, new, room_keys, room_tokens)
+        for n, t in vectors.items():
+            buffers[n].copy_(t)
+        pools["k"].copy_(x["k"])
+        pools["v"].copy_(x["v"])
+        sinks.copy_(x["sinks"])
+        attn.plan(x["kv"], x["dr"])
+        counts.add((attn.n_ctas, attn.n_merges))
+        out.fill_(7)
+        graph.replay()
+        total = int(sum(new))
+        assert int(attn.error_flag) == 0 and bool((out[total:] == 7).all())
+        fresh = TreeAttention(16, 2, d, batch, "cuda", ctas=23).plan(x["kv"], x["dr"])
+        want = launch(x, fresh)
+        assert torch.equal(out[:total], want)
+    assert len({n for n, _ in counts}) > 2 and len({m for _, m in counts}) > 2
+    for cached, new in (([room_keys, 1], [1, 1]), ([3, 3], [64, 57])):    # a key, a token too many
+        kv, dr = (np.concatenate(([0], np.cumsum(n))) for n in (cached, new))
+        attn.plan(kv, dr)
+        graph.replay()
+        with pytest.raises(RuntimeError, match="tensors hold"):
+            attn.check()
+
+
+def test_a_graph_captured_on_an_empty_plan():
+    c = make([300, 20], [5, 9], 2, 8, 64, torch.bfloat16, seed=33)
+    attn = attention(c)
+    want = launch(c, attention(c))
+    out = torch.zeros_like(want)
+    launch(c, attn, out=out)
+    attn.plan([0], [0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        launch(c, attn, out=out)
+    out.zero_()
+    graph.replay()
+    assert not bool(out.any())
+    attn.plan(c["kv"], c["dr"])
+    graph.replay()
+    assert torch.equal(out, want) and int(attn.error_flag) == 0
