@@ -384,6 +384,10 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
   using Pos = RingPos<C::kSlots>;
   constexpr int kHalf = std::is_same<T, __half>::value;  // fp16 operands
   constexpr bool kFree = D == 64;                        // P has columns of its own
+  // fp16's weights are taken 2^7 times as large, which still leaves room for
+  // the 2^8 that scores may pass the base by: a weight keeps 11 bits down to
+  // 2^-21 of the row's largest (2^-14 without) and counts down to 2^-32.
+  constexpr float kLift = kHalf ? 7.f : 0.f;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
   const uint32_t bars = base + C::kBarOff;
@@ -743,7 +747,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
               alpha = rescale ? fast_exp2(m - bm) : 0.f;
               m = bm;
             }
-            const float nb = m == -INFINITY ? 0.f : -m;
+            const float nb = m == -INFINITY ? 0.f : kLift - m;
             const f32x2 scale2 = f2_pack(p.scale_log2, p.scale_log2), nb2 = f2_pack(nb, nb);
             f32x2 sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
             // The last columns come first: P overwrites the second half of its
@@ -806,6 +810,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p) {
         }
       }
       if (!ok) break;
+      m -= kLift;  // the base that P, l and O are in
       // The item is read, and the row worked out, again: over the tiles they
       // would only hold registers.
       const TreeItem w = p.items[it];

@@ -231,3 +231,31 @@ def test_a_graph_captured_on_an_empty_plan():
     attn.plan(c["kv"], c["dr"])
     graph.replay()
     assert torch.equal(out, want) and int(attn.error_flag) == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ctas", [1, None])
+def test_many_small_weights_in_fp16(d, ctas):
+    """One key of score 0 with V 0 and 150,000 of weight 2^-26 with V 1: half of
+    fp16's smallest P, but 0.2 % of the sum.  Tolerance as compare() without its
+    term for subnormal P: a P of at least 2^-14 (base 2^7 up: weights of 2^-21
+    and more) keeps 11 bits, one below is off by at most 2^-25 in those units,
+    2^-32 of the row's largest weight, per key."""
+    n = 150000
+    c = make([n], [3], 1, 8, d, torch.float16, seed=41)
+    c["mask"].zero_()                       # cached keys alone
+    c["q"].zero_()
+    c["q"][:, :, 0] = 1.0
+    c["k"].zero_()
+    c["v"].fill_(1.0)
+    # score = q0 k0 / sqrt(d) + q1 k1 / sqrt(d): 26 ln 2 below, to fp16's steps
+    c["k"][:, :, 0] = -26 * np.log(2) * d**0.5
+    at = int(c["indices"][n // 3])
+    c["k"][at], c["v"][at] = 0.0, 0.0
+    out, lse = launch(c, attention(c, ctas), return_lse=True)
+    want, want_lse, mean, size = exact(c)
+    assert float(want.max()) > 1e-3
+    u = 2.0**-11
+    e32 = (d + 4) * 2.0**-23 * size + 2.0**-21 + n * 2.0**-24
+    bound = u * want.abs() + (u + 2 * e32[..., None]) * mean + n * 2.0**-32 + 2.0**-24
+    assert bool(((out.double() - want).abs() <= bound * (1 + u)).all())
