@@ -48,8 +48,9 @@ def tree_work_list(kv_indptr, draft_indptr, group, num_kv_heads, pair_heads, cta
     prefix, n = np.diff(kv), np.diff(dr)
     if np.any(prefix < 0) or np.any(n < 0):
         raise ValueError("kv_indptr and draft_indptr must not decrease")
-    if kv[-1] >= 2**31 or dr[-1] >= 2**31:
-        raise ValueError("the batch has 2^31 keys or more")
+    # Numbers of keys and tokens, the end of a request's last tile included, are 32 bits.
+    if kv[-1] + MAX_DRAFT + TILE_KEYS >= 2**31 or dr[-1] + MAX_DRAFT >= 2**31:
+        raise ValueError("the batch has 2^31 keys or more, or a request's last tile passes them")
     if n.size and n.max() > MAX_DRAFT:
         raise ValueError(f"a request has more than {MAX_DRAFT} drafted tokens")
     row_tiles = -(-n * group // TILE_ROWS)
