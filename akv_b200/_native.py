@@ -188,15 +188,24 @@ def _load():
 
 
 lib = _load()
+# fields(ndim, tensor, ...) -> address, device, type code, sizes and strides of each, and the
+# type codes.  The drafted-token step alone uses it; without it the rest works.
+INT32 = INT64 = None
+FIELD_CODE = {}  # type code -> AKV_* element type
 try:
     from . import _tensor_fields
-    from ._tensor_fields import fields  # noqa: F401  (address, device, type, sizes, strides)
+
+    if getattr(_tensor_fields, "BUILT_FOR", None) != torch.__version__:
+        raise ImportError("it was built for another torch")
+    fields = _tensor_fields.fields
+    INT32, INT64 = _tensor_fields.INT32, _tensor_fields.INT64
+    FIELD_CODE = {_tensor_fields.F16: AKV_F16, _tensor_fields.BF16: AKV_BF16,
+                  _tensor_fields.F32: AKV_F32}
 except ImportError as e:
-    raise ImportError(f"akv_b200._tensor_fields is not built; run `python -m akv_b200.build` ({e})")
-INT32, INT64 = _tensor_fields.INT32, _tensor_fields.INT64
-# fields()' type codes -> AKV_* element types
-FIELD_CODE = {_tensor_fields.F16: AKV_F16, _tensor_fields.BF16: AKV_BF16,
-              _tensor_fields.F32: AKV_F32}
+    _no_fields = f"akv_b200._tensor_fields cannot be used ({e}); run `python -m akv_b200.build`"
+
+    def fields(*args):
+        raise ImportError(_no_fields)
 
 
 def ptr(t):

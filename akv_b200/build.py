@@ -5,8 +5,10 @@
 Compiles every ``csrc/*.cu`` with nvcc for ``sm_100a`` only and links them
 into ``akv_b200/libakv_b200.so`` in the source tree, so the built library
 travels with the tree; ``csrc/tensor_fields.cpp`` becomes the CPython module
-``_tensor_fields`` beside it (g++, torch's headers).  ``-Xptxas -v`` output (registers, spills, shared
-memory) is written to ``akv_b200/_build/ptxas.txt``.
+``_tensor_fields`` beside it (g++, torch's headers), whose file name carries
+Python's ABI tag and which is built again for another torch.  ``-Xptxas -v``
+output (registers, spills, shared memory) is written to
+``akv_b200/_build/ptxas.txt``.
 """
 
 from __future__ import annotations
@@ -22,7 +24,8 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libakv_b200.so")
-FIELDS = os.path.join(PKG, "_tensor_fields.so")  # CPython module: a tensor's fields in one call
+# CPython module: a tensor's fields in one call
+FIELDS = os.path.join(PKG, "_tensor_fields" + sysconfig.get_config_var("EXT_SUFFIX"))
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -45,16 +48,24 @@ def build_fields(force: bool = False) -> str:
     import torch
 
     src = os.path.join(CSRC, "tensor_fields.cpp")
-    if force or _stale(FIELDS, [src]):
+    stamp = os.path.join(BUILD, "tensor_fields.txt")  # the torch it was built for
+    built_for = ""
+    if os.path.exists(stamp):
+        with open(stamp) as f:
+            built_for = f.read()
+    if force or built_for != torch.__version__ or _stale(FIELDS, [src]):
         t = os.path.dirname(torch.__file__)
         lib = os.path.join(t, "lib")
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+               f'-DAKV_TORCH_VERSION="{torch.__version__}"',
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                "-I", os.path.join(t, "include"),
                "-I", os.path.join(t, "include", "torch", "csrc", "api", "include"),
                "-I", sysconfig.get_paths()["include"], src, "-o", FIELDS,
                "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10"]
         subprocess.run(cmd, check=True)
+        with open(stamp, "w") as f:
+            f.write(torch.__version__)
     return FIELDS
 
 

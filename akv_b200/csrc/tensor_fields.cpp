@@ -69,6 +69,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_fields", nullptr, -1, meth
 PyMODINIT_FUNC PyInit__tensor_fields(void) {
   PyObject* m = PyModule_Create(&module);
   if (m == nullptr) return nullptr;
+  // The tensor's layout is that of this torch: _native checks it.
+  PyModule_AddStringConstant(m, "BUILT_FOR", AKV_TORCH_VERSION);
   PyModule_AddIntConstant(m, "INT32", (long)at::kInt);
   PyModule_AddIntConstant(m, "INT64", (long)at::kLong);
   PyModule_AddIntConstant(m, "F16", (long)at::kHalf);

@@ -1,6 +1,5 @@
 """Host side of the drafted-token step at its edges (no GPU needed)."""
 
-import os
 import subprocess
 import sys
 
@@ -20,3 +19,80 @@ def test_tree_work_list_refuses_batches_whose_last_tile_passes_32_bits():
     items, *_ = tree_work_list([0, 2**31 - 400], [0, 64], 8, 1, True, 1)
     assert items.dtype == np.int32 and (items[:, 4] >= 0).all() and (items[:, 5] > items[:, 4]).all()
     assert items[:, 5].max() == 2**31 - 336
+
+
+def run(code):
+    return subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True,
+                          timeout=300)
+
+
+BLOCK = """
+import sys, importlib.abc
+class No(importlib.abc.MetaPathFinder):
+    def find_spec(self, name, path=None, target=None):
+        if name.endswith("._tensor_fields"):
+            raise ImportError("not here")
+sys.meta_path.insert(0, No())
+"""
+
+
+def test_the_package_works_without_the_module_that_torch_is_compiled_into():
+    """Everything that needs the kernels' library alone imports and runs; the
+    drafted-token step says what to build."""
+    got = run(BLOCK + """
+import torch
+from akv_b200 import (_native, context_attention, context_drop, context_occurrence,
+                      context_page_table, context_prefill, context_reposition, context_rope,
+                      context_slots, context_tree)
+assert _native.lib.akv_map_slots(None, None) == _native.AKV_ERR_INVALID
+assert len(context_tree.tree_work_list([0, 500], [0, 4], 8, 8, True, 148)[0])
+x = torch.zeros(2, 8, 64, dtype=torch.bfloat16)
+try:
+    context_rope.qk_norm_rope(x, x, torch.zeros(2, dtype=torch.int32), torch.zeros(4, 64))
+except ImportError as e:
+    assert "akv_b200.build" in str(e) and "not here" in str(e), e
+    print("refused")
+""")
+    assert got.returncode == 0 and got.stdout.strip() == "refused", got.stderr[-2000:]
+
+
+def test_a_module_built_for_another_torch_is_not_used():
+    got = run("""
+import torch
+torch.__version__ = torch.__version__ + ".other"
+from akv_b200 import _native
+try:
+    _native.fields(1)
+except ImportError as e:
+    assert "another torch" in str(e), e
+    print("refused")
+""")
+    assert got.returncode == 0 and got.stdout.strip() == "refused", got.stderr[-2000:]
+
+
+def test_the_module_is_rebuilt_for_another_torch_or_python(tmp_path, monkeypatch):
+    import sysconfig
+
+    import torch
+
+    from akv_b200 import build
+
+    assert build.FIELDS.endswith(sysconfig.get_config_var("EXT_SUFFIX"))
+    calls = []
+    monkeypatch.setattr(build, "FIELDS", str(tmp_path / "_tensor_fields.so"))
+    monkeypatch.setattr(build, "BUILD", str(tmp_path))
+
+    def compile_(cmd, check):
+        calls.append(cmd)
+        open(build.FIELDS, "w").close()
+
+    monkeypatch.setattr(build.subprocess, "run", compile_)
+    build.build_fields()
+    build.build_fields()
+    assert len(calls) == 1
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    build.build_fields()
+    build.build_fields()
+    assert len(calls) == 2 and any("9.9.9" in part for part in calls[1])
+    build.build_fields(force=True)
+    assert len(calls) == 3
