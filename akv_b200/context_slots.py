@@ -114,9 +114,9 @@ class SlotMapper:
         the device sees are bits of ``status`` (``SlotMap.check``)."""
         index = self._index
         (rows_ptr, rows_dev, rows_dt, batch, rows_step, raw_ptr, raw_dev, raw_dt, n_raw, raw_step,
-         new_ptr, new_dev, new_dt, n_new, new_step, free_ptr, free_dev, _, free_n, free_step,
-         state_ptr, state_dev, state_dt, state_n, _) = _fields(1, row_ids, raw_lens, new_lens,
-                                                               ring.ring, ring.state)
+         new_ptr, new_dev, new_dt, n_new, new_step, free_ptr, free_dev, free_dt, free_n, free_step,
+         state_ptr, state_dev, state_dt, state_n, state_step) = _fields(
+             1, row_ids, raw_lens, new_lens, ring.ring, ring.state)
         if batch > self.max_batch:
             raise ValueError("batch exceeds max_batch")
         if n_raw != batch or n_new != batch or not rows_dev == raw_dev == new_dev == index or \
@@ -127,8 +127,10 @@ class SlotMapper:
             if dt != _INT32 and dt != _INT64:
                 raise ValueError("row_ids, raw_lens and new_lens must be int32 or int64")
         if free_dev != index or state_dev != index or free_n < ring.capacity or state_n < 2 or \
-                state_dt != _INT64:
-            raise ValueError("the free ring must be on the mapper's device")
+                free_dt != _INT32 or state_dt != _INT64 or state_step != 1 or \
+                (free_step != 1 and free_n > 1):
+            raise ValueError("the free ring must be contiguous int32 entries, with an int64 state, "
+                             "on the mapper's device")
         table, dev, dt, rows, columns, row_stride, unit = _fields(2, req_to_token)
         if dt != _INT32 or unit != 1 or dev != index:
             raise ValueError("req_to_token must be int32 [rows, columns] with unit last stride, "

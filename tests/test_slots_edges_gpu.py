@@ -241,3 +241,21 @@ def test_kept_offsets_refuse_lengths_that_leave_none(new):
     np.testing.assert_array_equal(t["rows"].cpu().numpy(), c["rows"])
     np.testing.assert_array_equal(t["table"].cpu().numpy(), c["table"])
     assert t["ring"].state.tolist() == [c["head"], c["tail"]]
+
+
+def test_rings_of_other_types_are_refused():
+    from akv_b200.context_drop import FreeSlotRing
+    from akv_b200.context_slots import SlotMapper
+
+    mapper = SlotMapper(1, 4, "cuda")
+    rows = torch.zeros(2, 8, dtype=torch.int32, device="cuda")
+    one = torch.ones(1, dtype=torch.int64, device="cuda")
+    for field, value in (("ring", torch.arange(8, device="cuda")),
+                         ("ring", torch.arange(16, dtype=torch.int32, device="cuda")[::2]),
+                         ("ring", torch.arange(7, dtype=torch.int32, device="cuda")),
+                         ("state", torch.zeros(2, dtype=torch.int32, device="cuda")),
+                         ("state", torch.zeros(4, dtype=torch.int64, device="cuda")[::2])):
+        ring = FreeSlotRing(torch.arange(8), device="cuda")
+        setattr(ring, field, value)
+        with pytest.raises(ValueError, match="free ring"):
+            mapper.run(rows, one - 1, one - 1, one, ring)
