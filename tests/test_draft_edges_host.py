@@ -96,3 +96,26 @@ def test_the_module_is_rebuilt_for_another_torch_or_python(tmp_path, monkeypatch
     assert len(calls) == 2 and any("9.9.9" in part for part in calls[1])
     build.build_fields(force=True)
     assert len(calls) == 3
+
+
+def test_the_polynomial_exponential_is_as_good_as_its_comment_says():
+    """2^f on [-1/2, 1/2] by the kernel's constants: as a real polynomial, and in
+    fp32 with one rounding per step, as the kernel's fused multiply-adds."""
+    import os
+    import re
+
+    text = open(os.path.join(ROOT, "akv_b200", "csrc", "tree_attention.cu")).read()
+    body = text[text.index("void exp2_pair"):]
+    body = body[: body.index("\n}\n")]
+    c = [float.fromhex(x) for x in re.findall(r"f2_pack\((0x[0-9a-fp.+-]+)f, ", body)] + [1.0]
+    assert len(c) == 6
+    f = np.linspace(-0.5, 0.5, 400001).astype(np.float32)
+    want = np.exp2(f.astype(np.longdouble))
+    real, rounded = np.longdouble(c[0]), np.full_like(f, c[0])
+    for k in c[1:]:
+        real = real * f + np.longdouble(k)
+        # The product of two fp32 numbers is exact in 64 bits; the sum's own rounding there is
+        # 2^-29 of one in fp32.
+        rounded = (rounded.astype(np.float64) * f + k).astype(np.float32)
+    assert np.abs(real / want - 1).max() < 1.1e-7
+    assert np.abs(rounded / want - 1).max() < 1.7e-7 < 2 * 2.0**-23
