@@ -24,11 +24,13 @@
 // below).  Measured, bf16 (calls one after another in a graph, other inputs each):
 // 16,411 tokens of 64 + 8 + 8 heads of 128 (681 MB) 124 us, 5.5 TB/s, 0.84 of the
 // copy rate, at 12 blocks of 64 threads per SM (80 registers); two rows per lane 132
-// us, eight 138 us, four at 16 warps per SM 141 us and at 28 146 us (spills).  2,048
-// tokens of head_dim 64 (42.5 MB) 11.8 us; one token 3.5 us.  With only a part of
-// D turning (fp16, pairs, 64 of 128, 76.6 MB) 17.5 us, 4.4 TB/s: 2.6 waves of
-// blocks, and the masks of what does not turn (16.5 without; two rows per lane
-// 18.8).
+// us, eight 138 us, four at 16 warps per SM 141 us and at 28 146 us (more spills:
+// at 80 registers every instantiation keeps 48 to 148 bytes of a thread in local
+// memory, 116 in this one).  fp32, 8,205 tokens of the same heads (676 MB) 105 us,
+// 6.4 TB/s.  2,048 tokens of head_dim 64 (42.5 MB) 12 us; one token 3.8 us.  With
+// only a part of D turning (fp16, pairs, 64 of 128, 76.6 MB) 17.5-18.1 us, 4.3
+// TB/s: 2.6 waves of blocks, and the masks of what does not turn (16.5 without;
+// two rows per lane 18.8).
 
 #include <type_traits>
 
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(kRopeThreads, 12) qk_norm_rope_kernel(const Ro
       } else {
         // Past the rotation the turn is by cos 1 and sin 0, and the products
         // are masked to 0: an infinity times sin 0 would be NaN.  The sign is
-        // set here too, since n2's registers would spill.
+        // set here too, since n2's registers would spill as well.
         const f32x2 on = NEOX || k < 2 ? keep : keep1;
         xs &= on;
         ys = (f2_mul(v.y[k], s2[k]) & on) ^ 0x8000000080000000ull;

@@ -24,12 +24,14 @@
 // Every block therefore sums the whole batch's lengths itself (a batch is a
 // few hundred loads from L2) instead of waiting for a scan kernel.  Measured
 // (device time, calls one after another in a graph): one request 4.2 us; 64
-// requests over 16-slot pages with block tables 5.4 us; 512 requests of 0-64
-// drafted tokens with block tables of 4.2M entries (33.8 MB) 14.9 us, of which the
-// tables about 8 (20.8 us with 4-byte copies; eight 16-byte loads in flight
-// instead of four, or blocks of 512 threads, 20 us: then not all blocks are
-// resident).  More blocks per request cost more sums than they save (4-byte
-// copies: 15.5 us at one block, 19.9 at two, 28 at four).
+// requests over 16-slot pages with block tables 5.7-6.1 us; 512 requests of 0-64
+// drafted tokens with block tables of 4.2M entries (33.8 MB) 14.7-15.2 us, of
+// which the tables about 8 (20.8 us with 4-byte copies; eight 16-byte loads in
+// flight instead of four, or blocks of 512 threads, 20 us: then not all blocks
+// are resident).  The loads of a table's old part wait for the sums only because
+// a refused call must leave the table alone.  More blocks per request cost more
+// sums than they save (4-byte copies: 15.5 us at one block, 19.9 at two, 28 at
+// four).
 
 #include <algorithm>
 

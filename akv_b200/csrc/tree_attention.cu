@@ -19,16 +19,17 @@
 // Bound.  A key costs Hkv D 4 bytes and 4 Hq D flops per drafted token: HBM up to
 // about 16 tokens per request at a group of 8, the softmax and the tensor
 // cores above.  Measured (device time): 64 requests of 16 tokens over 4K-12K
-// keys at random slots, 64 / 8 heads of 64 (1.11 GB): 262 us, 4.2 TB/s, 0.65 of
-// the copy rate, 533 TFLOP/s; with its softmax taken out 208 us (the gather), with
+// keys at random slots, 64 / 8 heads of 64 (1.11 GB): 260-310 us over calls in a
+// row (the SM clock falls under load; 260 us the fastest, 4.2 TB/s, 0.65 of the
+// copy rate, 533 TFLOP/s); with its softmax taken out 208 us (the gather), with
 // its loads taken out 253 us (scores -> P -> P.V per tile; a unit's 128 keys take
 // about 3,900 cycles, of which 2,200 are exponentials at two warps per
-// scheduler).  Trees of 33-64 tokens over 16K-32K keys of head_dim 128: 511 us,
-// 668 TFLOP/s, 0.40 of cuBLAS bf16; a head's K/V are gathered once per two row
-// tiles, 437 us alone.  Short items are a chain of latencies, about 10,000 cycles
-// for one of one tile: 128 requests of 8 tokens and 100-140 keys in a window 45 us
-// (48 before an item's Q was handed on ahead of the epilogue before it).
-//
+// scheduler).  Trees of 33-64 tokens over 16K-32K keys of head_dim 128: 575-600 us in
+// a row, 585 TFLOP/s (510-530 us alone); a head's K/V are gathered once per two row
+// tiles, 437 us alone.  Short items are a chain of latencies: 128 requests of 8
+// tokens and 100-140 keys in a window 45-54 us, of which at most five items of
+// about 10,000 cycles in a row explain 26; what the rest is was not found.
+
 // The pieces that decide the time: 128-key tiles with one CTA per SM (64-key
 // tiles with two CTAs 342 us on the first case, 80 registers a thread spill);
 // producers that issue a copy in four instructions (29 with a 64-bit
