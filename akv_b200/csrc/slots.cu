@@ -298,9 +298,19 @@ __global__ void __launch_bounds__(kSlotThreads) map_slots_kernel(const SlotArgs 
   {
     const long long stride = (long long)gridDim.y * step;
     for (long long i = (long long)s.all_fresh + (long long)b * step + start; i < a.capacity;
-         i += stride) {
-      if (a.slots[i] >= 0) a.slots[i] = -1;
-      if (a.positions[i] > 0) a.positions[i] = 0;
+         i += 4 * stride) {
+      int slot[4], position[4];  // all loads before the first store
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool in = i + k * stride < a.capacity;
+        slot[k] = in ? a.slots[i + k * stride] : -1;
+        position[k] = in ? a.positions[i + k * stride] : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (slot[k] >= 0) a.slots[i + k * stride] = -1;
+        if (position[k] > 0) a.positions[i + k * stride] = 0;
+      }
     }
   }
 
@@ -410,10 +420,12 @@ extern "C" int akv_map_slots(const akv_map_slots_args* args, void* stream) {
              x.next_positions, x.next_is64 != 0, x.parents, x.capacity, x.new_offsets, x.slots,
              x.positions, x.tree_mask, x.block_table, x.table_stride, x.table_columns, x.totals,
              x.status, x.workspace, keep ? (int)(x.commit & 1) : x.commit != 0, keep};
-  // Blocks per request: enough for about six per SM over the batch, no more
-  // than the request's share of tokens or its table row can use.
+  // Blocks per request: enough for about six per SM over the batch, no more than its
+  // tokens, its table row or its share of the entries behind the last token can use
+  // (a capacity of 131,072, one request's tree: one block 178 us, these 5).
   const long long longest =
-      std::max<long long>(x.parents ? 1 : x.capacity, x.block_table ? x.table_columns : 1);
+      std::max<long long>(x.parents ? (x.capacity + batch - 1) / batch : x.capacity,
+                          x.block_table ? x.table_columns : 1);
   const long long want = (longest + 4 * kSlotThreads - 1) / (4 * kSlotThreads);
   const long long fit = std::max(1, kNumSMs * 6 / batch);
   const dim3 grid((unsigned)std::max<long long>(1, std::min(want, fit)), batch);

@@ -259,3 +259,20 @@ def test_rings_of_other_types_are_refused():
         setattr(ring, field, value)
         with pytest.raises(ValueError, match="free ring"):
             mapper.run(rows, one - 1, one - 1, one, ring)
+
+
+@pytest.mark.parametrize("batch", [1, 3, 90])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("spare", [1, 5, 1023, 40000])
+def test_every_entry_behind_the_last_token_of_a_large_mapper(batch, tree, spare):
+    from akv_b200.context_slots import SlotMapper
+
+    rng = np.random.default_rng(spare + batch)
+    c = case(rng, rng.integers(0, 40, batch), rng.integers(1, 9, batch), 4, tree=tree, table=True)
+    total = int(c["new"].sum())
+    mapper = SlotMapper(batch + 2, total + spare, "cuda", page_size=4)
+    mapper._slots.copy_(torch.arange(total + spare))
+    mapper._positions.copy_(torch.arange(total + spare) + 3)
+    view, t = launch(c, mapper=mapper, capacity=total + spare)
+    check(c, view, t, True)
+    assert bool((view.slots[total:] == -1).all()) and bool((view.positions[total:] == 0).all())
