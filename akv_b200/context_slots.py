@@ -110,8 +110,8 @@ class SlotMapper:
         move up; with ``keep_offsets`` it keeps its entries, without slots, which is what tokens
         need that are laid out by the caller's own lengths (a length that is itself out of range
         then refuses the call).  Two requests of one call must not share a
-        row, unless at most one of them has new tokens.  Failures that only
-        the device sees are bits of ``status`` (``SlotMap.check``)."""
+        row, unless at most one of them has new tokens and the other's columns end before them.
+        Failures that only the device sees are bits of ``status`` (``SlotMap.check``)."""
         index = self._index
         (rows_ptr, rows_dev, rows_dt, batch, rows_step, raw_ptr, raw_dev, raw_dt, n_raw, raw_step,
          new_ptr, new_dev, new_dt, n_new, new_step, free_ptr, free_dev, free_dt, free_n, free_step,

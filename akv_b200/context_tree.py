@@ -168,7 +168,8 @@ class TreeAttention:
 
     def plan(self, kv_indptr_host, draft_indptr_host):
         """Work list from the host-known CSR offsets of the cached keys and of
-        the drafted tokens (at most ``MAX_DRAFT`` per request)."""
+        the drafted tokens (at most ``MAX_DRAFT`` per request), copied on the
+        current stream: runs and replays follow it there."""
         if len(kv_indptr_host) - 1 > self.max_batch:
             raise ValueError("batch exceeds max_batch")
         items, cta_items, merges, partials = tree_work_list(

@@ -714,8 +714,9 @@ int akv_gather_slots(const int64_t* tasks, const int32_t* chunks, int32_t n_chun
  * skipped over by the requests behind it; with commit they stay in the ring,
  * as the next ones to be given out, and totals do not count them); BAD_PARENT
  * makes the token a root.  Two requests of a call must not share a row, unless
- * at most one of them has new tokens.  workspace: DEVICE uint32 [2], zero before the first call and
- * left zero by every call; calls that share it must not overlap.
+ * at most one of them has new tokens and the other's columns end before them.
+ * workspace: DEVICE uint32 [2], zero before the first call and left zero by
+ * every call; calls that share it must not overlap.
  */
 typedef struct akv_map_slots_args {
   int32_t* req_to_token;
